@@ -299,6 +299,72 @@ int lmpb_peer_size(void);
 lmpb_status lmpb_reduce_allreduce(int op, int dtype, const void* in, const int64_t* shape, int ndim, int axis,
                                   void* out, void* stream);
 
+/* ------------------------------------------- transformer training
+ *
+ * Operators of a transformer block's training step.  No counterpart in the
+ * reference, whose layers stop at Linear, activations and Softmax. */
+
+/* Layer norm over the last axis of x [rows, features], FLOAT32 or FLOAT64:
+ *   y = (x - mean) / sqrt(var + eps) * weight + bias
+ * with var the mean of (x - mean)^2.  weight and bias [features] may each be
+ * null (1 and 0).  mean and rstd [rows] receive what the backward needs, or
+ * are both null. */
+lmpb_status lmpb_layer_norm(int dtype, const void* x, const void* weight, const void* bias, int64_t rows,
+                            int64_t features, double eps, void* y, void* mean, void* rstd, void* stream);
+/* Its gradients from grad [rows, features], overwriting dx [rows, features],
+ * dweight and dbias [features]; each may be null.  The sums over rows have a
+ * fixed order: the same call gives the same bits. */
+lmpb_status lmpb_layer_norm_backward(int dtype, const void* x, const void* weight, const void* mean,
+                                     const void* rstd, const void* grad, int64_t rows, int64_t features, void* dx,
+                                     void* dweight, void* dbias, void* stream);
+
+/* Lengths of sequences packed one behind the other without padding, and the
+ * tables that the attention kernels walk, on the device that is current at
+ * the call.  Synchronous: not during a stream capture.  A length may be 0.
+ * Release the handle when no kernel or recorded graph uses it any more. */
+typedef struct lmpb_sequences_s* lmpb_sequences;
+lmpb_status lmpb_sequences_create(const int64_t* lengths, int count, lmpb_sequences* handle);
+lmpb_status lmpb_sequences_release(lmpb_sequences handle);
+
+/* Causal attention, FLOAT32: q and out [tokens, heads, head_dim], k and v
+ * [tokens, kv_heads, head_dim], lse [heads, tokens].  Token i of a sequence
+ * sees that sequence's tokens j <= i; query head h reads key/value head
+ * h / (heads / kv_heads):
+ *   out = softmax(scale * q k^T) v,  lse = log(sum(exp(scale * q k^T)))
+ * Tokens behind the last sequence get 0 (their lse is not written).
+ * head_dim <= 128, heads a multiple of kv_heads, scale > 0. */
+lmpb_status lmpb_attention(const float* q, const float* k, const float* v, float* out, float* lse, int64_t tokens,
+                           int heads, int kv_heads, int head_dim, float scale, lmpb_sequences sequences,
+                           void* stream);
+/* Its gradients from the output's gradient `grad`, overwriting dq, dk and dv.
+ * dq may be null; dk and dv may be null together.  No atomics: the same call
+ * gives the same bits. */
+lmpb_status lmpb_attention_backward(const float* q, const float* k, const float* v, const float* out,
+                                    const float* lse, const float* grad, float* dq, float* dk, float* dv,
+                                    int64_t tokens, int heads, int kv_heads, int head_dim, float scale,
+                                    lmpb_sequences sequences, void* stream);
+
+/* One tensor of an AdamW step: n values of the parameter, its gradient and
+ * its two moments. */
+typedef struct {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  int64_t n;
+} lmpb_adamw_tensor;
+/* One AdamW step over `count` tensors of one dtype (FLOAT32 or FLOAT64), in
+ * place, with t = step[0] + 1:
+ *   exp_avg = beta1 * exp_avg + (1 - beta1) * grad
+ *   exp_avg_sq = beta2 * exp_avg_sq + (1 - beta2) * grad^2
+ *   param = param * (1 - lr * weight_decay)
+ *           - lr / (1 - beta1^t) * exp_avg / (sqrt(exp_avg_sq) / sqrt(1 - beta2^t) + eps)
+ * `step` is device memory for two counts: the steps taken so far, which the
+ * call advances by one, and a counter of the kernel's own that must be 0.
+ * The tensors must not overlap. */
+lmpb_status lmpb_adamw(int dtype, const lmpb_adamw_tensor* tensors, int count, double lr, double beta1,
+                       double beta2, double eps, double weight_decay, int64_t* step, void* stream);
+
 /* ------------------------------------------------------ fused kernels */
 
 /* The lazy-fusion compiler behind capture_on / capture.  Replaces the NVRTC

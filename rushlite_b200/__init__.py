@@ -9,14 +9,15 @@ from __future__ import annotations
 
 try:
     from ._C import *  # noqa: F401,F403
-    from ._C import Variable, cuda, device, dtype  # noqa: F401
+    from ._C import Sequences, Variable, cuda, device, dtype  # noqa: F401
 except ImportError as e:  # pragma: no cover - surfaced to the user
     raise ImportError(
         "rushlite_b200 native module is not built; run `python -c 'import __graft_entry__ as g; g.build()'` "
         f"({e})") from e
 
+from . import optim
 from .capture_mode import capture, capture_on
 from .grad_mode import no_grad
 from .nets.Module import Module
 
-__all__ = ["Variable", "Module", "capture_on", "capture", "no_grad"]
+__all__ = ["Variable", "Module", "Sequences", "capture_on", "capture", "no_grad", "optim"]

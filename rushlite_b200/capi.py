@@ -45,6 +45,8 @@ EXPORTS = [
     "lmpb_gemm_f32_bias_act", "lmpb_comm_unique_id", "lmpb_comm_init", "lmpb_comm_destroy", "lmpb_comm_size",
     "lmpb_allreduce", "lmpb_comm_join", "lmpb_peer_export", "lmpb_peer_import", "lmpb_peer_close",
     "lmpb_peer_size", "lmpb_reduce_allreduce", "lmpb_gemm_sched_tile", "lmpb_gemm_sched_unit", "lmpb_gemm_sched_splits",
+    "lmpb_layer_norm", "lmpb_layer_norm_backward", "lmpb_sequences_create", "lmpb_sequences_release",
+    "lmpb_attention", "lmpb_attention_backward", "lmpb_adamw",
 ]
 COMM_ID_BYTES = 128
 
@@ -67,6 +69,11 @@ class FLeaf(C.Structure):
 class FOut(C.Structure):
     _fields_ = [("node", C.c_int32), ("mode", C.c_int32), ("dtype", C.c_int32), ("addend", C.c_int32),
                 ("ndim", C.c_int32), ("reserved", C.c_int32), ("shape", C.c_int64 * MAX_DIMS)]
+
+
+class AdamWTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
+                ("n", C.c_int64)]
 
 
 _lib = None
@@ -114,6 +121,13 @@ def lib() -> C.CDLL:
         L.lmpb_peer_close.argtypes = []
         L.lmpb_peer_size.argtypes = []
         L.lmpb_reduce_allreduce.argtypes = [i32, i32, vp, P64, i32, i32, vp, vp]
+        L.lmpb_layer_norm.argtypes = [i32, vp, vp, vp, i64, i64, d, vp, vp, vp, vp]
+        L.lmpb_layer_norm_backward.argtypes = [i32, vp, vp, vp, vp, vp, i64, i64, vp, vp, vp, vp]
+        L.lmpb_sequences_create.argtypes = [P64, i32, C.POINTER(vp)]
+        L.lmpb_sequences_release.argtypes = [vp]
+        L.lmpb_attention.argtypes = [vp] * 5 + [i64, i32, i32, i32, C.c_float, vp, vp]
+        L.lmpb_attention_backward.argtypes = [vp] * 9 + [i64, i32, i32, i32, C.c_float, vp, vp]
+        L.lmpb_adamw.argtypes = [i32, C.POINTER(AdamWTensor), i32, d, d, d, d, d, vp, vp]
         PI = C.POINTER(C.c_int)
         L.lmpb_gemm_sched_tile.argtypes = [i32, i32, i32, i32, i32, PI, PI]
         L.lmpb_gemm_sched_tile.restype = None
@@ -185,6 +199,43 @@ def copy(kind, src, src_dt, dst, dst_dt, n, stream=0):
 
 def add_inplace(dt, dst, src, n, stream=0):
     check(lib().lmpb_add_inplace(dt, dst, src, n, stream))
+
+
+def layer_norm(dt, x, weight, bias, rows, features, eps, y, mean=None, rstd=None, stream=0):
+    check(lib().lmpb_layer_norm(dt, x, weight, bias, rows, features, eps, y, mean, rstd, stream))
+
+
+def layer_norm_backward(dt, x, weight, mean, rstd, grad, rows, features, dx=None, dweight=None, dbias=None, stream=0):
+    check(lib().lmpb_layer_norm_backward(dt, x, weight, mean, rstd, grad, rows, features, dx, dweight, dbias, stream))
+
+
+class Sequences:
+    """Lengths of packed sequences (lmpb_sequences handle)."""
+
+    def __init__(self, lengths):
+        h = C.c_void_p()
+        check(lib().lmpb_sequences_create(shape_arr(lengths), len(lengths), C.byref(h)))
+        self.h = h
+
+    def __del__(self):
+        if getattr(self, "h", None) and _lib is not None:
+            _lib.lmpb_sequences_release(self.h)
+            self.h = None
+
+
+def attention(q, k, v, out, lse, tokens, heads, kv_heads, head_dim, scale, seqs, stream=0):
+    check(lib().lmpb_attention(q, k, v, out, lse, tokens, heads, kv_heads, head_dim, scale, seqs.h, stream))
+
+
+def attention_backward(q, k, v, out, lse, grad, dq, dk, dv, tokens, heads, kv_heads, head_dim, scale, seqs, stream=0):
+    check(lib().lmpb_attention_backward(q, k, v, out, lse, grad, dq, dk, dv, tokens, heads, kv_heads, head_dim, scale,
+                                        seqs.h, stream))
+
+
+def adamw(dt, tensors, lr, beta1, beta2, eps, weight_decay, step, stream=0):
+    """tensors: (param, grad, exp_avg, exp_avg_sq, n) each; step: device int64 [steps taken, 0]."""
+    ts = (AdamWTensor * max(1, len(tensors)))(*[AdamWTensor(*t) for t in tensors])
+    check(lib().lmpb_adamw(dt, ts, len(tensors), lr, beta1, beta2, eps, weight_decay, step, stream))
 
 
 class Fused:

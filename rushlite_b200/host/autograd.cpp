@@ -205,8 +205,12 @@ static void dfs(const Variable& v, std::unordered_set<void*>& seen, std::vector<
 
 // Variable::backward (csrc/src/autograd/variable.cpp:46-55): seed ones, apply
 // every recorded function in reverse topological order.
-void Variable::backward() {
+void Variable::backward(const Tensor* seed) {
   LMP_CHECK(requires_grad(), "Must be declared with requires_grad");
+  if (seed)
+    LMP_CHECK(seed->shape() == impl_->data.shape() && seed->type() == impl_->data.type() &&
+                  seed->device() == impl_->data.device(),
+              "backward: the gradient must have the Variable's shape, dtype and device");
   std::vector<Variable> topo;
   std::unordered_set<void*> seen;
   dfs(*this, seen, topo);
@@ -234,7 +238,12 @@ void Variable::backward() {
     copies.push_back(node.grad_slot().impl());
   }
   if (!copies.empty()) tensor::realize_all(copies);
-  impl_->grad = tensor::ones_like(impl_->grad);
+  if (seed) {
+    impl_->grad = *seed;
+    impl_->grad_shared = true;  // the caller's tensor: copied before it is updated in place
+  } else {
+    impl_->grad = tensor::ones_like(impl_->grad);
+  }
   {
     tensor::lazy::CaptureGuard cap(true);
     for (Variable& node : topo)

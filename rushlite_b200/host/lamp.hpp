@@ -213,6 +213,8 @@ class Graph {
   void replay();
   size_t kernels() const { return kernels_; }  // kernel nodes in the graph
   void defer_free(void* p) { deferred_.push_back(p); }
+  // Keeps what the recorded kernels read alive until the Graph is destroyed.
+  void keep(std::shared_ptr<void> p) { kept_.push_back(std::move(p)); }
   const std::shared_ptr<bool>& live() const { return live_; }
 
  private:
@@ -223,9 +225,24 @@ class Graph {
   bool capturing_ = false;
   size_t kernels_ = 0;
   std::vector<void*> deferred_;
+  std::vector<std::shared_ptr<void>> kept_;
   std::shared_ptr<bool> live_;
 };
 Graph* capturing_graph();
+
+// Lengths of sequences packed one behind the other along a tensor's first
+// dimension, with the device tables that the attention kernels walk
+// (lmpb_sequences).  Made once per batch shape, outside a capture; a recorded
+// graph that uses it keeps it.
+struct Sequences {
+  explicit Sequences(const std::vector<int64_t>& lengths);
+  ~Sequences();
+  Sequences(const Sequences&) = delete;
+  Sequences& operator=(const Sequences&) = delete;
+  std::vector<int64_t> lengths;
+  int64_t tokens = 0;
+  lmpb_sequences handle = nullptr;
+};
 
 namespace ops {
 Tensor add(const Tensor& a, const Tensor& b);
@@ -330,7 +347,9 @@ class Variable {
   void copy(const Variable& other);
   void fill(Scalar item);
   void realize();
-  void backward();
+  // Seeds this Variable's gradient with ones, or with `seed` (same shape,
+  // dtype and device), and applies every recorded function.
+  void backward(const Tensor* seed = nullptr);
   bool defined() const { return impl_ != nullptr; }
   const std::shared_ptr<VariableImpl>& impl() const { return impl_; }
   // raw gradient slot (for the optimizer / gemm accumulation)
@@ -377,7 +396,21 @@ Variable reshape(const Variable& a, const std::vector<size_t>& shape);
 Variable squeeze(const Variable& a, size_t axis);
 Variable expand_dims(const Variable& a, size_t axis);
 Variable to(const Variable& a, DeviceType device);
+
+// Layer norm over the last dimension; weight and bias [features] may each be null.
+Variable layer_norm(const Variable& x, const Variable* weight, const Variable* bias, Scalar eps);
+// Causal attention within each of the packed sequences: q [tokens, heads,
+// head_dim], k and v [tokens, kv_heads, head_dim].  scale: null for
+// 1 / sqrt(head_dim).  Tokens behind the last sequence give 0.
+Variable causal_attention(const Variable& q, const Variable& k, const Variable& v,
+                          const std::shared_ptr<tensor::Sequences>& sequences, const Scalar* scale);
 }  // namespace ops
+
+// One AdamW step in place over all parameters, in one launch (lmpb_adamw).
+// step: int64 [2], the steps taken so far and a counter of the kernel's.
+void adamw_step(const std::vector<Variable>& params, const std::vector<Tensor>& exp_avg,
+                const std::vector<Tensor>& exp_avg_sq, const Tensor& step, Scalar lr, Scalar beta1, Scalar beta2,
+                Scalar eps, Scalar weight_decay);
 
 Variable zeros(const std::vector<size_t>& shape, bool requires_grad, DeviceType device, DataType dtype);
 Variable ones(const std::vector<size_t>& shape, bool requires_grad, DeviceType device, DataType dtype);

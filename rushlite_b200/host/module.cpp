@@ -10,6 +10,7 @@
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
+#include <optional>
 #include <random>
 
 #include "lamp.hpp"
@@ -280,7 +281,10 @@ PYBIND11_MODULE(_C, m) {
       .def_property_readonly("device", [](const Variable& v) { return v.data().device(); })
       .def_property_readonly("dtype", [](const Variable& v) { return v.data().type(); })
       .def_property_readonly("ndim", [](const Variable& v) { return v.data().shape().size(); })
-      .def("backward", &Variable::backward, py::call_guard<py::gil_scoped_release>())
+      .def("backward", [](Variable& v, const Variable* grad) { v.backward(grad ? &grad->data() : nullptr); },
+           py::arg("grad") = py::none(), py::call_guard<py::gil_scoped_release>(),
+           "Seeds this Variable's gradient with ones, or with `grad` (same shape, dtype and device), and "
+           "accumulates the gradients of everything it was computed from.")
       .def("tolist", [](const Variable& v) { return v.data().to_vector(); })
       .def("numpy", [](const Variable& v, py::object out) { return to_numpy(v.data(), out); }, py::arg("out") = py::none())
       .def("zero_grad", &Variable::zero_grad)
@@ -372,6 +376,31 @@ PYBIND11_MODULE(_C, m) {
   m.def("squeeze", &aops::squeeze, py::arg("a"), py::arg("axis"));
   m.def("expand_dims", &aops::expand_dims, py::arg("a"), py::arg("axis"));
   m.def("to", &aops::to, py::arg("a"), py::arg("device"));
+
+  // operators of a transformer's training step
+  py::class_<lmp::tensor::Sequences, std::shared_ptr<lmp::tensor::Sequences>>(
+      m, "Sequences",
+      "Lengths of sequences packed one behind the other along a tensor's first dimension, without padding.  Make it "
+      "once per batch shape, outside a CUDA-graph capture, on the device that will use it.")
+      .def(py::init<const std::vector<int64_t>&>(), py::arg("lengths"))
+      .def_property_readonly("lengths", [](const lmp::tensor::Sequences& s) { return s.lengths; })
+      .def_property_readonly("tokens", [](const lmp::tensor::Sequences& s) { return s.tokens; });
+  m.def("layer_norm", [](const Variable& x, const Variable* weight, const Variable* bias, Scalar eps) {
+        return aops::layer_norm(x, weight, bias, eps);
+      }, py::arg("x"), py::arg("weight") = py::none(), py::arg("bias") = py::none(), py::arg("eps") = 1e-5,
+      "(x - mean) / sqrt(var + eps) * weight + bias over the last dimension; weight and bias [features] or None.  "
+      "float32 or float64.");
+  m.def("causal_attention",
+      [](const Variable& q, const Variable& k, const Variable& v,
+         const std::shared_ptr<lmp::tensor::Sequences>& sequences, std::optional<Scalar> scale) {
+        return aops::causal_attention(q, k, v, sequences, scale ? &*scale : nullptr);
+      }, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("sequences"), py::arg("scale") = py::none(),
+      "softmax(scale * q k^T) v within each packed sequence, token i seeing tokens j <= i.  q [tokens, heads, "
+      "head_dim], k and v [tokens, kv_heads, head_dim], float32, head_dim <= 128; query head h reads key/value head "
+      "h // (heads // kv_heads).  scale: 1 / sqrt(head_dim) by default.  Tokens behind the last sequence give 0.");
+  m.def("adamw_step", &lmp::autograd::adamw_step, py::arg("params"), py::arg("exp_avg"), py::arg("exp_avg_sq"),
+        py::arg("step"), py::arg("lr"), py::arg("beta1"), py::arg("beta2"), py::arg("eps"), py::arg("weight_decay"),
+        "One AdamW step in place over all parameters in one launch; step: int64 [steps taken, 0].  See optim.AdamW.");
 
   // tensor-level kernels without autograd (the stub-level API)
   m.def("abs_backward", &tops::abs_backward, py::arg("input"), py::arg("grad"));

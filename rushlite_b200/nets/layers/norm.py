@@ -1,0 +1,23 @@
+from ... import _C
+from ..Module import Module
+
+
+class LayerNorm(Module):
+    """y = (x - mean) / sqrt(var + eps) * weights + bias over the last
+    dimension; weights start at 1, bias at 0."""
+
+    def __init__(self, features: int, eps: float = 1e-5, bias: bool = True, device=None, dtype=None) -> None:
+        super().__init__()
+        kw = {}
+        if device is not None:
+            kw["device"] = device
+        if dtype is not None:
+            kw["dtype"] = dtype
+        object.__setattr__(self, "eps", eps)
+        object.__setattr__(self, "requires_bias", bias)
+        self.weights = _C.ones([features], requires_grad=True, **kw)
+        if bias:
+            self.bias = _C.zeros([features], requires_grad=True, **kw)
+
+    def forward(self, x):
+        return _C.layer_norm(x, self.weights, self.bias if self.requires_bias else None, self.eps)

@@ -1,0 +1,404 @@
+"""Causal attention over packed sequences against the formula in 64 bits, its
+gradients against differences, and its refusals.
+
+Tolerances, per element, from what is added (magnitudes M below):
+* a score is a sum of D products.  On the tensor cores each operand is two
+  fp16 parts, together within 2^-22 of it, and the product of the two small
+  parts is left out (2^-22): 3 * 2^-22 of each product; the accumulator may
+  lose a step of 2^-23 of the sum of magnitudes at each addition of a product,
+  D * 2^-23 at most.  Plain fp32 loses at most D * 2^-24.  So a score is within
+  E = (3 + D / 2) * 2^-22 * scale * |q| . |k|.
+* a weight P is exp of a difference of two such scores (or score and lse, whose
+  value is rounded to fp32): within 2 E + 2^-23 |lse| + 2^-21 of itself.
+* what sums weights times values has the same 3 * 2^-22 a product, and at most
+  2^-23 a product and block of additions that follow one another: L 2^-23.
+Each bound is the sum of these times the magnitudes added, in 64 bits."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+CASES = [  # lengths, heads, kv_heads, head_dim, rows behind the last sequence
+    ([1], 1, 1, 1, 0), ([7], 4, 4, 64, 0), ([1, 2, 3, 0, 5], 2, 1, 8, 2), ([63, 64, 65], 4, 2, 33, 0),
+    ([128, 127, 129, 1], 4, 1, 128, 5), ([300, 17, 513], 6, 2, 80, 0), ([0, 0], 2, 2, 16, 3), ([], 2, 1, 4, 4),
+    ([1030], 3, 3, 96, 1), ([255, 256, 257], 8, 1, 16, 0), ([2049], 4, 2, 128, 0), ([1500, 31, 700, 1], 4, 2, 64, 0),
+    ([1] * 40, 3, 1, 31, 0), ([640] * 3, 2, 2, 65, 130),
+]
+
+
+def _inputs(torch, rng, case, scale=1.0):
+    lengths, hq, hkv, d, tail = case
+    t = sum(lengths) + tail
+    x = {"q": (t, hq, d), "k": (t, hkv, d), "v": (t, hkv, d), "g": (t, hq, d)}
+    x = {n: torch.from_numpy((rng.standard_normal(s) * scale).astype(np.float32)) for n, s in x.items()}
+    if tail:  # rows of no sequence: never read
+        for a in x.values():
+            a[t - tail:] = math.nan
+    return x
+
+
+def _reference(torch, x, lengths, scale=None):
+    """{name: (value, tolerance)}, rows behind the last sequence 0."""
+    x = {n: a.cuda().double() for n, a in x.items()}
+    q, k, v, g = (x[n] for n in "qkvg")
+    t, hq, d = q.shape
+    hkv = k.shape[1]
+    scale = 1 / math.sqrt(d) if scale is None else scale
+    zero = lambda a: [torch.zeros_like(a), torch.zeros_like(a)]  # noqa: E731
+    out = {"out": zero(q), "dq": zero(q), "dk": zero(k), "dv": zero(v)}
+    w = 2.0 ** -22
+    start = 0
+    for n in lengths:
+        rows = slice(start, start + n)
+        start += n
+        if n == 0:
+            continue
+        for h in range(hq):
+            j = h * hkv // hq
+            Q, K, V, G = q[rows, h], k[rows, j], v[rows, j], g[rows, h]
+            mask = torch.ones(n, n, dtype=torch.bool, device="cuda").tril()
+            S = (scale * Q @ K.T).masked_fill(~mask, -math.inf)
+            lse = torch.logsumexp(S, 1, keepdim=True)
+            P = torch.exp(S - lse)
+            E = ((3 + d / 2) * w * scale * (Q.abs() @ K.abs().T)).masked_fill(~mask, 0)
+            rel = 2 * E.amax(1, keepdim=True) + w * (lse.abs() / 2 + 2)  # of a weight
+            sums = (3 + n / 2) * w
+            O = P @ V
+            out["out"][0][rows, h], out["out"][1][rows, h] = O, (rel + sums) * (P @ V.abs())
+            dP = G @ V.T
+            delta = (G * O).sum(1, keepdim=True)
+            dS = P * (dP - delta)
+            # dP and delta: D products each, delta with the output's own error
+            size = (G.abs() @ V.abs().T) + (G.abs() * (P @ V.abs())).sum(1, keepdim=True)
+            dSt = (rel + (3 + d / 2) * w + sums) * P * size + rel * dS.abs()
+            dSm = P * size
+            out["dq"][0][rows, h] = scale * dS @ K
+            out["dq"][1][rows, h] = scale * (dSt @ K.abs() + sums * (dSm @ K.abs()))
+            out["dk"][0][rows, j] += scale * dS.T @ Q
+            out["dk"][1][rows, j] += scale * (dSt.T @ Q.abs() + sums * (dSm.T @ Q.abs()))
+            out["dv"][0][rows, j] += P.T @ G
+            out["dv"][1][rows, j] += (rel * P).T @ G.abs() + sums * (P.T @ G.abs())
+    return {n: (a.cpu().numpy(), b.cpu().numpy()) for n, (a, b) in out.items()}
+
+
+def _check(name, got, ref):
+    want, tol = ref
+    assert got.shape == want.shape, name
+    assert np.isfinite(got).all(), (name, np.argwhere(~np.isfinite(got))[:3])
+    worst = np.abs(got - want) - tol - 1e-37
+    assert (worst <= 0).all(), (name, np.argwhere(worst > 0)[:3], float(worst.max()))
+
+
+def _run(rsl, x, lengths, scale=None, seqs=None):
+    var = {n: rsl.Variable(x[n].numpy(), n != "g") for n in "qkvg"}
+    o = rsl.causal_attention(var["q"], var["k"], var["v"], seqs or rsl.Sequences(lengths), scale)
+    o.backward(var["g"])
+    return {"out": o.numpy(), **{"d" + n: var[n].grad.numpy() for n in "qkv"}}
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "%s-%d-%d-%d-%d" % ("_".join(map(str, c[0][:5])), *c[1:]))
+def test_forward_and_backward(cuda, case):
+    import rushlite_b200 as rsl
+
+    x = _inputs(cuda, np.random.default_rng(sum(case[0]) + case[3]), case)
+    got = _run(rsl, x, case[0])
+    ref = _reference(cuda, x, case[0])
+    for name in got:
+        _check(name, got[name], ref[name])
+    # and as a whole, for inputs of unit size, where roundings average out: 2^-18 (forward) and 2^-17
+    for name in got:
+        norm = np.linalg.norm(ref[name][0])
+        if norm > 1e-3 * np.linalg.norm(ref[name][1]) / 2.0 ** -22:
+            assert np.linalg.norm(got[name] - ref[name][0]) <= 2.0 ** (-18 if name == "out" else -17) * norm, name
+
+
+@pytest.mark.parametrize("scale", [1e-3, 0.7, 3.0])
+def test_scale(cuda, scale):
+    import rushlite_b200 as rsl
+
+    case = ([200, 9], 2, 1, 40, 0)
+    x = _inputs(cuda, np.random.default_rng(7), case)
+    got, ref = _run(rsl, x, case[0], scale), _reference(cuda, x, case[0], float(np.float32(scale)))
+    for name in got:
+        _check(name, got[name], ref[name])
+
+
+@pytest.mark.parametrize("size", [1e-20, 1e-6, 30.0])
+def test_sizes_of_values(cuda, size):
+    """Products of tiny values underflow to 0, which the formula's are too within fp32's smallest steps."""
+    import rushlite_b200 as rsl
+
+    case = ([300, 40], 2, 2, 64, 0)
+    x = _inputs(cuda, np.random.default_rng(8), case, size)
+    if size == 1e-20:  # gradients of it underflow: the forward alone
+        got = rsl.causal_attention(*(rsl.Variable(x[n].numpy()) for n in "qkv"), rsl.Sequences(case[0])).numpy()
+        return _check("out", got, _reference(cuda, x, case[0])["out"])
+    got, ref = _run(rsl, x, case[0]), _reference(cuda, x, case[0])
+    for name in got:
+        _check(name, got[name], ref[name])
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, 3e38, 1e30])
+@pytest.mark.parametrize("dim", [48, 128])
+def test_what_a_row_does_not_see_does_not_reach_it(cuda, bad, dim):
+    """Values behind the diagonal, in another sequence and in another group's
+    heads: rows before them and the other heads keep results within tolerance."""
+    import rushlite_b200 as rsl
+
+    lengths, t = [400, 300, 5], 705
+    x = _inputs(cuda, np.random.default_rng(9), (lengths, 4, 2, dim, 0))
+    ref = _reference(cuda, x, lengths)
+    p = 190  # in the first sequence
+    x["k"][p, 1, 3] = bad
+    x["v"][p + 1, 1, 0] = bad
+    got = {n: a for n, a in _run(rsl, x, lengths).items()}
+    for name in ("out", "dq"):  # group 0's heads; group 1's rows of the first sequence before p; the other sequences
+        for rows, heads in ((slice(0, t), slice(0, 2)), (slice(0, p), slice(2, 4)), (slice(400, t), slice(2, 4))):
+            _check(name, got[name][rows, heads], tuple(a[rows, heads] for a in ref[name]))
+    for name in ("dk", "dv"):  # keys of group 1's first sequence hear from rows behind p
+        for rows, heads in ((slice(0, t), slice(0, 1)), (slice(400, t), slice(1, 2))):
+            _check(name, got[name][rows, heads], tuple(a[rows, heads] for a in ref[name]))
+    if not math.isfinite(bad):
+        assert not np.isfinite(got["out"][p + 1:400, 2:]).any(axis=-1).all()
+    # a query's own values reach its row alone, and the keys it sees
+    x = _inputs(cuda, np.random.default_rng(9), (lengths, 4, 2, dim, 0))
+    x["q"][p, 3, 1] = bad
+    x["g"][p, 3, 2] = bad
+    got = _run(rsl, x, lengths)
+    keep = np.ones(t, bool)
+    keep[p] = False
+    for name in ("out", "dq"):
+        _check(name, got[name][keep], tuple(a[keep] for a in ref[name]))
+    for name in ("dk", "dv"):
+        _check(name, got[name][:, 0], tuple(a[:, 0] for a in ref[name]))
+        _check(name, got[name][p + 1:, 1], tuple(a[p + 1:, 1] for a in ref[name]))
+
+
+def test_a_score_of_minus_infinity_has_no_weight(cuda):
+    import rushlite_b200 as rsl
+
+    lengths = [150]
+    x = _inputs(cuda, np.random.default_rng(10), (lengths, 1, 1, 32, 0))
+    x["q"][:, :, 0] = 1.0
+    x["k"][70, 0, 0] = -math.inf
+    got = rsl.causal_attention(*(rsl.Variable(x[n].numpy()) for n in "qkv"), rsl.Sequences(lengths)).numpy()
+    want = _reference(cuda, {**x, "k": x["k"].clone().nan_to_num_(neginf=-1e30)}, lengths)["out"]
+    want = (want[0], _reference(cuda, {**x, "k": x["k"].clone().nan_to_num_(neginf=0.0)}, lengths)["out"][1])
+    _check("out", got, want)
+
+
+def test_lowest_values_as_a_mask(cuda):
+    """A program that masks keys by fp32's lowest value in k: those keys weigh nothing."""
+    import rushlite_b200 as rsl
+
+    lengths = [260]
+    x = _inputs(cuda, np.random.default_rng(11), (lengths, 2, 1, 64, 0))
+    x["q"][:, :, 0] = 1.0
+    x["k"][100:180, 0] = 0.0
+    x["k"][100:180, 0, 0] = float(np.finfo(np.float32).min)
+    got = _run(rsl, x, lengths)
+    soft = {**x, "k": x["k"].clone()}
+    soft["k"][100:180, 0, 0] = -1e4
+    ref, tol = _reference(cuda, soft, lengths), _reference(cuda, {**x, "k": x["k"].clone().clamp_(min=-50)}, lengths)
+    for name in ("out", "dv"):
+        _check(name, got[name], (ref[name][0], tol[name][1]))
+
+
+def test_gradients_are_the_differences(cuda):
+    """A directional difference of the formula in 64 bits; its own error is
+    h^2 times a third derivative of terms of size 1, below 1e-6 here."""
+    import rushlite_b200 as rsl
+
+    torch = cuda
+    lengths = [90, 200]
+    x = _inputs(torch, np.random.default_rng(12), (lengths, 4, 2, 24, 0))
+    got = _run(rsl, x, lengths)
+    ref = _reference(torch, x, lengths)
+    h = 1e-4
+    for n in "qkv":
+        d = torch.randn(x[n].shape, dtype=torch.float64)
+        value = [float((torch.from_numpy(_reference(torch, {**x, n: x[n].double() + s * h * d}, lengths)["out"][0])
+                        * x["g"].double()).sum()) for s in (1, -1)]
+        slope = (value[0] - value[1]) / (2 * h)
+        mine = float((torch.from_numpy(got["d" + n]).double() * d).sum())
+        room = float((torch.from_numpy(ref["d" + n][1]) * d.abs()).sum()) + 1e-6 * float(x["g"].abs().sum())
+        assert abs(mine - slope) <= room, n
+
+
+def test_repeats_to_the_bit_and_accumulates(cuda):
+    import rushlite_b200 as rsl
+
+    lengths = [700, 129]
+    x = _inputs(cuda, np.random.default_rng(13), (lengths, 4, 1, 64, 0))
+    seqs = rsl.Sequences(lengths)
+    assert seqs.lengths == lengths and seqs.tokens == 829
+    a, b = _run(rsl, x, lengths, seqs=seqs), _run(rsl, x, lengths, seqs=seqs)
+    assert all((a[n] == b[n]).all() for n in a)
+    var = {n: rsl.Variable(x[n].numpy(), n != "g") for n in "qkvg"}
+    for _ in range(2):
+        rsl.causal_attention(var["q"], var["k"], var["v"], seqs).backward(var["g"])
+    for n in "qkv":
+        assert (var[n].grad.numpy() == a["d" + n] + a["d" + n]).all()
+
+
+def test_gradients_of_some_inputs(cuda):
+    import rushlite_b200 as rsl
+
+    lengths = [200]
+    x = _inputs(cuda, np.random.default_rng(14), (lengths, 2, 2, 64, 0))
+    full = _run(rsl, x, lengths)
+    for want in ("q", "k", "v", "qv"):
+        var = {n: rsl.Variable(x[n].numpy(), n in want) for n in "qkvg"}
+        rsl.causal_attention(var["q"], var["k"], var["v"], rsl.Sequences(lengths)).backward(var["g"])
+        for n in want:
+            assert (var[n].grad.numpy() == full["d" + n]).all(), (want, n)
+    with rsl.no_grad():
+        assert not rsl.causal_attention(*(rsl.Variable(x[n].numpy(), True) for n in "qkv"), rsl.Sequences(lengths)).requires_grad
+
+
+def test_one_variable_in_all_places(cuda):
+    import rushlite_b200 as rsl
+
+    lengths = [140, 3]
+    x = _inputs(cuda, np.random.default_rng(15), (lengths, 2, 2, 32, 0))
+    x["k"] = x["v"] = x["q"]
+    ref = _reference(cuda, x, lengths)
+    q, g = rsl.Variable(x["q"].numpy(), True), rsl.Variable(x["g"].numpy())
+    rsl.causal_attention(q, q, q, rsl.Sequences(lengths)).backward(g)
+    total, tol = (sum(ref[n][i] for n in ("dq", "dk", "dv")) for i in (0, 1))
+    _check("sum", q.grad.numpy(), (total, tol + 2.0 ** -22 * (sum(np.abs(ref[n][0]) for n in ("dq", "dk", "dv")))))
+
+
+def test_other_streams_and_sequences_outlive_their_handle(cuda):
+    import rushlite_b200 as rsl
+
+    torch = cuda
+    lengths = [300, 200]
+    x = _inputs(torch, np.random.default_rng(16), (lengths, 2, 1, 64, 0))
+    want = _run(rsl, x, lengths)
+    s = torch.cuda.Stream()
+    try:
+        rsl.cuda.set_stream(s.cuda_stream)
+        got = _run(rsl, x, lengths)
+        var = {n: rsl.Variable(x[n].numpy(), n != "g") for n in "qkvg"}
+        graph, seqs = rsl.cuda.Graph(), rsl.Sequences(lengths)
+        with graph:
+            o = rsl.causal_attention(var["q"], var["k"], var["v"], seqs)
+            o.backward(var["g"])
+        del seqs  # the graph keeps it
+        junk = [rsl.Sequences([5] * 50) for _ in range(4)]
+        graph.replay()
+        rec = {"out": o.numpy(), **{"d" + n: var[n].grad.numpy() for n in "qkv"}}
+        del junk
+    finally:
+        rsl.cuda.synchronize()
+        rsl.cuda.set_stream(0)
+    for name in want:
+        assert (got[name] == want[name]).all() and (rec[name] == want[name]).all(), name
+
+
+def test_two_graphs_in_turn(cuda):
+    """Each recorded call has a workspace of its own."""
+    import rushlite_b200 as rsl
+
+    recs = []
+    for seed, lengths in ((17, [400]), (18, [130, 260])):
+        x = _inputs(cuda, np.random.default_rng(seed), (lengths, 2, 2, 64, 0))
+        want = _run(rsl, x, lengths)
+        var = {n: rsl.Variable(x[n].numpy(), n != "g") for n in "qkvg"}
+        g, seqs = rsl.cuda.Graph(), rsl.Sequences(lengths)
+        with g:
+            o = rsl.causal_attention(var["q"], var["k"], var["v"], seqs)
+            o.backward(var["g"])
+        recs.append((g, o, var, want))
+    for _ in range(3):
+        for g, *_ in recs:
+            g.replay()
+    for g, o, var, want in recs:
+        g.replay()
+        assert (o.numpy() == want["out"]).all()
+        for n in "qkv":
+            assert (var[n].grad.numpy() == want["d" + n]).all(), n
+
+
+def test_offsets_past_32_bits(cuda):
+    """q, out and their gradients hold over 2^31 values."""
+    from rushlite_b200 import capi
+
+    torch = cuda
+    heads, d, n, count = 256, 128, 300, 220
+    t = n * count
+    assert t * heads * d > 2 ** 31
+    if torch.cuda.mem_get_info()[0] < 90 << 30:
+        pytest.skip("not enough free memory")
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q, g = (torch.randn(t, heads, d, device="cuda", generator=gen) for _ in range(2))
+    k, v = (torch.randn(t, 1, d, device="cuda", generator=gen) for _ in range(2))
+    out, dq = torch.empty_like(q), torch.empty_like(q)
+    dk, dv, lse = torch.empty_like(k), torch.empty_like(v), torch.empty(heads, t, device="cuda")
+    seqs = capi.Sequences([n] * count)
+    args = (t, heads, 1, d, 1 / math.sqrt(d), seqs)
+    ptr = lambda *ts: [a.data_ptr() for a in ts]  # noqa: E731
+    capi.attention(*ptr(q, k, v, out, lse), *args)
+    capi.attention_backward(*ptr(q, k, v, out, lse, g, dq, dk, dv), *args)
+    torch.cuda.synchronize()
+    for i in (0, count - 1):
+        rows = slice(i * n, (i + 1) * n)
+        ref = _reference(torch, {"q": q[rows].cpu(), "k": k[rows].cpu(), "v": v[rows].cpu(), "g": g[rows].cpu()}, [n])
+        for name, a in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+            _check(name, a[rows].cpu().numpy(), ref[name])
+
+
+def test_unaligned_buffers_through_the_c_entry(cuda):
+    from rushlite_b200 import capi
+
+    torch = cuda
+    lengths, hq, hkv, d = [150, 40], 2, 1, 64
+    x = _inputs(torch, np.random.default_rng(19), (lengths, hq, hkv, d, 0))
+    t = sum(lengths)
+
+    def off(a):
+        b = torch.full((a.numel() + 2,), 7.0, device="cuda")
+        b[1:-1] = a.reshape(-1).cuda()
+        return b
+
+    ins = {n: off(a) for n, a in x.items()}
+    outs = {n: off(torch.zeros_like(x[s])) for n, s in (("out", "q"), ("dq", "q"), ("dk", "k"), ("dv", "v"))}
+    lse = torch.empty(hq * t + 1, device="cuda")
+    p = {n: b[1:].data_ptr() for n, b in {**ins, **outs, "lse": lse}.items()}
+    args = (t, hq, hkv, d, 1 / math.sqrt(d), capi.Sequences(lengths))
+    capi.attention(p["q"], p["k"], p["v"], p["out"], p["lse"], *args)
+    capi.attention_backward(p["q"], p["k"], p["v"], p["out"], p["lse"], p["g"], p["dq"], p["dk"], p["dv"], *args)
+    torch.cuda.synchronize()
+    ref = _reference(torch, x, lengths)
+    for n, b in outs.items():
+        _check(n, b[1:-1].cpu().numpy().reshape(ref[n][0].shape), ref[n])
+        assert b[0] == 7 and b[-1] == 7, n
+
+
+def test_refusals(cuda):
+    import rushlite_b200 as rsl
+
+    q, kv, s = rsl.ones([6, 4, 8]), rsl.ones([6, 2, 8]), rsl.Sequences([2, 4])
+    bad = [((rsl.ones([6, 4, 8], dtype=rsl.dtype.float64), kv, kv, s), "float32"),
+           ((rsl.ones([6, 4, 8], device=rsl.device.cpu), kv, kv, s), "CUDA"), ((rsl.ones([6, 32]), kv, kv, s), "head_dim"),
+           ((q, kv, rsl.ones([6, 2, 4]), s), "same shape"), ((q, rsl.ones([6, 3, 8]), rsl.ones([6, 3, 8]), s), "multiple"),
+           ((q, rsl.ones([5, 2, 8]), rsl.ones([5, 2, 8]), s), "tokens"), ((q, kv, kv, rsl.Sequences([7])), "tokens"),
+           ((rsl.ones([6, 2, 129]),) * 3 + (s,), "128"), ((q, kv, kv, s, 0.0), "scale"), ((q, kv, kv, s, -1.0), "scale"),
+           ((q, kv, kv, s, float("nan")), "scale"), ((q, kv, kv, s, float("inf")), "scale")]
+    for args, text in bad:
+        with pytest.raises(RuntimeError, match=text):
+            rsl.causal_attention(*args)
+    with pytest.raises(RuntimeError, match="negative"):
+        rsl.Sequences([3, -1])
+    g = rsl.cuda.Graph()
+    with pytest.raises(RuntimeError, match="before the capture"):
+        with g:
+            rsl.Sequences([3])
+    with pytest.raises(TypeError):
+        rsl.causal_attention(q, kv, kv, [2, 4])
+    assert rsl.causal_attention(q, kv, kv, s).shape == [6, 4, 8]  # still usable
