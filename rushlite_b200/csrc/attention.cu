@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <numeric>
 #include <vector>
 
@@ -128,22 +129,49 @@ __device__ __forceinline__ float over16(float v, bool maximum) {
   return v;
 }
 
-// Whether this CTA has anything to do: always without flags; with them, if
-// any tile of the sequence, in any head plane of the group, is flagged.
-// Planes: query heads, then key heads, value heads and (backward) gradient heads.
+// Flagged tiles.  Planes: query heads, then key heads, value heads and
+// (backward) gradient heads.
+__device__ __forceinline__ bool any_flag(const AttentionArgs& a) {
+  if (!a.flags) return true;
+  const int64_t n = ((int64_t)(a.grad ? 2 : 1) * a.heads + 2 * a.kv_heads) * a.tiles;
+  unsigned any = 0;
+  for (int64_t i = threadIdx.x; i < n / 16; i += kThreads) {  // the array starts on a 16-byte boundary
+    const uint4 f = reinterpret_cast<const uint4*>(a.flags)[i];
+    any |= f.x | f.y | f.z | f.w;
+  }
+  for (int64_t i = n / 16 * 16 + threadIdx.x; i < n; i += kThreads) any |= a.flags[i];
+  return __syncthreads_or(any != 0) != 0;
+}
+
+// Whether the sequence of tile t needs this group of heads computed: always
+// without flags; with them, if any of its tiles in any of the group's planes is flagged.
 __device__ __forceinline__ bool wanted(const AttentionArgs& a, const int4& t, int kv_head) {
   if (!a.flags) return true;
   const int n = (t.y + kTileRows - 1) / kTileRows, g = a.heads / a.kv_heads;
   const int planes = a.grad ? 2 * g + 2 : g + 2;
   int any = 0;
-  for (int i = threadIdx.x; i < n * planes; i += kThreads) {
-    const int p = i / n;
+  for (int64_t i = threadIdx.x; i < (int64_t)n * planes; i += kThreads) {
+    const int p = (int)(i / n);
     const int plane = p < g          ? kv_head * g + p
                       : p < g + 2    ? a.heads + (p - g) * a.kv_heads + kv_head
                                      : a.heads + 2 * a.kv_heads + kv_head * g + (p - g - 2);
     any |= a.flags[(int64_t)plane * a.tiles + t.w + i % n];
   }
   return __syncthreads_or(any) != 0;
+}
+
+// Calls body(tile, first row, head) for this CTA's 64-row half tiles: heads
+// of one half tile next to each other, those with the most work first.
+template <typename F>
+__device__ __forceinline__ void for_halves(const AttentionArgs& a, const int* order, int heads, F body) {
+  if (!any_flag(a)) return;
+  const int64_t items = 2 * (int64_t)a.tiles * heads;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t i = item / heads;
+    const int4 t = a.tile[order[i >> 1]];
+    const int row0 = t.z * kTileRows + (int)(i & 1) * kB, head = (int)(item % heads);
+    if (row0 < t.y && wanted(a, t, head / (heads / a.kv_heads))) body(t, row0, head);
+  }
 }
 
 template <int DP>
@@ -158,64 +186,62 @@ template <int DP>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const AttentionArgs a, bool vec) {
   extern __shared__ __align__(16) unsigned char raw[];
   ForwardSmem<DP>& s = *reinterpret_cast<ForwardSmem<DP>*>(raw);
-  const int4 t = a.tile[a.by_queries[blockIdx.x >> 1]];
-  const int q0 = t.z * kTileRows + (blockIdx.x & 1) * kB;
-  if (q0 >= t.y) return;
-  const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
-  if (!wanted(a, t, kv_head)) return;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const float c = a.scale * kLog2e;
-  load_tile<DP>(s.q, a.q, t.x + q0, t.y - q0, a.heads, head, a.dim, vec);
-  float acc[4][DP / 16] = {}, m[4], l[4] = {};
+  for_halves(a, a.by_queries, a.heads, [&](const int4& t, int q0, int head) {
+    const int kv_head = head / (a.heads / a.kv_heads);
+    load_tile<DP>(s.q, a.q, t.x + q0, t.y - q0, a.heads, head, a.dim, vec);
+    float acc[4][DP / 16] = {}, m[4], l[4] = {};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) m[i] = -INFINITY;
-  for (int k0 = 0; k0 <= q0; k0 += kB) {
-    const bool diag = k0 == q0;
-    load_tile<DP>(s.kv, a.k, t.x + k0, t.y - k0, a.kv_heads, kv_head, a.dim, vec);
-    __syncthreads();
-    float z[4][4];
-    dot_tile<DP>(s.q, s.kv, ty, tx, z);
+    for (int i = 0; i < 4; ++i) m[i] = -INFINITY;
+    for (int k0 = 0; k0 <= q0; k0 += kB) {
+      const bool diag = k0 == q0;
+      load_tile<DP>(s.kv, a.k, t.x + k0, t.y - k0, a.kv_heads, kv_head, a.dim, vec);
+      __syncthreads();
+      float z[4][4];
+      dot_tile<DP>(s.q, s.kv, ty, tx, z);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool see = !diag || tx + 16 * j <= 4 * ty + i;
+          z[i][j] = see ? z[i][j] * c : -INFINITY;
+          mx = fmaxf(mx, z[i][j]);  // drops a NaN: exp2f below keeps it in the row's sum
+        }
+        const float mn = fmaxf(m[i], over16(mx, true));
+        const float base = mn == -INFINITY ? 0.f : mn;  // nothing finite yet: all weights 0
+        const float alpha = exp2f(m[i] - base);
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float p = exp2f(z[i][j] - base);
+          s.p[4 * ty + i][tx + 16 * j] = p;
+          sum += p;
+        }
+        m[i] = mn;
+        l[i] = l[i] * alpha + over16(sum, false);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) acc[i][k] *= alpha;
+      }
+      __syncthreads();
+      load_tile<DP>(s.kv, a.v, t.x + k0, t.y - k0, a.kv_heads, kv_head, a.dim, vec);
+      __syncthreads();
+      mul_tile<DP>(s.kv, tx, acc, [&](int i, int j) { return s.p[4 * ty + i][j]; }, diag,
+                   [&](int i, int j) { return j <= 4 * ty + i; });
+      __syncthreads();
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float mx = -INFINITY;
+      const int row = q0 + 4 * ty + i;
+      if (row >= t.y) continue;
+      float* o = a.out + ((int64_t)(t.x + row) * a.heads + head) * a.dim;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool see = !diag || tx + 16 * j <= 4 * ty + i;
-        z[i][j] = see ? z[i][j] * c : -INFINITY;
-        mx = fmaxf(mx, z[i][j]);  // drops a NaN: exp2f below keeps it in the row's sum
-      }
-      const float mn = fmaxf(m[i], over16(mx, true));
-      const float base = mn == -INFINITY ? 0.f : mn;  // nothing finite yet: all weights 0
-      const float alpha = exp2f(m[i] - base);
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float p = exp2f(z[i][j] - base);
-        s.p[4 * ty + i][tx + 16 * j] = p;
-        sum += p;
-      }
-      m[i] = mn;
-      l[i] = l[i] * alpha + over16(sum, false);
-#pragma unroll
-      for (int k = 0; k < DP / 16; ++k) acc[i][k] *= alpha;
+      for (int k = 0; k < DP / 16; ++k)
+        if (column<DP>(tx, k) < a.dim) o[column<DP>(tx, k)] = __fdiv_rn(acc[i][k], l[i]);
+      if (tx == 0) a.lse[(int64_t)head * a.tokens + t.x + row] = (m[i] + log2f(l[i])) * kLn2;
     }
-    __syncthreads();
-    load_tile<DP>(s.kv, a.v, t.x + k0, t.y - k0, a.kv_heads, kv_head, a.dim, vec);
-    __syncthreads();
-    mul_tile<DP>(s.kv, tx, acc, [&](int i, int j) { return s.p[4 * ty + i][j]; }, diag,
-                 [&](int i, int j) { return j <= 4 * ty + i; });
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = q0 + 4 * ty + i;
-    if (row >= t.y) continue;
-    float* o = a.out + ((int64_t)(t.x + row) * a.heads + head) * a.dim;
-#pragma unroll
-    for (int k = 0; k < DP / 16; ++k)
-      if (column<DP>(tx, k) < a.dim) o[column<DP>(tx, k)] = __fdiv_rn(acc[i][k], l[i]);
-    if (tx == 0) a.lse[(int64_t)head * a.tokens + t.x + row] = (m[i] + log2f(l[i])) * kLn2;
-  }
+  });
 }
 
 // delta[h, t] = sum(grad * out): a warp per row.
@@ -270,84 +296,82 @@ template <int DP>
 __global__ void __launch_bounds__(kThreads) dq_kernel(const AttentionArgs a, bool vec) {
   extern __shared__ __align__(16) unsigned char raw[];
   BackwardSmem<DP>& s = *reinterpret_cast<BackwardSmem<DP>*>(raw);
-  const int4 t = a.tile[a.by_queries[blockIdx.x >> 1]];
-  const int q0 = t.z * kTileRows + (blockIdx.x & 1) * kB;
-  if (q0 >= t.y) return;
-  const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
-  if (!wanted(a, t, kv_head)) return;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  load_tile<DP>(s.q, a.q, t.x + q0, t.y - q0, a.heads, head, a.dim, vec);
-  load_tile<DP>(s.g, a.grad, t.x + q0, t.y - q0, a.heads, head, a.dim, vec);
-  float acc[4][DP / 16] = {};
-  for (int k0 = 0; k0 <= q0; k0 += kB) {
-    load_tile<DP>(s.k, a.k, t.x + k0, t.y - k0, a.kv_heads, kv_head, a.dim, vec);
-    load_tile<DP>(s.v, a.v, t.x + k0, t.y - k0, a.kv_heads, kv_head, a.dim, vec);
-    __syncthreads();
-    probabilities<DP, false>(a, s, t, head, q0, k0, ty, tx);
-    __syncthreads();
-    mul_tile<DP>(s.k, tx, acc, [&](int i, int j) { return s.ds[4 * ty + i][j]; }, k0 == q0,
-                 [&](int i, int j) { return j <= 4 * ty + i; });
-    __syncthreads();
-  }
+  for_halves(a, a.by_queries, a.heads, [&](const int4& t, int q0, int head) {
+    const int kv_head = head / (a.heads / a.kv_heads);
+    load_tile<DP>(s.q, a.q, t.x + q0, t.y - q0, a.heads, head, a.dim, vec);
+    load_tile<DP>(s.g, a.grad, t.x + q0, t.y - q0, a.heads, head, a.dim, vec);
+    float acc[4][DP / 16] = {};
+    for (int k0 = 0; k0 <= q0; k0 += kB) {
+      load_tile<DP>(s.k, a.k, t.x + k0, t.y - k0, a.kv_heads, kv_head, a.dim, vec);
+      load_tile<DP>(s.v, a.v, t.x + k0, t.y - k0, a.kv_heads, kv_head, a.dim, vec);
+      __syncthreads();
+      probabilities<DP, false>(a, s, t, head, q0, k0, ty, tx);
+      __syncthreads();
+      mul_tile<DP>(s.k, tx, acc, [&](int i, int j) { return s.ds[4 * ty + i][j]; }, k0 == q0,
+                   [&](int i, int j) { return j <= 4 * ty + i; });
+      __syncthreads();
+    }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = q0 + 4 * ty + i;
-    if (row >= t.y) continue;
-    float* o = a.dq + ((int64_t)(t.x + row) * a.heads + head) * a.dim;
+    for (int i = 0; i < 4; ++i) {
+      const int row = q0 + 4 * ty + i;
+      if (row >= t.y) continue;
+      float* o = a.dq + ((int64_t)(t.x + row) * a.heads + head) * a.dim;
 #pragma unroll
-    for (int k = 0; k < DP / 16; ++k)
-      if (column<DP>(tx, k) < a.dim) o[column<DP>(tx, k)] = acc[i][k] * a.scale;
-  }
+      for (int k = 0; k < DP / 16; ++k)
+        if (column<DP>(tx, k) < a.dim) o[column<DP>(tx, k)] = acc[i][k] * a.scale;
+    }
+  });
 }
 
 template <int DP>
 __global__ void __launch_bounds__(kThreads) dkv_kernel(const AttentionArgs a, bool vec) {
   extern __shared__ __align__(16) unsigned char raw[];
   BackwardSmem<DP>& s = *reinterpret_cast<BackwardSmem<DP>*>(raw);
-  const int4 t = a.tile[a.by_keys[blockIdx.x >> 1]];
-  const int k0 = t.z * kTileRows + (blockIdx.x & 1) * kB;
-  if (k0 >= t.y) return;
-  const int kv_head = blockIdx.y, group = a.heads / a.kv_heads;
-  if (!wanted(a, t, kv_head)) return;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  load_tile<DP>(s.k, a.k, t.x + k0, t.y - k0, a.kv_heads, kv_head, a.dim, vec);
-  load_tile<DP>(s.v, a.v, t.x + k0, t.y - k0, a.kv_heads, kv_head, a.dim, vec);
-  float dk[4][DP / 16] = {}, dv[4][DP / 16] = {};
-  for (int head = kv_head * group; head < (kv_head + 1) * group; ++head) {
-    for (int q0 = k0; q0 < t.y; q0 += kB) {
-      load_tile<DP>(s.q, a.q, t.x + q0, t.y - q0, a.heads, head, a.dim, vec);
-      load_tile<DP>(s.g, a.grad, t.x + q0, t.y - q0, a.heads, head, a.dim, vec);
-      __syncthreads();
-      probabilities<DP, true>(a, s, t, head, q0, k0, ty, tx);
-      __syncthreads();
-      const bool diag = q0 == k0;
-      const auto see = [&](int i, int j) { return 4 * ty + i <= j; };  // row i: the key, j: the query
-      mul_tile<DP>(s.g, tx, dv, [&](int i, int j) { return s.p[j][4 * ty + i]; }, diag, see);
-      mul_tile<DP>(s.q, tx, dk, [&](int i, int j) { return s.ds[j][4 * ty + i]; }, diag, see);
-      __syncthreads();
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, group = a.heads / a.kv_heads;
+  for_halves(a, a.by_keys, a.kv_heads, [&](const int4& t, int k0, int kv_head) {
+    load_tile<DP>(s.k, a.k, t.x + k0, t.y - k0, a.kv_heads, kv_head, a.dim, vec);
+    load_tile<DP>(s.v, a.v, t.x + k0, t.y - k0, a.kv_heads, kv_head, a.dim, vec);
+    float dk[4][DP / 16] = {}, dv[4][DP / 16] = {};
+    for (int head = kv_head * group; head < (kv_head + 1) * group; ++head) {
+      for (int q0 = k0; q0 < t.y; q0 += kB) {
+        load_tile<DP>(s.q, a.q, t.x + q0, t.y - q0, a.heads, head, a.dim, vec);
+        load_tile<DP>(s.g, a.grad, t.x + q0, t.y - q0, a.heads, head, a.dim, vec);
+        __syncthreads();
+        probabilities<DP, true>(a, s, t, head, q0, k0, ty, tx);
+        __syncthreads();
+        const bool diag = q0 == k0;
+        const auto see = [&](int i, int j) { return 4 * ty + i <= j; };  // row i: the key, j: the query
+        mul_tile<DP>(s.g, tx, dv, [&](int i, int j) { return s.p[j][4 * ty + i]; }, diag, see);
+        mul_tile<DP>(s.q, tx, dk, [&](int i, int j) { return s.ds[j][4 * ty + i]; }, diag, see);
+        __syncthreads();
+      }
     }
-  }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = k0 + 4 * ty + i;
-    if (row >= t.y) continue;
-    const int64_t at = ((int64_t)(t.x + row) * a.kv_heads + kv_head) * a.dim;
+    for (int i = 0; i < 4; ++i) {
+      const int row = k0 + 4 * ty + i;
+      if (row >= t.y) continue;
+      const int64_t at = ((int64_t)(t.x + row) * a.kv_heads + kv_head) * a.dim;
 #pragma unroll
-    for (int k = 0; k < DP / 16; ++k) {
-      const int col = column<DP>(tx, k);
-      if (col >= a.dim) continue;
-      a.dk[at + col] = dk[i][k] * a.scale;
-      a.dv[at + col] = dv[i][k];
+      for (int k = 0; k < DP / 16; ++k) {
+        const int col = column<DP>(tx, k);
+        if (col >= a.dim) continue;
+        a.dk[at + col] = dk[i][k] * a.scale;
+        a.dv[at + col] = dv[i][k];
+      }
     }
-  }
+  });
 }
 
-// Launches `kernel` with the padded head size that holds `dim`.
+// A CTA per half tile and head; where flags pick the few that are wanted, no
+// more than fill the GPU once, since reading the flags is then all most do.
 template <typename K>
-lmpb_status launch(K kernel, size_t smem, dim3 grid, const AttentionArgs& a, bool vec, const char* what,
+lmpb_status launch(K kernel, size_t smem, int heads, const AttentionArgs& a, bool vec, const char* what,
                    cudaStream_t st) {
   LMPB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kernel<<<grid, kThreads, smem, st>>>(a, vec);
+  const int64_t items = 2 * (int64_t)a.tiles * heads;
+  const int64_t grid = std::min<int64_t>(items, a.flags ? sm_count() : INT32_MAX);
+  kernel<<<(unsigned)grid, kThreads, smem, st>>>(a, vec);
   return launch_status(what);
 }
 
@@ -356,28 +380,26 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 }  // namespace
 
 lmpb_status attention_simt(const AttentionArgs& a, cudaStream_t st) {
-  const dim3 grid(2 * (unsigned)a.tiles, (unsigned)a.heads);
   const bool vec = a.dim % 4 == 0 && aligned16(a.q) && aligned16(a.k) && aligned16(a.v);
-  if (a.dim <= 32) return launch(forward_kernel<32>, sizeof(ForwardSmem<32>), grid, a, vec, "attention", st);
-  if (a.dim <= 64) return launch(forward_kernel<64>, sizeof(ForwardSmem<64>), grid, a, vec, "attention", st);
-  return launch(forward_kernel<128>, sizeof(ForwardSmem<128>), grid, a, vec, "attention", st);
+  if (a.dim <= 32) return launch(forward_kernel<32>, sizeof(ForwardSmem<32>), a.heads, a, vec, "attention", st);
+  if (a.dim <= 64) return launch(forward_kernel<64>, sizeof(ForwardSmem<64>), a.heads, a, vec, "attention", st);
+  return launch(forward_kernel<128>, sizeof(ForwardSmem<128>), a.heads, a, vec, "attention", st);
 }
 
 lmpb_status attention_simt_backward(const AttentionArgs& a, cudaStream_t st) {
-  const dim3 gq(2 * (unsigned)a.tiles, (unsigned)a.heads), gk(2 * (unsigned)a.tiles, (unsigned)a.kv_heads);
   const bool vec = a.dim % 4 == 0 && aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.grad);
   lmpb_status s = LMPB_OK;
   if (a.dq) {
     const char* what = "attention_backward (dq)";
-    s = a.dim <= 32   ? launch(dq_kernel<32>, sizeof(BackwardSmem<32>), gq, a, vec, what, st)
-        : a.dim <= 64 ? launch(dq_kernel<64>, sizeof(BackwardSmem<64>), gq, a, vec, what, st)
-                      : launch(dq_kernel<128>, sizeof(BackwardSmem<128>), gq, a, vec, what, st);
+    s = a.dim <= 32   ? launch(dq_kernel<32>, sizeof(BackwardSmem<32>), a.heads, a, vec, what, st)
+        : a.dim <= 64 ? launch(dq_kernel<64>, sizeof(BackwardSmem<64>), a.heads, a, vec, what, st)
+                      : launch(dq_kernel<128>, sizeof(BackwardSmem<128>), a.heads, a, vec, what, st);
   }
   if (s == LMPB_OK && a.dk) {
     const char* what = "attention_backward (dk, dv)";
-    s = a.dim <= 32   ? launch(dkv_kernel<32>, sizeof(BackwardSmem<32>), gk, a, vec, what, st)
-        : a.dim <= 64 ? launch(dkv_kernel<64>, sizeof(BackwardSmem<64>), gk, a, vec, what, st)
-                      : launch(dkv_kernel<128>, sizeof(BackwardSmem<128>), gk, a, vec, what, st);
+    s = a.dim <= 32   ? launch(dkv_kernel<32>, sizeof(BackwardSmem<32>), a.kv_heads, a, vec, what, st)
+        : a.dim <= 64 ? launch(dkv_kernel<64>, sizeof(BackwardSmem<64>), a.kv_heads, a, vec, what, st)
+                      : launch(dkv_kernel<128>, sizeof(BackwardSmem<128>), a.kv_heads, a, vec, what, st);
   }
   return s;
 }
@@ -402,6 +424,12 @@ lmpb_status check(const char* what, int64_t tokens, int heads, int kv_heads, int
                                             ", the current device is " + std::to_string(dev));
   }
   return LMPB_OK;
+}
+
+// Sequences of under 65 tokens leave half of every 128-row tile empty.
+bool on_tensor_cores(const AttentionArgs& a, const lmpb_sequences_s* seqs) {
+  static const bool off = getenv("LMPB_ATTENTION_SIMT") != nullptr;  // A/B switch
+  return !off && seqs->longest > 64 && attention_fits_sm100(a);
 }
 
 // Rows behind the last sequence belong to nobody: 0.
@@ -505,7 +533,7 @@ extern "C" lmpb_status lmpb_attention(const float* q, const float* k, const floa
   a.q = q, a.k = k, a.v = v, a.out = out, a.lse = lse;
   a.tokens = tokens, a.heads = heads, a.kv_heads = kv_heads, a.dim = head_dim, a.scale = scale;
   a.tile = seqs->tile, a.by_queries = seqs->by_queries, a.by_keys = seqs->by_keys, a.tiles = seqs->tiles;
-  return attention_simt(a, st);
+  return on_tensor_cores(a, seqs) ? attention_sm100(a, st) : attention_simt(a, st);
 }
 
 extern "C" lmpb_status lmpb_attention_backward(const float* q, const float* k, const float* v, const float* out,

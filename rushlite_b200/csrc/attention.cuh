@@ -40,6 +40,10 @@ struct AttentionArgs {
   const unsigned char* flags;
 };
 
+// Tensor-core kernels (attention_sm100.cu), for sequences that fill tiles.
+bool attention_fits_sm100(const AttentionArgs& a);
+lmpb_status attention_sm100(const AttentionArgs& a, cudaStream_t st);
+
 // fp32 kernels for any values and lengths (attention.cu).
 lmpb_status attention_simt(const AttentionArgs& a, cudaStream_t st);
 lmpb_status attention_simt_backward(const AttentionArgs& a, cudaStream_t st);

@@ -1,0 +1,702 @@
+// Causal attention over packed sequences on the B200 tensor cores, float32 in
+// and out: fp16 hi/lo split operands, tcgen05.mma, TMEM.
+//
+// fp32 accuracy.  A 128-row tile of q, k, v or grad is scaled by the power of
+// two that puts its largest magnitude into [2^14, 2^15) and each element x of
+// it becomes hi = fp16(x), lo = fp16(x - hi); a product of two operands is
+// the three MMAs lo.hi + hi.lo + hi.hi (lo.lo is 2^-22 of it).  hi and lo
+// together hold 22 bits of any x down to 2^-18 of the tile's maximum, and
+// 2^-40 of that maximum below.  Weights and their gradients are split the
+// same way on the fly, scaled by 2^14 (weights are at most 1) and by a bound
+// on the gradients' size.  The MMA's fp32 accumulator truncates, so nothing
+// accumulates in it for longer than one 128-row block: each block's product
+// is drained into registers, where the running sums round to nearest.
+//
+// Tiles whose values that cannot carry (infinities, NaN, rows over 2^18 apart,
+// magnitudes outside [2^-80, 2^60]) are flagged by the split; the fp32 kernels
+// of attention.cu then redo the sequences and head groups that hold one.
+//
+// 1. Split pass: a CTA per tile and head plane writes the tile's hi and lo as
+//    one block in the very layout the MMAs read from shared memory (128-byte
+//    swizzled rows of 64 halves), so the kernels fetch operands with plain
+//    bulk copies of up to 32 KB, no tensor maps.  Tiles never span sequences and rows
+//    behind a sequence are 0.  For v and grad it also finds the largest row
+//    norm, for grad the row sums delta = sum(grad * out).
+// 2. forward_kernel, dq_kernel, dkv_kernel: one CTA per tile and head, one
+//    CTA per SM.  Warp 0 feeds a ring of 32 KB stages, warp 1 issues the
+//    MMAs, 8 warps compute.  A row of the 128 x 128 score tile lives in one
+//    TMEM lane; two threads of different warps share it, 64 columns each.
+//    Scores are overwritten in place by the split weights, which are then the
+//    next MMA's A operand straight from TMEM.
+//    Every mbarrier wait is bounded; after one expires the thread stops
+//    waiting and issuing, runs its loops out and the kernel returns with its
+//    TMEM freed and lmpb_device_error set.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <mutex>
+#include <vector>
+
+#include "attention.cuh"
+#include "tcgen05.cuh"
+
+namespace lmpb {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kWeightBits = 14.f;  // weights enter the MMA times 2^14
+constexpr int kStage = 32768;
+
+__device__ unsigned int g_attention_error = 0;
+
+// Wait that gives up for good: false from the first expiry on.
+struct Waiter {
+  bool ok = true;
+  unsigned code;
+  __device__ __forceinline__ explicit Waiter(unsigned c) : code(c) {}
+  __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity) {
+    if (ok) ok = mbar_wait_bounded(bar, parity, &g_attention_error, code);
+    return ok;
+  }
+};
+
+// Bytes of one part (hi or lo) and of one tile's block.
+template <int DP>
+constexpr int part_bytes() { return DP / 64 * 128 * 128; }
+template <int DP>
+constexpr int block_bytes() { return 2 * part_bytes<DP>(); }
+
+// Where the split pass puts things.  Planes: query heads, key heads, value
+// heads, gradient heads; a plane's tile t is block plane * tiles + t.
+struct Split {
+  unsigned char* blocks;
+  int* expo;             // the tile was scaled by 2^expo
+  float* norm;           // largest row norm (v, grad)
+  float* dmax;           // largest |delta| (grad)
+  unsigned char* flags;
+};
+
+// ------------------------------------------------------------ split pass
+
+// hi and lo of two values, packed.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(__fsub_rn(a, f.x), __fsub_rn(b, f.y));
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+__device__ __forceinline__ float two_to(int e) { return __int_as_float((e + 127) << 23); }  // e in [-126, 127]
+
+// Grid: tiles x planes, 256 threads, a warp per 16 rows.  Lane l holds
+// columns 4 l.. of a row (DP = 128), or lanes l and l + 16 hold one of two rows (DP = 64).
+template <int DP>
+__global__ void __launch_bounds__(256) split_kernel(const AttentionArgs a, const Split o, float* __restrict__ delta, bool vec) {
+  constexpr int RPS = 128 / DP, STEPS = 16 / RPS, LANES = 32 / RPS;  // rows a step, steps, lanes a row
+  const int64_t plane = blockIdx.y;
+  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int4 tile = a.tile[t];
+  const int row0 = tile.z * kTileRows, rows = min(kTileRows, tile.y - row0);
+  const float* src;
+  int heads = a.kv_heads, head;
+  bool is_v = false, is_g = false;
+  if (plane < a.heads) src = a.q, heads = a.heads, head = (int)plane;
+  else if (plane < a.heads + a.kv_heads) src = a.k, head = (int)plane - a.heads;
+  else if (plane < a.heads + 2 * a.kv_heads) src = a.v, head = (int)plane - a.heads - a.kv_heads, is_v = true;
+  else src = a.grad, heads = a.heads, head = (int)plane - a.heads - 2 * a.kv_heads, is_g = true;
+  const int64_t first = (int64_t)(tile.x + row0), pitch = (int64_t)heads * a.dim;
+  const float* base = src + first * pitch + (int64_t)head * a.dim;
+  const float* obase = is_g ? a.out + first * pitch + (int64_t)head * a.dim : nullptr;
+  const int sub = lane / LANES, col = (lane % LANES) * 4;
+  auto load4 = [&](const float* p, int r) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r >= rows || col >= a.dim) return v;
+    p += r * pitch + col;
+    if (vec) return __ldg(reinterpret_cast<const float4*>(p));
+    v.x = __ldg(p);
+    if (col + 1 < a.dim) v.y = __ldg(p + 1);
+    if (col + 2 < a.dim) v.z = __ldg(p + 2);
+    if (col + 3 < a.dim) v.w = __ldg(p + 3);
+    return v;
+  };
+  float4 v[STEPS];
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) v[i] = load4(base, warp * 16 + i * RPS + sub);
+  float mx = 0.f, mn = INFINITY, nrm = 0.f, dmx = 0.f;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    float m = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
+    bad |= !(fabsf(v[i].x) < INFINITY && fabsf(v[i].y) < INFINITY && fabsf(v[i].z) < INFINITY && fabsf(v[i].w) < INFINITY);
+#pragma unroll
+    for (int s = LANES / 2; s; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+    mx = fmaxf(mx, m);
+    if (m > 0.f) mn = fminf(mn, m);
+    if (is_v || is_g) {
+      float q = v[i].x * v[i].x + v[i].y * v[i].y + v[i].z * v[i].z + v[i].w * v[i].w, d = 0.f;
+      const int r = warp * 16 + i * RPS + sub;
+      if (is_g) {
+        const float4 u = load4(obase, r);
+        d = v[i].x * u.x + v[i].y * u.y + v[i].z * u.z + v[i].w * u.w;
+      }
+#pragma unroll
+      for (int s = LANES / 2; s; s >>= 1) {
+        q += __shfl_xor_sync(0xffffffffu, q, s);
+        d += __shfl_xor_sync(0xffffffffu, d, s);
+      }
+      nrm = fmaxf(nrm, q);
+      dmx = fmaxf(dmx, fabsf(d));
+      if (is_g && lane % LANES == 0 && r < rows) delta[(int64_t)head * a.tokens + first + r] = d;
+    }
+  }
+  __shared__ float red[4][8];
+#pragma unroll
+  for (int s = 16; s; s >>= 1) {
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
+    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, s));
+    nrm = fmaxf(nrm, __shfl_xor_sync(0xffffffffu, nrm, s));
+    dmx = fmaxf(dmx, __shfl_xor_sync(0xffffffffu, dmx, s));
+  }
+  if (lane == 0) red[0][warp] = mx, red[1][warp] = mn, red[2][warp] = nrm, red[3][warp] = dmx;
+  const int bads = __syncthreads_or(bad);
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    mx = fmaxf(mx, red[0][w]);
+    mn = fminf(mn, red[1][w]);
+    nrm = fmaxf(nrm, red[2][w]);
+    dmx = fmaxf(dmx, red[3][w]);
+  }
+  // a gradient's small rows only ever add to larger sums: no limit on their range
+  const bool range = mx > 0.f && (mx > 0x1p60f || mx < 0x1p-80f || (!is_g && mn < mx * 0x1p-18f));
+  const bool flag = bads || range || !(dmx < INFINITY);
+  const int e = flag ? 0 : row_exp(mx);
+  const int64_t block = plane * a.tiles + t;
+  if (threadIdx.x == 0) {
+    o.expo[block] = e;
+    o.flags[block] = flag;
+    if (is_v || is_g) {
+      o.norm[block] = sqrtf(nrm) * 1.0001f;  // rounded sums: never below the norm
+      o.dmax[block] = dmx;
+    }
+  }
+  const float s = two_to(e);  // unflagged: e in [-46, 94]
+  unsigned char* out = o.blocks + block * block_bytes<DP>();
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int r = warp * 16 + i * RPS + sub;
+    uint2 hi, lo;
+    split2(v[i].x * s, v[i].y * s, hi.x, lo.x);
+    split2(v[i].z * s, v[i].w * s, hi.y, lo.y);
+    // 16-byte chunk c of row r sits at chunk c ^ (r & 7) of its 128 bytes
+    const int byte = (col & 63) * 2, at = (col >> 6) * 16384 + r * 128 + ((((byte >> 4) ^ (r & 7)) << 4) | (byte & 15));
+    *reinterpret_cast<uint2*>(out + at) = hi;
+    *reinterpret_cast<uint2*>(out + part_bytes<DP>() + at) = lo;
+  }
+}
+
+// ------------------------------------------------------------ PTX helpers
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+// 128-byte swizzled operand tiles, 8-row atoms 1024 bytes apart; `lbo`: the
+// stride between 64-column groups of an operand whose rows are the K axis.
+__device__ __forceinline__ uint64_t desc128(uint32_t addr, uint32_t lbo) {
+  return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+// f16 operands, fp32 accumulators, M = 128; B K-major, or with K as its rows.
+constexpr uint32_t idesc_of(int n, bool b_rows) {
+  return (1u << 4) | ((b_rows ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 2^x to 2^-22 of it; results below 2^-126 are 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A computing warp's wait: all its lanes go on together, with what the
+// barrier orders before them visible to their tcgen05 operations.
+__device__ __forceinline__ void warp_wait(Waiter& wait, uint32_t bar, uint32_t parity) {
+  wait(bar, parity);
+  __syncwarp();
+  tc_fence_after();
+}
+
+// Barrier of the 256 computing threads.
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// ------------------------------------------------------------ operand feed
+//
+// The ring carries, per operand tile, either its columns (the operand is
+// contracted over D: stage c holds hi and lo of columns [64 c, 64 c + 64) of
+// all 128 rows) or its rows (contracted over tokens: stage r holds hi and lo
+// of rows [64 r, 64 r + 64), all columns).  With DP = 64 a tile is one stage
+// that serves as either.
+
+template <int DP>
+constexpr int stages_per_tile() { return DP / 64; }
+
+struct Ring {
+  uint32_t base, full, empty;  // shared addresses; 8-byte barriers
+  int n;
+  uint32_t it = 0;
+  __device__ __forceinline__ uint32_t stage() const { return base + (it % n) * kStage; }
+  __device__ __forceinline__ uint32_t full_bar() const { return full + (it % n) * 8; }
+  __device__ __forceinline__ uint32_t empty_bar() const { return empty + (it % n) * 8; }
+  __device__ __forceinline__ uint32_t phase() const { return (it / n) & 1; }
+};
+
+template <int DP>
+__device__ __forceinline__ void feed(Ring& ring, Waiter& wait, const unsigned char* block, bool rows) {
+#pragma unroll
+  for (int s = 0; s < stages_per_tile<DP>(); ++s) {
+    if (!wait(ring.empty_bar(), ring.phase() ^ 1)) return;
+    const uint32_t bar = ring.full_bar(), dst = ring.stage();
+    mbar_expect_tx(bar, kStage);
+    if (DP == 64) {
+      bulk_load(dst, block, kStage, bar);
+    } else if (!rows) {
+      bulk_load(dst, block + s * 16384, 16384, bar);
+      bulk_load(dst + 16384, block + part_bytes<DP>() + s * 16384, 16384, bar);
+    } else {
+#pragma unroll
+      for (int part = 0; part < 2; ++part)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          bulk_load(dst + part * 16384 + c * 8192, block + part * part_bytes<DP>() + c * 16384 + s * 8192, 8192, bar);
+    }
+    ++ring.it;
+  }
+}
+
+// After the last feed: every copy that was started has landed.
+__device__ __forceinline__ void feed_done(const Ring& ring) {
+  const uint32_t n = min(ring.it, (uint32_t)ring.n);
+  for (uint32_t i = 0; i < n; ++i) {
+    const uint32_t k = ring.it - 1 - i;
+    Waiter wait(31);
+    wait(ring.full + (k % ring.n) * 8, (k / ring.n) & 1);
+  }
+}
+
+// D[128, 128] = A (shared, resident block) . B^T (a tile's columns from the ring).
+template <int DP>
+__device__ __forceinline__ void mma_columns(uint32_t d, uint32_t a_block, Ring& ring, Waiter& wait) {
+  constexpr uint32_t idesc = idesc_of(128, false);
+#pragma unroll
+  for (int s = 0; s < stages_per_tile<DP>(); ++s) {
+    if (!wait(ring.full_bar(), ring.phase())) return;
+    tc_fence_after();
+    const uint32_t b = ring.stage(), a = a_block + s * 16384;
+    const uint64_t ah = desc128(a, 16), al = desc128(a + part_bytes<DP>(), 16), bh = desc128(b, 16), bl = desc128(b + 16384, 16);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {  // 16 halves = 32 bytes a step
+      mma_ss(d, al + 2 * k, bh + 2 * k, idesc, s || k);
+      mma_ss(d, ah + 2 * k, bl + 2 * k, idesc, 1);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) mma_ss(d, ah + 2 * k, bh + 2 * k, idesc, 1);
+    mma_commit(ring.empty_bar());
+    ++ring.it;
+  }
+}
+
+// D[128, DP] = W . B, W the split weights in TMEM (16 columns for 16 tokens:
+// 8 of hi, 8 of lo), B a tile's rows from the ring.
+template <int DP>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t w, Ring& ring, Waiter& wait) {
+  constexpr uint32_t idesc = idesc_of(DP, true);
+  constexpr int N = stages_per_tile<DP>(), STEPS = 8 / N;
+#pragma unroll
+  for (int s = 0; s < N; ++s) {
+    if (!wait(ring.full_bar(), ring.phase())) return;
+    tc_fence_after();
+    const uint32_t b = ring.stage(), ws = w + s * STEPS * 16;
+    const uint64_t bh = desc128(b, 8192), bl = desc128(b + 16384, 8192);
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) {  // 16 rows = 2 atoms = 2048 bytes a step
+      mma_ts(d, ws + k * 16 + 8, bh + 128 * k, idesc, s || k);
+      mma_ts(d, ws + k * 16, bl + 128 * k, idesc, 1);
+    }
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) mma_ts(d, ws + k * 16, bh + 128 * k, idesc, 1);
+    mma_commit(ring.empty_bar());
+    ++ring.it;
+  }
+}
+
+// ------------------------------------------------------------ shared memory
+
+constexpr int kBars = 48;
+
+template <int DP, int RESIDENT, int RING>
+struct Layout {
+  static constexpr int kRing = RESIDENT * block_bytes<DP>();
+  static constexpr int kBarsAt = kRing + RING * kStage;
+  static constexpr int kScratch = kBarsAt + kBars * 8 + 16;
+  static constexpr int kBytes = kScratch + 2048;
+};
+
+template <int DP>
+constexpr int forward_ring() { return DP == 64 ? 4 : 5; }
+template <int DP>
+constexpr int backward_ring() { return DP == 64 ? 4 : 3; }
+template <int DP>
+using ForwardLayout = Layout<DP, 1, forward_ring<DP>()>;
+template <int DP>
+using BackwardLayout = Layout<DP, 2, backward_ring<DP>()>;
+
+// Sets up the barriers and all of TMEM; every thread calls it.  False (for
+// all) when the shared memory does not start on a swizzle atom.
+__device__ __forceinline__ bool setup(unsigned char* smem, uint32_t bars, uint32_t* slot, int ring, const int* counts, int n) {
+  const int warp = threadIdx.x >> 5;
+  const bool aligned = (smem_u32(smem) & 1023u) == 0;
+  if (!aligned) {
+    if (threadIdx.x == 0) atomicCAS(&g_attention_error, 0u, 99u);
+    return false;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2 * ring; ++i) mbar_init(bars + 8 * i, 1);
+    for (int i = 0; i < n; ++i) mbar_init(bars + 8 * (2 * ring + i), counts[i]);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  return true;
+}
+
+__device__ __forceinline__ void teardown(uint32_t tmem) {
+  tc_fence_before();
+  __syncthreads();
+  if ((threadIdx.x >> 5) == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// What a computing thread is: warps 2..9, TMEM lane quarter warp % 4, so rows
+// quarter * 32 + lane; the first four warps take columns 0..63 of a score row
+// (and the first half of D), the others the rest.
+struct Who {
+  int row, half;
+  uint32_t lanes;  // TMEM lane offset of this warp's quarter
+  __device__ __forceinline__ explicit Who(int first_warp) {
+    const int warp = threadIdx.x >> 5;
+    row = (warp & 3) * 32 + (threadIdx.x & 31);
+    half = (warp - first_warp) >> 2;
+    lanes = (uint32_t)((warp & 3) * 32) << 16;
+  }
+};
+
+// acc += (or, with `scale_acc`, acc * alpha +) f * this thread's D columns of a drained block.
+template <int DP>
+__device__ __forceinline__ void drain(uint32_t taddr, float (&acc)[DP / 2], float alpha, float f) {
+#pragma unroll
+  for (int c = 0; c < DP / 2; c += 32) {
+    uint32_t r[16], u[16];
+    tmem_ld16_issue(taddr + c, r);
+    tmem_ld16_issue(taddr + c + 16, u);
+    tmem_ld_wait();
+    tmem_regs_ready(r);
+    tmem_regs_ready(u);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      acc[c + i] = fmaf(__uint_as_float(r[i]), f, acc[c + i] * alpha);
+      acc[c + 16 + i] = fmaf(__uint_as_float(u[i]), f, acc[c + 16 + i] * alpha);
+    }
+  }
+}
+
+// One row's share of a result: DP / 2 values of columns [half * DP / 2, ...).
+template <int DP>
+__device__ __forceinline__ void store_row(float* p, const float (&acc)[DP / 2], int half, int dim, float f, bool vec) {
+  const int c0 = half * (DP / 2);
+  if (vec) {
+#pragma unroll
+    for (int c = 0; c < DP / 2; c += 4)
+      if (c0 + c < dim)
+        *reinterpret_cast<float4*>(p + c0 + c) = make_float4(acc[c] * f, acc[c + 1] * f, acc[c + 2] * f, acc[c + 3] * f);
+  } else {
+#pragma unroll
+    for (int c = 0; c < DP / 2; ++c)
+      if (c0 + c < dim) p[c0 + c] = acc[c] * f;
+  }
+}
+
+// ------------------------------------------------------------ forward
+//
+// TMEM: scores of even and odd key blocks in columns [0, 128) and [128, 256),
+// the block's product with v in [256, 256 + DP).  While the computing warps
+// turn block j's scores into weights, the MMAs of block j + 1's scores run.
+
+constexpr int kThreads = 320;
+
+template <int DP>
+__global__ void __launch_bounds__(kThreads, 1) forward_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  using L = ForwardLayout<DP>;
+  constexpr int RING = forward_ring<DP>();
+  const uint32_t base = smem_u32(smem), bars = base + L::kBarsAt;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + L::kBarsAt + kBars * 8);
+  float* xch = reinterpret_cast<float*>(smem + L::kScratch);  // [2][2][128]
+  // q, scores of each parity, weights, product, product drained, end
+  const int counts[7] = {1, 1, 1, 256, 1, 256, 1};
+  if (!setup(smem, bars, slot, RING, counts, 7)) return;
+  const uint32_t qfull = bars + 16 * RING, sfull = qfull + 8, pfull = qfull + 24, ofull = qfull + 32,
+                 oempty = qfull + 40, done = qfull + 48;
+  const uint32_t tmem = *slot;
+  const int order = blockIdx.x / a.heads, head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
+  const int t = a.by_queries[order];
+  const int4 tile = a.tile[t];
+  const int n = tile.z + 1;  // key blocks
+  const int64_t kplane = (int64_t)(a.heads + kv_head) * a.tiles + tile.w;
+  const int64_t vplane = kplane + (int64_t)a.kv_heads * a.tiles;
+  const int64_t qblock = (int64_t)head * a.tiles + t;
+  const int warp = threadIdx.x >> 5;
+  if (warp == 0) {
+    if ((threadIdx.x & 31) == 0) {
+      Ring ring{base + L::kRing, bars, bars + 8 * RING, RING};
+      Waiter wait(1);
+      mbar_expect_tx(qfull, block_bytes<DP>());
+      bulk_load(base, sp.blocks + qblock * block_bytes<DP>(), block_bytes<DP>(), qfull);
+      feed<DP>(ring, wait, sp.blocks + kplane * block_bytes<DP>(), false);
+      for (int j = 0; j < n; ++j) {
+        if (j + 1 < n) feed<DP>(ring, wait, sp.blocks + (kplane + j + 1) * block_bytes<DP>(), false);
+        feed<DP>(ring, wait, sp.blocks + (vplane + j) * block_bytes<DP>(), true);
+      }
+      feed_done(ring);
+      Waiter last(32);
+      last(qfull, 0);
+    }
+  } else if (warp == 1) {
+    if ((threadIdx.x & 31) == 0) {
+      Ring ring{base + L::kRing, bars, bars + 8 * RING, RING};
+      Waiter wait(2);
+      wait(qfull, 0);
+      mma_columns<DP>(tmem, base, ring, wait);
+      mma_commit(sfull);
+      for (int j = 0; j < n && wait.ok; ++j) {
+        if (j + 1 < n) {
+          mma_columns<DP>(tmem + ((j + 1) & 1) * 128, base, ring, wait);
+          mma_commit(sfull + 8 * ((j + 1) & 1));
+        }
+        wait(pfull, j & 1);
+        wait(oempty, (j & 1) ^ 1);
+        tc_fence_after();
+        if (wait.ok) mma_rows<DP>(tmem + 256, tmem + (j & 1) * 128, ring, wait);
+        mma_commit(ofull);
+      }
+      Waiter last(33);  // nothing of this CTA is in flight when it ends
+      mma_commit(done);
+      last(done, 0);
+    }
+  } else {
+    const Who me(2);
+    Waiter wait(3);
+    float acc[DP / 2], m = -INFINITY, l = 0.f, alpha = 0.f, of = 0.f;
+#pragma unroll
+    for (int i = 0; i < DP / 2; ++i) acc[i] = 0.f;
+    const int eq = sp.expo[qblock];
+    int ek = sp.expo[kplane], ev = sp.expo[vplane];
+    const uint32_t own = tmem + me.lanes + me.half * 64, oown = tmem + 256 + me.lanes + me.half * (DP / 2);
+    for (int j = 0; j < n; ++j) {
+      const float c = ldexpf(a.scale * kLog2e, -(eq + ek));
+      const float f = two_to(-ev);
+      if (j + 1 < n) ek = sp.expo[kplane + j + 1], ev = sp.expo[vplane + j + 1];
+      const uint32_t s = own + (j & 1) * 128;
+      // columns this row sees: all but in the last block, where column <= row
+      const bool diag = j + 1 == n;
+      const int see = diag ? me.row - me.half * 64 + 1 : 64;
+      warp_wait(wait, sfull + 8 * (j & 1), (j >> 1) & 1);
+      float mx = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 64; k += 32) {
+        uint32_t r[16], u[16];
+        tmem_ld16_issue(s + k, r);
+        tmem_ld16_issue(s + k + 16, u);
+        tmem_ld_wait();
+        tmem_regs_ready(r);
+        tmem_regs_ready(u);
+        if (!diag) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(r[i]), __uint_as_float(u[i])));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if (k + i < see) mx = fmaxf(mx, __uint_as_float(r[i]));
+            if (k + 16 + i < see) mx = fmaxf(mx, __uint_as_float(u[i]));
+          }
+        }
+      }
+      float* x = xch + (j & 1) * 256;
+      x[me.half * 128 + me.row] = mx;
+      compute_sync();
+      mx = fmaxf(mx, x[(me.half ^ 1) * 128 + me.row]);
+      const float mn = fmaxf(m, mx * c);  // finite: every row sees key 0 of the first block
+      const float next = exp2_fast(m - mn), bias = kWeightBits - mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 64; k += 16) {
+        uint32_t r[16], w[16];
+        tmem_ld16_issue(s + k, r);
+        tmem_ld_wait();
+        tmem_regs_ready(r);
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          float p0 = exp2_fast(fmaf(__uint_as_float(r[i]), c, bias));
+          float p1 = exp2_fast(fmaf(__uint_as_float(r[i + 1]), c, bias));
+          if (diag) {
+            if (k + i >= see) p0 = 0.f;
+            if (k + i + 1 >= see) p1 = 0.f;
+          }
+          sum += p0 + p1;
+          split2(p0, p1, w[i / 2], w[8 + i / 2]);
+        }
+        tmem_st16(s + k, w);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(pfull);
+      l = l * next + sum;
+      m = mn;
+      if (j > 0) {
+        warp_wait(wait, ofull, (j - 1) & 1);
+        drain<DP>(oown, acc, alpha, of);
+        tc_fence_before();
+        mbar_arrive(oempty);
+      }
+      alpha = next;
+      of = f;
+    }
+    warp_wait(wait, ofull, (n - 1) & 1);
+    drain<DP>(oown, acc, alpha, of);
+    float* x = xch + (n & 1) * 256;
+    x[me.half * 128 + me.row] = l;
+    compute_sync();
+    l = x[me.row] + x[128 + me.row];
+    const int row = tile.z * kTileRows + me.row;
+    if (row < tile.y && wait.ok) {
+      const int64_t at = tile.x + row;
+      store_row<DP>(a.out + (at * a.heads + head) * a.dim, acc, me.half, a.dim, __frcp_rn(l), vec_out);
+      if (me.half == 0) a.lse[(int64_t)head * a.tokens + at] = (m + log2f(l) - kWeightBits) * kLn2;
+    }
+  }
+  teardown(tmem);
+}
+
+// ------------------------------------------------------------ host side
+
+template <typename K>
+lmpb_status allow_smem(K kernel, int bytes) {
+  LMPB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  return LMPB_OK;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// One allocation for the split blocks and what goes with them.
+lmpb_status make_split(const AttentionArgs& a, bool backward, int dp, Split& s, float** delta, void** ws, cudaStream_t st) {
+  auto up = [](size_t b) { return (b + 255) / 256 * 256; };
+  const size_t planes = (size_t)(backward ? 2 : 1) * a.heads + 2 * a.kv_heads, n = planes * a.tiles;
+  const size_t blocks = n * (dp == 64 ? block_bytes<64>() : block_bytes<128>());
+  const size_t dbytes = backward ? up((size_t)a.tokens * a.heads * 4) : 0;
+  LMPB_CUDA_TRY(stream_alloc(ws, blocks + 3 * up(4 * n) + up(n) + dbytes, st));
+  unsigned char* p = static_cast<unsigned char*>(*ws);
+  s.blocks = p;
+  s.expo = reinterpret_cast<int*>(p + blocks);
+  s.norm = reinterpret_cast<float*>(p + blocks + up(4 * n));
+  s.dmax = reinterpret_cast<float*>(p + blocks + 2 * up(4 * n));
+  s.flags = p + blocks + 3 * up(4 * n);
+  *delta = reinterpret_cast<float*>(s.flags + up(n));
+  return LMPB_OK;
+}
+
+template <int DP>
+lmpb_status split(const AttentionArgs& a, const Split& s, float* delta, cudaStream_t st) {
+  const unsigned planes = (a.grad ? 2 : 1) * a.heads + 2 * a.kv_heads;
+  const bool vec = a.dim % 4 == 0 && aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.grad) &&
+                   (!a.grad || aligned16(a.out));
+  split_kernel<DP><<<dim3((unsigned)a.tiles, planes), 256, 0, st>>>(a, s, delta, vec);
+  return launch_status("attention (split)");
+}
+
+template <int DP>
+lmpb_status forward(const AttentionArgs& a, const Split& s, cudaStream_t st) {
+  lmpb_status r = split<DP>(a, s, nullptr, st);
+  if (r == LMPB_OK) r = allow_smem(forward_kernel<DP>, ForwardLayout<DP>::kBytes);
+  if (r != LMPB_OK) return r;
+  const bool vec = a.dim % 4 == 0 && aligned16(a.out);
+  forward_kernel<DP><<<(unsigned)(a.tiles * a.heads), kThreads, ForwardLayout<DP>::kBytes, st>>>(a, s, vec);
+  return launch_status("attention");
+}
+
+}  // namespace
+
+bool attention_fits_sm100(const AttentionArgs& a) {
+  return (int64_t)a.tiles * a.heads <= 0x7fffffff && 2 * a.heads + 2 * a.kv_heads <= 65535;
+}
+
+lmpb_status attention_sm100(const AttentionArgs& args, cudaStream_t st) {
+  AttentionArgs a = args;
+  Split s{};
+  float* unused = nullptr;
+  void* ws = nullptr;
+  const int dp = a.dim <= 64 ? 64 : 128;
+  lmpb_status r = make_split(a, false, dp, s, &unused, &ws, st);
+  if (r != LMPB_OK) return r;
+  r = dp == 64 ? forward<64>(a, s, st) : forward<128>(a, s, st);
+  a.flags = s.flags;
+  if (r == LMPB_OK) r = attention_simt(a, st);
+  const cudaError_t e = cudaFreeAsync(ws, st);
+  if (r == LMPB_OK && e != cudaSuccess)
+    return set_error(LMPB_ERR_CUDA, std::string("cudaFreeAsync: ") + cudaGetErrorString(e));
+  return r;
+}
+
+// Reads and clears the attention kernels' error word (0 = none).
+unsigned int attention_take_error() {
+  unsigned int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_attention_error, sizeof v) != cudaSuccess) return 0xFFFFFFFFu;
+  if (v) cudaMemcpyToSymbol(g_attention_error, &zero, sizeof zero);
+  return v;
+}
+
+}  // namespace lmpb
