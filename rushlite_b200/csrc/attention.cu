@@ -551,17 +551,19 @@ extern "C" lmpb_status lmpb_attention_backward(const float* q, const float* k, c
   if (s == LMPB_OK) s = clear_tail(dk, seqs->tokens, tokens, (int64_t)kv_heads * head_dim, st);
   if (s == LMPB_OK) s = clear_tail(dv, seqs->tokens, tokens, (int64_t)kv_heads * head_dim, st);
   if (s != LMPB_OK || seqs->tiles == 0) return s;
+  AttentionArgs a{};
+  a.q = q, a.k = k, a.v = v, a.out = const_cast<float*>(out), a.lse = const_cast<float*>(lse), a.grad = grad;
+  a.dq = dq, a.dk = dk, a.dv = dv;
+  a.tokens = tokens, a.heads = heads, a.kv_heads = kv_heads, a.dim = head_dim, a.scale = scale;
+  a.tile = seqs->tile, a.by_queries = seqs->by_queries, a.by_keys = seqs->by_keys, a.tiles = seqs->tiles;
+  if (on_tensor_cores(a, seqs)) return attention_sm100_backward(a, st);
   float* delta = nullptr;
   LMPB_CUDA_TRY(stream_alloc((void**)&delta, (size_t)tokens * heads * 4, st));
   const int64_t rows = seqs->tokens * heads;
   delta_kernel<<<(unsigned)((rows + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st>>>(
       grad, out, delta, seqs->tokens, tokens, heads, head_dim);
   s = launch_status("attention_backward (delta)");
-  AttentionArgs a{};
-  a.q = q, a.k = k, a.v = v, a.lse = const_cast<float*>(lse), a.grad = grad, a.delta = delta;
-  a.dq = dq, a.dk = dk, a.dv = dv;
-  a.tokens = tokens, a.heads = heads, a.kv_heads = kv_heads, a.dim = head_dim, a.scale = scale;
-  a.tile = seqs->tile, a.by_queries = seqs->by_queries, a.by_keys = seqs->by_keys, a.tiles = seqs->tiles;
+  a.delta = delta;
   if (s == LMPB_OK) s = attention_simt_backward(a, st);
   const cudaError_t e = cudaFreeAsync(delta, st);
   if (s == LMPB_OK && e != cudaSuccess)

@@ -43,6 +43,7 @@ struct AttentionArgs {
 // Tensor-core kernels (attention_sm100.cu), for sequences that fill tiles.
 bool attention_fits_sm100(const AttentionArgs& a);
 lmpb_status attention_sm100(const AttentionArgs& a, cudaStream_t st);
+lmpb_status attention_sm100_backward(const AttentionArgs& a, cudaStream_t st);  // computes delta itself
 
 // fp32 kernels for any values and lengths (attention.cu).
 lmpb_status attention_simt(const AttentionArgs& a, cudaStream_t st);

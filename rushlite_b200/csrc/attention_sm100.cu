@@ -13,7 +13,7 @@
 // is drained into registers, where the running sums round to nearest.
 //
 // Tiles whose values that cannot carry (infinities, NaN, rows over 2^18 apart,
-// magnitudes outside [2^-80, 2^60]) are flagged by the split; the fp32 kernels
+// magnitudes outside [2^-60, 2^40]) are flagged by the split; the fp32 kernels
 // of attention.cu then redo the sequences and head groups that hold one.
 //
 // 1. Split pass: a CTA per tile and head plane writes the tile's hi and lo as
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(256) split_kernel(const AttentionArgs a, const
     dmx = fmaxf(dmx, red[3][w]);
   }
   // a gradient's small rows only ever add to larger sums: no limit on their range
-  const bool range = mx > 0.f && (mx > 0x1p60f || mx < 0x1p-80f || (!is_g && mn < mx * 0x1p-18f));
+  const bool range = mx > 0.f && (mx > 0x1p40f || mx < 0x1p-60f || (!is_g && mn < mx * 0x1p-18f));
   const bool flag = bads || range || !(dmx < INFINITY);
   const int e = flag ? 0 : row_exp(mx);
   const int64_t block = plane * a.tiles + t;
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(256) split_kernel(const AttentionArgs a, const
       o.dmax[block] = dmx;
     }
   }
-  const float s = two_to(e);  // unflagged: e in [-46, 94]
+  const float s = two_to(e);  // unflagged: e in [-26, 75]
   unsigned char* out = o.blocks + block * block_bytes<DP>();
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
@@ -280,7 +280,7 @@ struct Ring {
 
 template <int DP>
 __device__ __forceinline__ void feed(Ring& ring, Waiter& wait, const unsigned char* block, bool rows) {
-#pragma unroll
+#pragma unroll 1
   for (int s = 0; s < stages_per_tile<DP>(); ++s) {
     if (!wait(ring.empty_bar(), ring.phase() ^ 1)) return;
     const uint32_t bar = ring.full_bar(), dst = ring.stage();
@@ -315,7 +315,7 @@ __device__ __forceinline__ void feed_done(const Ring& ring) {
 template <int DP>
 __device__ __forceinline__ void mma_columns(uint32_t d, uint32_t a_block, Ring& ring, Waiter& wait) {
   constexpr uint32_t idesc = idesc_of(128, false);
-#pragma unroll
+#pragma unroll 1
   for (int s = 0; s < stages_per_tile<DP>(); ++s) {
     if (!wait(ring.full_bar(), ring.phase())) return;
     tc_fence_after();
@@ -339,7 +339,7 @@ template <int DP>
 __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t w, Ring& ring, Waiter& wait) {
   constexpr uint32_t idesc = idesc_of(DP, true);
   constexpr int N = stages_per_tile<DP>(), STEPS = 8 / N;
-#pragma unroll
+#pragma unroll 1
   for (int s = 0; s < N; ++s) {
     if (!wait(ring.full_bar(), ring.phase())) return;
     tc_fence_after();
@@ -622,6 +622,350 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const AttentionArg
   teardown(tmem);
 }
 
+// ------------------------------------------------------------ backward
+//
+// dS of a block is split into fp16 under a power of two chosen for the block
+// from a bound on its values: |dP_ij| <= |grad_i| |v_j| and P <= 1, so
+// |dS_ij| <= max|grad_i| max|v_j| + max|delta_i| over the block's rows.
+
+struct DsScale {
+  int e;        // dS enters the MMA times 2^e
+  float dp, d;  // dS 2^e = P (dp * dP' - d * delta), dP' the scaled operands' product
+};
+
+__device__ __forceinline__ DsScale ds_scale(float gnorm, float vnorm, float dmax, int eg, int ev, float weight_bits) {
+  DsScale s;
+  s.e = min(100, row_exp(fmaf(gnorm, vnorm, dmax)));
+  s.dp = ldexpf(1.f, s.e - eg - ev - (int)weight_bits);
+  s.d = ldexpf(1.f, s.e - (int)weight_bits);
+  return s;
+}
+
+// dq of one query tile and head.  TMEM: scores of even and odd key blocks in
+// columns [0, 256), overwritten by dS; dP in [256, 384); the block's product
+// with k in [384, 384 + DP).  Block j + 1's scores run while the computing
+// warps turn block j's scores and dP into dS.
+template <int DP>
+__global__ void __launch_bounds__(kThreads, 1) dq_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  using L = BackwardLayout<DP>;
+  constexpr int RING = backward_ring<DP>();
+  const uint32_t base = smem_u32(smem), bars = base + L::kBarsAt;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + L::kBarsAt + kBars * 8);
+  // q and grad, scores and dP, dS, product, product drained, end
+  const int counts[6] = {1, 1, 256, 1, 256, 1};
+  if (!setup(smem, bars, slot, RING, counts, 6)) return;
+  const uint32_t resident = bars + 16 * RING, spfull = resident + 8, dsfull = resident + 16, ofull = resident + 24,
+                 oempty = resident + 32, done = resident + 40;
+  const uint32_t tmem = *slot;
+  const int order = blockIdx.x / a.heads, head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
+  const int t = a.by_queries[order];
+  const int4 tile = a.tile[t];
+  const int n = tile.z + 1;  // key blocks
+  const int64_t kplane = (int64_t)(a.heads + kv_head) * a.tiles + tile.w;
+  const int64_t vplane = kplane + (int64_t)a.kv_heads * a.tiles;
+  const int64_t qblock = (int64_t)head * a.tiles + t;
+  const int64_t gblock = qblock + (int64_t)(a.heads + 2 * a.kv_heads) * a.tiles;
+  const int warp = threadIdx.x >> 5;
+  constexpr int64_t BB = block_bytes<DP>();
+  if (warp == 0) {
+    if ((threadIdx.x & 31) == 0) {
+      Ring ring{base + L::kRing, bars, bars + 8 * RING, RING};
+      Waiter wait(11);
+      mbar_expect_tx(resident, 2 * BB);
+      bulk_load(base, sp.blocks + qblock * BB, BB, resident);
+      bulk_load(base + BB, sp.blocks + gblock * BB, BB, resident);
+      feed<DP>(ring, wait, sp.blocks + kplane * BB, false);
+      feed<DP>(ring, wait, sp.blocks + vplane * BB, false);
+      for (int j = 0; j < n; ++j) {
+        if (j + 1 < n) {
+          feed<DP>(ring, wait, sp.blocks + (kplane + j + 1) * BB, false);
+          feed<DP>(ring, wait, sp.blocks + (vplane + j + 1) * BB, false);
+        }
+        feed<DP>(ring, wait, sp.blocks + (kplane + j) * BB, true);
+      }
+      feed_done(ring);
+      Waiter last(32);
+      last(resident, 0);
+    }
+  } else if (warp == 1) {
+    if ((threadIdx.x & 31) == 0) {
+      Ring ring{base + L::kRing, bars, bars + 8 * RING, RING};
+      Waiter wait(12);
+      wait(resident, 0);
+      mma_columns<DP>(tmem, base, ring, wait);
+      mma_columns<DP>(tmem + 256, base + BB, ring, wait);
+      mma_commit(spfull);
+      for (int j = 0; j < n && wait.ok; ++j) {
+        if (j + 1 < n) mma_columns<DP>(tmem + ((j + 1) & 1) * 128, base, ring, wait);
+        wait(dsfull, j & 1);
+        tc_fence_after();
+        if (j + 1 < n && wait.ok) {
+          mma_columns<DP>(tmem + 256, base + BB, ring, wait);
+          mma_commit(spfull);
+        }
+        wait(oempty, (j & 1) ^ 1);
+        tc_fence_after();
+        if (wait.ok) mma_rows<DP>(tmem + 384, tmem + (j & 1) * 128, ring, wait);
+        mma_commit(ofull);
+      }
+      Waiter last(33);
+      mma_commit(done);
+      last(done, 0);
+    }
+  } else {
+    const Who me(2);
+    Waiter wait(13);
+    float acc[DP / 2], of = 0.f;
+#pragma unroll
+    for (int i = 0; i < DP / 2; ++i) acc[i] = 0.f;
+    const int row = tile.z * kTileRows + me.row;
+    const int64_t at = (int64_t)head * a.tokens + tile.x + row;
+    const float lse = row < tile.y ? a.lse[at] * kLog2e : INFINITY;  // rows behind the sequence: no weight
+    const float delta = row < tile.y ? a.delta[at] : 0.f;
+    const int eq = sp.expo[qblock], eg = sp.expo[gblock];
+    const float gnorm = sp.norm[gblock], dmax = sp.dmax[gblock];
+    int ek = sp.expo[kplane], ev = sp.expo[vplane];
+    float vnorm = sp.norm[vplane];
+    const uint32_t own = tmem + me.lanes + me.half * 64, oown = tmem + 384 + me.lanes + me.half * (DP / 2);
+    for (int j = 0; j < n; ++j) {
+      const float c = ldexpf(a.scale * kLog2e, -(eq + ek));
+      const DsScale ds = ds_scale(gnorm, vnorm, dmax, eg, ev, 0.f);
+      const float f = ldexpf(a.scale, -(ds.e + ek)), dd = delta * ds.d;
+      if (j + 1 < n) ek = sp.expo[kplane + j + 1], ev = sp.expo[vplane + j + 1], vnorm = sp.norm[vplane + j + 1];
+      const uint32_t s = own + (j & 1) * 128, dp = own + 256;
+      const bool diag = j + 1 == n;
+      const int see = me.row - me.half * 64 + 1;
+      warp_wait(wait, spfull, j & 1);
+#pragma unroll
+      for (int k = 0; k < 64; k += 16) {
+        uint32_t r[16], u[16], w[16];
+        tmem_ld16_issue(s + k, r);
+        tmem_ld16_issue(dp + k, u);
+        tmem_ld_wait();
+        tmem_regs_ready(r);
+        tmem_regs_ready(u);
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          float d0 = exp2_fast(fmaf(__uint_as_float(r[i]), c, -lse)) * fmaf(__uint_as_float(u[i]), ds.dp, -dd);
+          float d1 = exp2_fast(fmaf(__uint_as_float(r[i + 1]), c, -lse)) * fmaf(__uint_as_float(u[i + 1]), ds.dp, -dd);
+          if (diag) {
+            if (k + i >= see) d0 = 0.f;
+            if (k + i + 1 >= see) d1 = 0.f;
+          }
+          split2(d0, d1, w[i / 2], w[8 + i / 2]);
+        }
+        tmem_st16(s + k, w);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(dsfull);
+      if (j > 0) {
+        warp_wait(wait, ofull, (j - 1) & 1);
+        drain<DP>(oown, acc, 1.f, of);
+        tc_fence_before();
+        mbar_arrive(oempty);
+      }
+      of = f;
+    }
+    warp_wait(wait, ofull, (n - 1) & 1);
+    drain<DP>(oown, acc, 1.f, of);
+    if (row < tile.y && wait.ok)
+      store_row<DP>(a.dq + ((int64_t)(tile.x + row) * a.heads + head) * a.dim, acc, me.half, a.dim, 1.f, vec_out);
+  }
+  teardown(tmem);
+}
+
+// dk and dv of one key tile and key/value head, over the group's query heads
+// and their tiles from the diagonal on.  Rows are keys, columns queries.
+// TMEM: scores in columns [0, 128), overwritten by the weights; dP in
+// [128, 256), overwritten by dS; the block's shares of dv and dk in
+// [256, 256 + DP) and [384, 384 + DP).  The MMAs of a block run scores, dP,
+// dv, dk: weights are computed under dP, dS under dv.
+//
+// Both running sums are held in registers, 2 x DP / 2 a thread.  12 warps of
+// 168 registers are launched; the first four keep 88 so that the
+// computing eight can have 208 (128 x 88 + 256 x 208 = 384 x 168).
+constexpr int kThreadsKV = 384;
+
+template <int DP>
+__global__ void __launch_bounds__(kThreadsKV, 1) dkv_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  using L = BackwardLayout<DP>;
+  constexpr int RING = backward_ring<DP>();
+  const uint32_t base = smem_u32(smem), bars = base + L::kBarsAt;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + L::kBarsAt + kBars * 8);
+  float* stat = reinterpret_cast<float*>(smem + L::kScratch);  // [2][2][128]: weight offset, scaled delta
+  // k and v, scores, dP, weights, dS, dv, dv drained, dk, dk drained, end
+  const int counts[10] = {1, 1, 1, 256, 256, 1, 256, 1, 256, 1};
+  if (!setup(smem, bars, slot, RING, counts, 10)) return;
+  const uint32_t resident = bars + 16 * RING, sfull = resident + 8, dpfull = resident + 16, pfull = resident + 24,
+                 dsfull = resident + 32, vfull = resident + 40, vempty = resident + 48, kfull = resident + 56,
+                 kempty = resident + 64, done = resident + 72;
+  const uint32_t tmem = *slot;
+  const int order = blockIdx.x / a.kv_heads, kv_head = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
+  const int t = a.by_keys[order];
+  const int4 tile = a.tile[t];
+  const int per_head = (tile.y + kTileRows - 1) / kTileRows - tile.z, n = per_head * group;  // query blocks
+  const int64_t kblock = (int64_t)(a.heads + kv_head) * a.tiles + t;
+  const int64_t vblock = kblock + (int64_t)a.kv_heads * a.tiles;
+  const int64_t gplanes = (int64_t)(a.heads + 2 * a.kv_heads) * a.tiles;
+  // block i: query head and tile, as a block index of the q planes
+  auto qblock = [&](int i) { return (int64_t)(kv_head * group + i / per_head) * a.tiles + t + i % per_head; };
+  const int warp = threadIdx.x >> 5;
+  constexpr int64_t BB = block_bytes<DP>();
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 0 && (threadIdx.x & 31) == 0) {
+      Ring ring{base + L::kRing, bars, bars + 8 * RING, RING};
+      Waiter wait(21);
+      mbar_expect_tx(resident, 2 * BB);
+      bulk_load(base, sp.blocks + kblock * BB, BB, resident);
+      bulk_load(base + BB, sp.blocks + vblock * BB, BB, resident);
+      for (int i = 0; i < n; ++i) {
+        const unsigned char *q = sp.blocks + qblock(i) * BB, *g = q + gplanes * BB;
+        feed<DP>(ring, wait, q, false);
+        feed<DP>(ring, wait, g, false);
+        feed<DP>(ring, wait, g, true);
+        feed<DP>(ring, wait, q, true);
+      }
+      feed_done(ring);
+      Waiter last(32);
+      last(resident, 0);
+    } else if (warp == 1 && (threadIdx.x & 31) == 0) {
+      Ring ring{base + L::kRing, bars, bars + 8 * RING, RING};
+      Waiter wait(22);
+      wait(resident, 0);
+      for (int i = 0; i < n && wait.ok; ++i) {
+        mma_columns<DP>(tmem, base, ring, wait);
+        mma_commit(sfull);
+        mma_columns<DP>(tmem + 128, base + BB, ring, wait);
+        mma_commit(dpfull);
+        wait(pfull, i & 1);
+        wait(vempty, (i & 1) ^ 1);
+        tc_fence_after();
+        if (wait.ok) mma_rows<DP>(tmem + 256, tmem, ring, wait);
+        mma_commit(vfull);
+        wait(dsfull, i & 1);
+        wait(kempty, (i & 1) ^ 1);
+        tc_fence_after();
+        if (wait.ok) mma_rows<DP>(tmem + 384, tmem + 128, ring, wait);
+        mma_commit(kfull);
+      }
+      Waiter last(33);
+      mma_commit(done);
+      last(done, 0);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const Who me(4);
+    Waiter wait(23);
+    float dk[DP / 2], dv[DP / 2], fk = 0.f;
+#pragma unroll
+    for (int i = 0; i < DP / 2; ++i) dk[i] = dv[i] = 0.f;
+    const int ek = sp.expo[kblock], ev = sp.expo[vblock];
+    const float vnorm = sp.norm[vblock];
+    const uint32_t own = tmem + me.lanes + me.half * 64, oown = tmem + 256 + me.lanes + me.half * (DP / 2);
+    // one value of the next block's row statistics a thread: lse (first half) or delta
+    const int tid = threadIdx.x - 128;
+    const float* source = tid < 128 ? a.lse : a.delta;
+    auto fetch = [&](int i) {
+      const int r = (tile.z + i % per_head) * kTileRows + (tid & 127);
+      const int64_t at = (int64_t)(kv_head * group + i / per_head) * a.tokens + tile.x + r;
+      return r < tile.y ? __ldg(source + at) : tid < 128 ? INFINITY : 0.f;
+    };
+    float next = fetch(0);
+    for (int i = 0; i < n; ++i) {
+      const int64_t qb = qblock(i), gb = qb + gplanes;
+      const int eq = sp.expo[qb], eg = sp.expo[gb];
+      const float c = ldexpf(a.scale * kLog2e, -(eq + ek));
+      const DsScale ds = ds_scale(sp.norm[gb], vnorm, sp.dmax[gb], eg, ev, kWeightBits);
+      float* st = stat + (i & 1) * 256;
+      st[tid] = tid < 128 ? kWeightBits - next * kLog2e : next * ds.d;
+      compute_sync();
+      if (i + 1 < n) next = fetch(i + 1);
+      const bool diag = i % per_head == 0;
+      const int from = me.row - me.half * 64;  // on the diagonal, queries from this column on see the key
+      const float4* bias = reinterpret_cast<const float4*>(st + me.half * 64);
+      const float4* dd = reinterpret_cast<const float4*>(st + 128 + me.half * 64);
+      warp_wait(wait, sfull, i & 1);
+#pragma unroll
+      for (int k = 0; k < 64; k += 16) {
+        uint32_t r[16], w[16];
+        tmem_ld16_issue(own + k, r);
+        tmem_ld_wait();
+        tmem_regs_ready(r);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 b = bias[(k + j) / 4];
+          float p[4] = {exp2_fast(fmaf(__uint_as_float(r[j]), c, b.x)), exp2_fast(fmaf(__uint_as_float(r[j + 1]), c, b.y)),
+                        exp2_fast(fmaf(__uint_as_float(r[j + 2]), c, b.z)), exp2_fast(fmaf(__uint_as_float(r[j + 3]), c, b.w))};
+          if (diag) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (k + j + x < from) p[x] = 0.f;
+          }
+          split2(p[0], p[1], w[j / 2], w[8 + j / 2]);
+          split2(p[2], p[3], w[j / 2 + 1], w[8 + j / 2 + 1]);
+        }
+        tmem_st16(own + k, w);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(pfull);
+      if (i > 0) {
+        warp_wait(wait, kfull, (i - 1) & 1);
+        drain<DP>(oown + 128, dk, 1.f, fk);
+        tc_fence_before();
+        mbar_arrive(kempty);
+      }
+      warp_wait(wait, dpfull, i & 1);
+#pragma unroll
+      for (int k = 0; k < 64; k += 16) {
+        uint32_t r[16], u[16], w[16];
+        tmem_ld16_issue(own + k, r);
+        tmem_ld16_issue(own + 128 + k, u);
+        tmem_ld_wait();
+        tmem_regs_ready(r);
+        tmem_regs_ready(u);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 d = dd[(k + j) / 4];
+          const float dx[4] = {d.x, d.y, d.z, d.w};
+          float v[4];
+#pragma unroll
+          for (int x = 0; x < 4; x += 2) {  // the weight is exactly hi + lo
+            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&r[(j + x) / 2]));
+            const float2 l = __half22float2(*reinterpret_cast<const __half2*>(&r[8 + (j + x) / 2]));
+            v[x] = (h.x + l.x) * fmaf(__uint_as_float(u[j + x]), ds.dp, -dx[x]);
+            v[x + 1] = (h.y + l.y) * fmaf(__uint_as_float(u[j + x + 1]), ds.dp, -dx[x + 1]);
+          }
+          split2(v[0], v[1], w[j / 2], w[8 + j / 2]);
+          split2(v[2], v[3], w[j / 2 + 1], w[8 + j / 2 + 1]);
+        }
+        tmem_st16(own + 128 + k, w);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(dsfull);
+      warp_wait(wait, vfull, i & 1);
+      drain<DP>(oown, dv, 1.f, two_to(-(int)kWeightBits - eg));
+      tc_fence_before();
+      mbar_arrive(vempty);
+      fk = ldexpf(a.scale, -(ds.e + eq));
+    }
+    warp_wait(wait, kfull, (n - 1) & 1);
+    drain<DP>(oown + 128, dk, 1.f, fk);
+    const int row = tile.z * kTileRows + me.row;
+    if (row < tile.y && wait.ok) {
+      const int64_t at = ((int64_t)(tile.x + row) * a.kv_heads + kv_head) * a.dim;
+      store_row<DP>(a.dk + at, dk, me.half, a.dim, 1.f, vec_out);
+      store_row<DP>(a.dv + at, dv, me.half, a.dim, 1.f, vec_out);
+    }
+  }
+  teardown(tmem);
+}
+
 // ------------------------------------------------------------ host side
 
 template <typename K>
@@ -668,6 +1012,27 @@ lmpb_status forward(const AttentionArgs& a, const Split& s, cudaStream_t st) {
   return launch_status("attention");
 }
 
+template <int DP>
+lmpb_status backward(const AttentionArgs& a, const Split& s, float* delta, cudaStream_t st) {
+  lmpb_status r = split<DP>(a, s, delta, st);
+  constexpr int bytes = BackwardLayout<DP>::kBytes;
+  if (r == LMPB_OK && a.dk) {
+    r = allow_smem(dkv_kernel<DP>, bytes);
+    if (r != LMPB_OK) return r;
+    const bool vec = a.dim % 4 == 0 && aligned16(a.dk) && aligned16(a.dv);
+    dkv_kernel<DP><<<(unsigned)(a.tiles * a.kv_heads), kThreadsKV, bytes, st>>>(a, s, vec);
+    r = launch_status("attention_backward (dk, dv)");
+  }
+  if (r == LMPB_OK && a.dq) {
+    r = allow_smem(dq_kernel<DP>, bytes);
+    if (r != LMPB_OK) return r;
+    const bool vec = a.dim % 4 == 0 && aligned16(a.dq);
+    dq_kernel<DP><<<(unsigned)(a.tiles * a.heads), kThreads, bytes, st>>>(a, s, vec);
+    r = launch_status("attention_backward (dq)");
+  }
+  return r;
+}
+
 }  // namespace
 
 bool attention_fits_sm100(const AttentionArgs& a) {
@@ -685,6 +1050,24 @@ lmpb_status attention_sm100(const AttentionArgs& args, cudaStream_t st) {
   r = dp == 64 ? forward<64>(a, s, st) : forward<128>(a, s, st);
   a.flags = s.flags;
   if (r == LMPB_OK) r = attention_simt(a, st);
+  const cudaError_t e = cudaFreeAsync(ws, st);
+  if (r == LMPB_OK && e != cudaSuccess)
+    return set_error(LMPB_ERR_CUDA, std::string("cudaFreeAsync: ") + cudaGetErrorString(e));
+  return r;
+}
+
+lmpb_status attention_sm100_backward(const AttentionArgs& args, cudaStream_t st) {
+  AttentionArgs a = args;
+  Split s{};
+  float* delta = nullptr;
+  void* ws = nullptr;
+  const int dp = a.dim <= 64 ? 64 : 128;
+  lmpb_status r = make_split(a, true, dp, s, &delta, &ws, st);
+  if (r != LMPB_OK) return r;
+  a.delta = delta;
+  r = dp == 64 ? backward<64>(a, s, delta, st) : backward<128>(a, s, delta, st);
+  a.flags = s.flags;
+  if (r == LMPB_OK) r = attention_simt_backward(a, st);
   const cudaError_t e = cudaFreeAsync(ws, st);
   if (r == LMPB_OK && e != cudaSuccess)
     return set_error(LMPB_ERR_CUDA, std::string("cudaFreeAsync: ") + cudaGetErrorString(e));
