@@ -21,11 +21,15 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
+#include <cstring>
 #include <numeric>
 #include <vector>
 
 #include "attention.cuh"
 
+#ifndef TENSOR_MIN
+#define TENSOR_MIN 64
+#endif
 namespace lmpb {
 namespace {
 
@@ -133,7 +137,7 @@ __device__ __forceinline__ float over16(float v, bool maximum) {
 // (backward) gradient heads.
 __device__ __forceinline__ bool any_flag(const AttentionArgs& a) {
   if (!a.flags) return true;
-  const int64_t n = ((int64_t)(a.grad ? 2 : 1) * a.heads + 2 * a.kv_heads) * a.tiles;
+  const int64_t n = ((int64_t)(a.grad ? 2 : 1) * a.heads + 2 * a.kv_heads) * a.flag_tiles;
   unsigned any = 0;
   for (int64_t i = threadIdx.x; i < n / 16; i += kThreads) {  // the array starts on a 16-byte boundary
     const uint4 f = reinterpret_cast<const uint4*>(a.flags)[i];
@@ -155,7 +159,7 @@ __device__ __forceinline__ bool wanted(const AttentionArgs& a, const int4& t, in
     const int plane = p < g          ? kv_head * g + p
                       : p < g + 2    ? a.heads + (p - g) * a.kv_heads + kv_head
                                      : a.heads + 2 * a.kv_heads + kv_head * g + (p - g - 2);
-    any |= a.flags[(int64_t)plane * a.tiles + t.w + i % n];
+    any |= a.flags[(int64_t)plane * a.flag_tiles + t.w + i % n];
   }
   return __syncthreads_or(any) != 0;
 }
@@ -404,6 +408,11 @@ lmpb_status attention_simt_backward(const AttentionArgs& a, cudaStream_t st) {
   return s;
 }
 
+void use_tiles(AttentionArgs& a, const lmpb_sequences_s* seqs, const lmpb_sequences_s::Tiles& t) {
+  a.tile = t.tile, a.by_queries = t.by_queries, a.by_keys = t.by_keys, a.tiles = t.count;
+  a.pack = seqs->pack, a.flag_tiles = seqs->packed.count;
+}
+
 namespace {
 
 lmpb_status check(const char* what, int64_t tokens, int heads, int kv_heads, int dim, float scale,
@@ -418,7 +427,7 @@ lmpb_status check(const char* what, int64_t tokens, int heads, int kv_heads, int
   LMPB_CHECK_ARG(seqs->tokens <= tokens, w + ": the sequences have " + std::to_string(seqs->tokens) +
                                              " tokens, the tensors " + std::to_string(tokens));
   int dev = 0;
-  if (seqs->tiles) {
+  if (seqs->plain.count) {
     LMPB_CUDA_TRY(cudaGetDevice(&dev));
     LMPB_CHECK_ARG(dev == seqs->device, w + ": the sequences are on device " + std::to_string(seqs->device) +
                                             ", the current device is " + std::to_string(dev));
@@ -429,7 +438,7 @@ lmpb_status check(const char* what, int64_t tokens, int heads, int kv_heads, int
 // Sequences of under 65 tokens leave half of every 128-row tile empty.
 bool on_tensor_cores(const AttentionArgs& a, const lmpb_sequences_s* seqs) {
   static const bool off = getenv("LMPB_ATTENTION_SIMT") != nullptr;  // A/B switch
-  return !off && seqs->longest > 64 && attention_fits_sm100(a);
+  return !off && seqs->longest > TENSOR_MIN && attention_fits_sm100(a);
 }
 
 // Rows behind the last sequence belong to nobody: 0.
@@ -458,24 +467,52 @@ extern "C" lmpb_status lmpb_sequences_create(const int64_t* lengths, int count, 
   lmpb_sequences_s* h = nullptr;
   try {
     h = new lmpb_sequences_s;
-    h->count = count;
     h->tokens = tokens;
     h->longest = longest;
-    h->tiles = (int)tiles;
-    std::vector<int> host((size_t)tiles * 6);
-    int4* tile = reinterpret_cast<int4*>(host.data());
-    int *byq = host.data() + 4 * tiles, *byk = byq + tiles, t = 0;
+    std::vector<int4> plain, packed;
+    std::vector<uchar2> pack;
     int64_t start = 0;
-    for (int i = 0; i < count; ++i) {
-      const int n = (int)((lengths[i] + kTileRows - 1) / kTileRows), first = t;
-      for (int k = 0; k < n; ++k) tile[t++] = make_int4((int)start, (int)lengths[i], k, first);
-      start += lengths[i];
+    for (int i = 0; i < count;) {
+      // whole sequences that fit one tile together, or one longer sequence
+      int end = i;
+      int64_t rows = 0;
+      while (end < count && (end == i || rows + lengths[end] <= kTileRows)) rows += lengths[end++];
+      const int first = (int)packed.size(), n = (int)((rows + kTileRows - 1) / kTileRows);
+      const bool shared = end - i > 1;
+      for (int k = 0; k < n; ++k) packed.push_back(make_int4((int)start, (int)rows, k, shared ? ~(int)(pack.size() / kTileRows) : first));
+      h->pair_tiles += (int64_t)n * (n + 1) / 2;
+      if (shared && n) {
+        const size_t at = pack.size();
+        pack.resize(at + kTileRows, make_uchar2(0, 0));
+        int64_t low = 0;
+        for (int q = i; q < end; low += lengths[q++])
+          for (int64_t r = low; r < low + lengths[q]; ++r) pack[at + r] = make_uchar2((unsigned char)low, (unsigned char)(low + lengths[q]));
+      }
+      for (; i < end; start += lengths[i++])
+        for (int k = 0; k < (int)((lengths[i] + kTileRows - 1) / kTileRows); ++k)
+          plain.push_back(make_int4((int)start, (int)lengths[i], k, first));
     }
-    std::iota(byq, byq + tiles, 0);
-    std::iota(byk, byk + tiles, 0);
-    const auto queries = [&](int x) { return (tile[x].y + kTileRows - 1) / kTileRows - tile[x].z; };
-    std::stable_sort(byq, byq + tiles, [&](int x, int y) { return tile[x].z > tile[y].z; });
-    std::stable_sort(byk, byk + tiles, [&](int x, int y) { return queries(x) > queries(y); });
+    // both lists of tiles with their two orders, then the bounds
+    std::vector<int> host;
+    size_t at[2];
+    for (int which = 0; which < 2; ++which) {
+      const std::vector<int4>& tile = which ? packed : plain;
+      const int n = (int)tile.size();
+      at[which] = host.size();
+      for (const int4& t : tile) host.insert(host.end(), {t.x, t.y, t.z, t.w});
+      std::vector<int> order(n);
+      std::iota(order.begin(), order.end(), 0);
+      std::stable_sort(order.begin(), order.end(), [&](int x, int y) { return tile[x].z > tile[y].z; });
+      host.insert(host.end(), order.begin(), order.end());
+      std::iota(order.begin(), order.end(), 0);
+      const auto queries = [&](int x) { return (tile[x].y + kTileRows - 1) / kTileRows - tile[x].z; };
+      std::stable_sort(order.begin(), order.end(), [&](int x, int y) { return queries(x) > queries(y); });
+      host.insert(host.end(), order.begin(), order.end());
+      host.resize((host.size() + 3) / 4 * 4);  // int4 boundary
+    }
+    const size_t pack_at = host.size();
+    host.resize(pack_at + pack.size() * sizeof(uchar2) / sizeof(int));
+    if (!pack.empty()) std::memcpy(host.data() + pack_at, pack.data(), pack.size() * sizeof(uchar2));
     if (tiles) {
       const size_t bytes = host.size() * sizeof(int);
       cudaError_t e = cudaGetDevice(&h->device);
@@ -487,9 +524,15 @@ extern "C" lmpb_status lmpb_sequences_create(const int64_t* lengths, int count, 
         delete h;
         return set_error(LMPB_ERR_CUDA, std::string("lmpb_sequences_create: ") + cudaGetErrorString(e));
       }
-      h->tile = static_cast<const int4*>(h->block);
-      h->by_queries = static_cast<const int*>(h->block) + 4 * tiles;
-      h->by_keys = h->by_queries + tiles;
+      const int* dev = static_cast<const int*>(h->block);
+      for (int which = 0; which < 2; ++which) {
+        lmpb_sequences_s::Tiles& t = which ? h->packed : h->plain;
+        t.count = (int)(which ? packed : plain).size();
+        t.tile = reinterpret_cast<const int4*>(dev + at[which]);
+        t.by_queries = dev + at[which] + 4 * t.count;
+        t.by_keys = t.by_queries + t.count;
+      }
+      h->pack = reinterpret_cast<const uchar2*>(dev + pack_at);
     }
   } catch (const std::exception& e) {
     delete h;
@@ -528,12 +571,15 @@ extern "C" lmpb_status lmpb_attention(const float* q, const float* k, const floa
   LMPB_CHECK_ARG(q && k && v && out && lse, "lmpb_attention: null pointer");
   cudaStream_t st = as_stream(stream);
   s = clear_tail(out, seqs->tokens, tokens, (int64_t)heads * head_dim, st);
-  if (s != LMPB_OK || seqs->tiles == 0) return s;
+  if (s != LMPB_OK || seqs->plain.count == 0) return s;
   AttentionArgs a{};
   a.q = q, a.k = k, a.v = v, a.out = out, a.lse = lse;
   a.tokens = tokens, a.heads = heads, a.kv_heads = kv_heads, a.dim = head_dim, a.scale = scale;
-  a.tile = seqs->tile, a.by_queries = seqs->by_queries, a.by_keys = seqs->by_keys, a.tiles = seqs->tiles;
-  return on_tensor_cores(a, seqs) ? attention_sm100(a, st) : attention_simt(a, st);
+  a.used = seqs->tokens, a.pair_tiles = seqs->pair_tiles, a.longest_tiles = (seqs->longest + kTileRows - 1) / kTileRows, a.splits = 1;
+  use_tiles(a, seqs, seqs->packed);
+  if (on_tensor_cores(a, seqs)) return attention_sm100(a, seqs, st);
+  use_tiles(a, seqs, seqs->plain);
+  return attention_simt(a, st);
 }
 
 extern "C" lmpb_status lmpb_attention_backward(const float* q, const float* k, const float* v, const float* out,
@@ -550,13 +596,15 @@ extern "C" lmpb_status lmpb_attention_backward(const float* q, const float* k, c
   s = clear_tail(dq, seqs->tokens, tokens, (int64_t)heads * head_dim, st);
   if (s == LMPB_OK) s = clear_tail(dk, seqs->tokens, tokens, (int64_t)kv_heads * head_dim, st);
   if (s == LMPB_OK) s = clear_tail(dv, seqs->tokens, tokens, (int64_t)kv_heads * head_dim, st);
-  if (s != LMPB_OK || seqs->tiles == 0) return s;
+  if (s != LMPB_OK || seqs->plain.count == 0) return s;
   AttentionArgs a{};
   a.q = q, a.k = k, a.v = v, a.out = const_cast<float*>(out), a.lse = const_cast<float*>(lse), a.grad = grad;
   a.dq = dq, a.dk = dk, a.dv = dv;
   a.tokens = tokens, a.heads = heads, a.kv_heads = kv_heads, a.dim = head_dim, a.scale = scale;
-  a.tile = seqs->tile, a.by_queries = seqs->by_queries, a.by_keys = seqs->by_keys, a.tiles = seqs->tiles;
-  if (on_tensor_cores(a, seqs)) return attention_sm100_backward(a, st);
+  a.used = seqs->tokens, a.pair_tiles = seqs->pair_tiles, a.longest_tiles = (seqs->longest + kTileRows - 1) / kTileRows, a.splits = 1;
+  use_tiles(a, seqs, seqs->packed);
+  if (on_tensor_cores(a, seqs)) return attention_sm100_backward(a, seqs, st);
+  use_tiles(a, seqs, seqs->plain);
   float* delta = nullptr;
   LMPB_CUDA_TRY(stream_alloc((void**)&delta, (size_t)tokens * heads * 4, st));
   const int64_t rows = seqs->tokens * heads;

@@ -19,13 +19,13 @@
 // 1. Split pass: a CTA per tile and head plane writes the tile's hi and lo as
 //    one block in the very layout the MMAs read from shared memory (128-byte
 //    swizzled rows of 64 halves), so the kernels fetch operands with plain
-//    bulk copies of up to 32 KB, no tensor maps.  Tiles never span sequences and rows
+//    bulk copies, no tensor maps.  Tiles never span sequences and rows
 //    behind a sequence are 0.  For v and grad it also finds the largest row
 //    norm, for grad the row sums delta = sum(grad * out).
 // 2. forward_kernel, dq_kernel, dkv_kernel: one CTA per tile and head, one
-//    CTA per SM.  Warp 0 feeds a ring of 32 KB stages, warp 1 issues the
-//    MMAs, 8 warps compute.  A row of the 128 x 128 score tile lives in one
-//    TMEM lane; two threads of different warps share it, 64 columns each.
+//    CTA per SM.  Warp 0 feeds a ring of 16 KB units, warp 1 issues the
+//    MMAs, 8 or 16 warps compute.  A row of the 128 x 128 score tile lives in one
+//    TMEM lane; two or four threads of different warps share it.
 //    Scores are overwritten in place by the split weights, which are then the
 //    next MMA's A operand straight from TMEM.
 //    Every mbarrier wait is bounded; after one expires the thread stops
@@ -47,7 +47,6 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kWeightBits = 14.f;  // weights enter the MMA times 2^14
-constexpr int kStage = 32768;
 
 __device__ unsigned int g_attention_error = 0;
 
@@ -67,6 +66,11 @@ template <int DP>
 constexpr int part_bytes() { return DP / 64 * 128 * 128; }
 template <int DP>
 constexpr int block_bytes() { return 2 * part_bytes<DP>(); }
+
+constexpr int kMaxSplits = 16;
+
+// The first tile of tile t's sequence.
+__device__ __forceinline__ int first_tile(const int4& tile, int t) { return tile.w < 0 ? t : tile.w; }
 
 // Where the split pass puts things.  Planes: query heads, key heads, value
 // heads, gradient heads; a plane's tile t is block plane * tiles + t.
@@ -205,29 +209,38 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
-// 128-byte swizzled operand tiles, 8-row atoms 1024 bytes apart; `lbo`: the
-// stride between 64-column groups of an operand whose rows are the K axis.
-__device__ __forceinline__ uint64_t desc128(uint32_t addr, uint32_t lbo) {
-  return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
-         (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
+// Descriptors of 128-byte swizzled operand tiles with 8-row atoms 1024 bytes
+// apart.  The high word is always the same; the low one holds the address and
+// `lbo`, the stride between 64-column groups of an operand whose rows are the K axis.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return (addr & 0x3FFFF) >> 4 | (lbo >> 4) << 16; }
+constexpr uint32_t kDescHi = (1024 >> 4) | 1u << 14 | 2u << 29;
 
 // f16 operands, fp32 accumulators, M = 128; B K-major, or with K as its rows.
 constexpr uint32_t idesc_of(int n, bool b_rows) {
   return (1u << 4) | ((b_rows ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// a and b: low descriptor words, or a TMEM address for a.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %4, 0;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHi)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p;\n .reg .b64 y;\n setp.ne.b32 p, %4, 0;\n mov.b64 y, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHi)
       : "memory");
+}
+
+// One lane of a converged warp, the same at every call.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+  return p != 0;
 }
 
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -254,129 +267,188 @@ __device__ __forceinline__ void warp_wait(Waiter& wait, uint32_t bar, uint32_t p
   tc_fence_after();
 }
 
-// Barrier of the 256 computing threads.
-__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+// Barrier of the computing warps.
+template <int WARPS>
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); }
 
 // ------------------------------------------------------------ operand feed
 //
-// The ring carries, per operand tile, either its columns (the operand is
-// contracted over D: stage c holds hi and lo of columns [64 c, 64 c + 64) of
-// all 128 rows) or its rows (contracted over tokens: stage r holds hi and lo
-// of rows [64 r, 64 r + 64), all columns).  With DP = 64 a tile is one stage
-// that serves as either.
+// The ring carries parts: all of a tile's lo, then all of its hi, one bulk
+// copy each.  The same bytes serve as an operand contracted over D (its rows
+// are the product's columns) and as one contracted over tokens (its rows are
+// the K axis); only the descriptors differ.  The lo part comes first: the
+// accumulator is still small while the two cross products are added, so
+// their roundings are, and the lo part is free again after one product.
 
-template <int DP>
-constexpr int stages_per_tile() { return DP / 64; }
-
+// Position in a ring of N parts; full and empty barriers are 8 bytes each,
+// all full ones first.
+template <int DP, int N>
 struct Ring {
-  uint32_t base, full, empty;  // shared addresses; 8-byte barriers
-  int n;
-  uint32_t it = 0;
-  __device__ __forceinline__ uint32_t stage() const { return base + (it % n) * kStage; }
-  __device__ __forceinline__ uint32_t full_bar() const { return full + (it % n) * 8; }
-  __device__ __forceinline__ uint32_t empty_bar() const { return empty + (it % n) * 8; }
-  __device__ __forceinline__ uint32_t phase() const { return (it / n) & 1; }
+  uint32_t parts, bars;  // shared addresses
+  uint32_t slot = 0, phase = 0, started = 0;
+  __device__ __forceinline__ uint32_t part() const { return parts + slot * part_bytes<DP>(); }
+  __device__ __forceinline__ uint32_t full() const { return bars + slot * 8; }
+  __device__ __forceinline__ uint32_t empty() const { return bars + (N + slot) * 8; }
+  __device__ __forceinline__ void next() {
+    if (++slot == N) slot = 0, phase ^= 1;
+  }
 };
 
-template <int DP>
-__device__ __forceinline__ void feed(Ring& ring, Waiter& wait, const unsigned char* block, bool rows) {
-#pragma unroll 1
-  for (int s = 0; s < stages_per_tile<DP>(); ++s) {
-    if (!wait(ring.empty_bar(), ring.phase() ^ 1)) return;
-    const uint32_t bar = ring.full_bar(), dst = ring.stage();
-    mbar_expect_tx(bar, kStage);
-    if (DP == 64) {
-      bulk_load(dst, block, kStage, bar);
-    } else if (!rows) {
-      bulk_load(dst, block + s * 16384, 16384, bar);
-      bulk_load(dst + 16384, block + part_bytes<DP>() + s * 16384, 16384, bar);
-    } else {
+template <int DP, int N>
+__device__ __forceinline__ void feed(Ring<DP, N>& ring, Waiter& wait, const unsigned char* block) {
 #pragma unroll
-      for (int part = 0; part < 2; ++part)
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          bulk_load(dst + part * 16384 + c * 8192, block + part * part_bytes<DP>() + c * 16384 + s * 8192, 8192, bar);
-    }
-    ++ring.it;
+  for (int part = 1; part >= 0; --part) {
+    if (!wait(ring.empty(), ring.phase ^ 1)) return;
+    mbar_expect_tx(ring.full(), part_bytes<DP>());
+    bulk_load(ring.part(), block + part * part_bytes<DP>(), part_bytes<DP>(), ring.full());
+    ring.next();
+    ++ring.started;
   }
 }
 
 // After the last feed: every copy that was started has landed.
-__device__ __forceinline__ void feed_done(const Ring& ring) {
-  const uint32_t n = min(ring.it, (uint32_t)ring.n);
-  for (uint32_t i = 0; i < n; ++i) {
-    const uint32_t k = ring.it - 1 - i;
+template <int DP, int N>
+__device__ __forceinline__ void feed_done(Ring<DP, N> ring) {
+  const uint32_t n = min(ring.started, (uint32_t)N);
+  for (uint32_t k = 0; k < n; ++k) {
+    if (ring.slot == 0) ring.slot = N, ring.phase ^= 1;
+    --ring.slot;
     Waiter wait(31);
-    wait(ring.full + (k % ring.n) * 8, (k / ring.n) & 1);
+    wait(ring.full(), ring.phase);
   }
 }
 
-// D[128, 128] = A (shared, resident block) . B^T (a tile's columns from the ring).
-template <int DP>
-__device__ __forceinline__ void mma_columns(uint32_t d, uint32_t a_block, Ring& ring, Waiter& wait) {
-  constexpr uint32_t idesc = idesc_of(128, false);
-#pragma unroll 1
-  for (int s = 0; s < stages_per_tile<DP>(); ++s) {
-    if (!wait(ring.full_bar(), ring.phase())) return;
-    tc_fence_after();
-    const uint32_t b = ring.stage(), a = a_block + s * 16384;
-    const uint64_t ah = desc128(a, 16), al = desc128(a + part_bytes<DP>(), 16), bh = desc128(b, 16), bl = desc128(b + 16384, 16);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {  // 16 halves = 32 bytes a step
-      mma_ss(d, al + 2 * k, bh + 2 * k, idesc, s || k);
-      mma_ss(d, ah + 2 * k, bl + 2 * k, idesc, 1);
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) mma_ss(d, ah + 2 * k, bh + 2 * k, idesc, 1);
-    mma_commit(ring.empty_bar());
-    ++ring.it;
-  }
-}
+// The MMA warp.  An elected lane issues; the whole warp runs along, so that
+// addresses stay in uniform registers.  The tensor core's queue holds a few
+// MMAs of 64 clocks, and a wait costs the issuing warp 100 clocks and more
+// even where nothing is to be waited for, so waits are done while MMAs are
+// still queued: the next operand's barrier (and what `ahead` tests) is looked
+// at before the last third of a product is issued.  With each wait at the
+// place of its need the tensor core idled 1,300 of 4,300 clocks a key block.
+template <int DP, int N>
+struct Issuer {
+  Ring<DP, N> ring;
+  Waiter wait;
+  bool landed = false;  // the ring's next part, as far as is known
 
-// D[128, DP] = W . B, W the split weights in TMEM (16 columns for 16 tokens:
-// 8 of hi, 8 of lo), B a tile's rows from the ring.
-template <int DP>
-__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t w, Ring& ring, Waiter& wait) {
-  constexpr uint32_t idesc = idesc_of(DP, true);
-  constexpr int N = stages_per_tile<DP>(), STEPS = 8 / N;
-#pragma unroll 1
-  for (int s = 0; s < N; ++s) {
-    if (!wait(ring.full_bar(), ring.phase())) return;
+  __device__ __forceinline__ Issuer(uint32_t parts, uint32_t bars, unsigned code) : ring{parts, bars}, wait(code) {}
+
+  // Lanes agree on the outcome; what the barrier orders is visible to the MMAs.
+  __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
+    wait(bar, parity);
+    wait.ok = __all_sync(0xffffffffu, wait.ok);
     tc_fence_after();
-    const uint32_t b = ring.stage(), ws = w + s * STEPS * 16;
-    const uint64_t bh = desc128(b, 8192), bl = desc128(b + 16384, 8192);
-#pragma unroll
-    for (int k = 0; k < STEPS; ++k) {  // 16 rows = 2 atoms = 2048 bytes a step
-      mma_ts(d, ws + k * 16 + 8, bh + 128 * k, idesc, s || k);
-      mma_ts(d, ws + k * 16, bl + 128 * k, idesc, 1);
-    }
-#pragma unroll
-    for (int k = 0; k < STEPS; ++k) mma_ts(d, ws + k * 16, bh + 128 * k, idesc, 1);
-    mma_commit(ring.empty_bar());
-    ++ring.it;
+    return wait.ok;
   }
+  __device__ __forceinline__ bool test(uint32_t bar, uint32_t parity) const {
+    return __all_sync(0xffffffffu, mbar_test(bar, parity));
+  }
+  __device__ __forceinline__ bool take() {
+    if (landed) tc_fence_after();
+    else if (!wait_for(ring.full(), ring.phase)) return false;
+    landed = false;
+    return true;
+  }
+
+  // D[128, 128] = A (shared, resident block) . B^T, B the ring's next tile.
+  template <typename Ahead>
+  __device__ __forceinline__ void columns(uint32_t d, uint32_t a_block, Ahead ahead) {
+    constexpr uint32_t idesc = idesc_of(128, false);
+    constexpr int U = DP / 64;
+    const uint32_t ah = desc_lo(a_block, 16), al = ah + (part_bytes<DP>() >> 4);
+    product<4 * U>([&](uint32_t b, int k, bool lo_a, uint32_t acc) {  // 16 columns = 32 bytes a step, 64 a swizzle atom
+      const uint32_t o = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
+      mma_ss(d, (lo_a ? al : ah) + o, b + o, idesc, acc);
+    }, 16, ahead);
+  }
+
+  // D[128, DP] = W . B, W the split weights in TMEM (16 columns for 16
+  // tokens: 8 of hi, 8 of lo), B the ring's next tile.
+  template <typename Ahead>
+  __device__ __forceinline__ void rows(uint32_t d, uint32_t w, Ahead ahead) {
+    constexpr uint32_t idesc = idesc_of(DP, true);
+    product<8>([&](uint32_t b, int k, bool lo_w, uint32_t acc) {  // 16 rows = 2048 bytes a step
+      mma_ts(d, w + k * 16 + (lo_w ? 8 : 0), b + k * (2048 >> 4), idesc, acc);
+    }, 16384, ahead);
+  }
+
+  template <int STEPS, typename Mma, typename Ahead>
+  __device__ __forceinline__ void product(Mma mma, uint32_t lbo, Ahead ahead) {
+    if (!take()) return;
+    uint32_t b = desc_lo(ring.part(), lbo);
+    if (elect_one()) {
+#pragma unroll
+      for (int k = 0; k < STEPS; ++k) mma(b, k, false, k != 0);
+      mma_commit(ring.empty());
+    }
+    __syncwarp();
+    ring.next();
+    if (!wait_for(ring.full(), ring.phase)) return;
+    b = desc_lo(ring.part(), lbo);
+    if (elect_one()) {
+#pragma unroll
+      for (int k = 0; k < STEPS; ++k) mma(b, k, true, 1);
+    }
+    __syncwarp();
+    const uint32_t free_bar = ring.empty();
+    ring.next();
+    landed = test(ring.full(), ring.phase);
+    ahead();
+    if (elect_one()) {
+#pragma unroll
+      for (int k = 0; k < STEPS; ++k) mma(b, k, false, 1);
+      mma_commit(free_bar);
+    }
+    __syncwarp();
+  }
+};
+
+// Signals `bar` when every product issued so far is done.
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if (elect_one()) mma_commit(bar);
+  __syncwarp();
 }
 
 // ------------------------------------------------------------ shared memory
 
 constexpr int kBars = 48;
 
-template <int DP, int RESIDENT, int RING>
+// A kernel's warps: four that feed, issue or idle, then W that compute, four
+// of them to each share of a score row's columns.  The launch gives every
+// warp the same registers (what __launch_bounds__ leaves, LAUNCH); the first
+// four keep LOW of theirs so that the others can have HIGH.
+template <int W, int LAUNCH, int LOW, int HIGH>
+struct Warps {
+  static constexpr int kWarps = W, kParts = W / 4, kCols = 128 / kParts, kThreads = (4 + W) * 32;
+  static_assert(4 * LOW + W * HIGH <= (4 + W) * LAUNCH, "more registers than the launch has");
+  static __device__ __forceinline__ void few() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(LOW)); }
+  static __device__ __forceinline__ void many() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(HIGH)); }
+};
+using Warps8 = Warps<8, 168, 88, 208>;
+using Warps16 = Warps<16, 96, 56, 104>;
+// Forward with DP = 64, where the weights' arithmetic bounds: 16 warps, 0.446
+// ms for [8192] x 16 heads (8 warps: 0.467); with DP = 128, where the tensor
+// core does, 8 warps: 1.24 ms for [16384] x 8 (16: 1.25; that backward: 4.94, 5.10).
+template <int DP>
+using ForwardWarps = std::conditional_t<DP == 64, Warps16, Warps8>;
+
+template <int DP, int RESIDENT, int RING, int SCRATCH>
 struct Layout {
   static constexpr int kRing = RESIDENT * block_bytes<DP>();
-  static constexpr int kBarsAt = kRing + RING * kStage;
+  static constexpr int kBarsAt = kRing + RING * part_bytes<DP>();
   static constexpr int kScratch = kBarsAt + kBars * 8 + 16;
-  static constexpr int kBytes = kScratch + 2048;
+  static constexpr int kBytes = kScratch + SCRATCH;
+  static_assert(kBytes <= 232448, "over 227 KB of shared memory");
 };
 
 template <int DP>
-constexpr int forward_ring() { return DP == 64 ? 4 : 5; }
+constexpr int forward_ring() { return DP == 64 ? 8 : 5; }
 template <int DP>
-constexpr int backward_ring() { return DP == 64 ? 4 : 3; }
+constexpr int backward_ring() { return DP == 64 ? 8 : 3; }
 template <int DP>
-using ForwardLayout = Layout<DP, 1, forward_ring<DP>()>;
+using ForwardLayout = Layout<DP, 1, forward_ring<DP>(), 2 * ForwardWarps<DP>::kParts * 128 * 4>;
 template <int DP>
-using BackwardLayout = Layout<DP, 2, backward_ring<DP>()>;
+using BackwardLayout = Layout<DP, 2, backward_ring<DP>(), 2048>;
 
 // Sets up the barriers and all of TMEM; every thread calls it.  False (for
 // all) when the shared memory does not start on a swizzle atom.
@@ -400,6 +472,12 @@ __device__ __forceinline__ bool setup(unsigned char* smem, uint32_t bars, uint32
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (*slot != 0) {  // 512 columns can only start at 0
+    if (warp == 1)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(*slot) : "memory");
+    if (threadIdx.x == 0) atomicCAS(&g_attention_error, 0u, 98u);
+    return false;
+  }
   return true;
 }
 
@@ -412,51 +490,53 @@ __device__ __forceinline__ void teardown(uint32_t tmem) {
   }
 }
 
-// What a computing thread is: warps 2..9, TMEM lane quarter warp % 4, so rows
-// quarter * 32 + lane; the first four warps take columns 0..63 of a score row
-// (and the first half of D), the others the rest.
+// What a computing thread is.  TMEM lane quarter warp % 4, so rows quarter * 32
+// + lane; each four warps in a row take the next PARTS-th of a score row's
+// columns and of D.
+template <int PARTS>
 struct Who {
-  int row, half;
+  int row, part;
   uint32_t lanes;  // TMEM lane offset of this warp's quarter
   __device__ __forceinline__ explicit Who(int first_warp) {
     const int warp = threadIdx.x >> 5;
     row = (warp & 3) * 32 + (threadIdx.x & 31);
-    half = (warp - first_warp) >> 2;
+    part = (warp - first_warp) >> 2;
     lanes = (uint32_t)((warp & 3) * 32) << 16;
   }
 };
 
-// acc += (or, with `scale_acc`, acc * alpha +) f * this thread's D columns of a drained block.
-template <int DP>
-__device__ __forceinline__ void drain(uint32_t taddr, float (&acc)[DP / 2], float alpha, float f) {
+// A computing warp is done with what `bar` guards (one arrival a warp).
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+  tc_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+// acc = acc * alpha + f * this thread's C columns of a drained block.
+template <int C>
+__device__ __forceinline__ void drain(uint32_t taddr, float (&acc)[C], float alpha, float f) {
 #pragma unroll
-  for (int c = 0; c < DP / 2; c += 32) {
-    uint32_t r[16], u[16];
+  for (int c = 0; c < C; c += 16) {
+    uint32_t r[16];
     tmem_ld16_issue(taddr + c, r);
-    tmem_ld16_issue(taddr + c + 16, u);
     tmem_ld_wait();
     tmem_regs_ready(r);
-    tmem_regs_ready(u);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      acc[c + i] = fmaf(__uint_as_float(r[i]), f, acc[c + i] * alpha);
-      acc[c + 16 + i] = fmaf(__uint_as_float(u[i]), f, acc[c + 16 + i] * alpha);
-    }
+    for (int i = 0; i < 16; ++i) acc[c + i] = fmaf(__uint_as_float(r[i]), f, acc[c + i] * alpha);
   }
 }
 
-// One row's share of a result: DP / 2 values of columns [half * DP / 2, ...).
-template <int DP>
-__device__ __forceinline__ void store_row(float* p, const float (&acc)[DP / 2], int half, int dim, float f, bool vec) {
-  const int c0 = half * (DP / 2);
+// One row's share of a result: columns [c0, c0 + C).
+template <int C>
+__device__ __forceinline__ void store_row(float* p, const float (&acc)[C], int c0, int dim, float f, bool vec) {
   if (vec) {
 #pragma unroll
-    for (int c = 0; c < DP / 2; c += 4)
+    for (int c = 0; c < C; c += 4)
       if (c0 + c < dim)
         *reinterpret_cast<float4*>(p + c0 + c) = make_float4(acc[c] * f, acc[c + 1] * f, acc[c + 2] * f, acc[c + 3] * f);
   } else {
 #pragma unroll
-    for (int c = 0; c < DP / 2; ++c)
+    for (int c = 0; c < C; ++c)
       if (c0 + c < dim) p[c0 + c] = acc[c] * f;
   }
 }
@@ -464,159 +544,155 @@ __device__ __forceinline__ void store_row(float* p, const float (&acc)[DP / 2], 
 // ------------------------------------------------------------ forward
 //
 // TMEM: scores of even and odd key blocks in columns [0, 128) and [128, 256),
-// the block's product with v in [256, 256 + DP).  While the computing warps
+// their products with v in [256, 256 + DP) and [384, 384 + DP).  While the computing warps
 // turn block j's scores into weights, the MMAs of block j + 1's scores run.
 
-constexpr int kThreads = 320;
-
 template <int DP>
-__global__ void __launch_bounds__(kThreads, 1) forward_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
+__global__ void __launch_bounds__(ForwardWarps<DP>::kThreads, 1) forward_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
   extern __shared__ __align__(1024) unsigned char smem[];
   using L = ForwardLayout<DP>;
+  using W = ForwardWarps<DP>;
+  constexpr int WARPS = W::kWarps, PARTS = W::kParts, COLS = W::kCols;
   constexpr int RING = forward_ring<DP>();
   const uint32_t base = smem_u32(smem), bars = base + L::kBarsAt;
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + L::kBarsAt + kBars * 8);
-  float* xch = reinterpret_cast<float*>(smem + L::kScratch);  // [2][2][128]
-  // q, scores of each parity, weights, product, product drained, end
-  const int counts[7] = {1, 1, 1, 256, 1, 256, 1};
+  float* xch = reinterpret_cast<float*>(smem + L::kScratch);  // [2][PARTS][128]
+  // q, scores of each parity, weights, product of each parity, end
+  const int counts[7] = {1, 1, 1, WARPS, 1, 1, 1};
   if (!setup(smem, bars, slot, RING, counts, 7)) return;
-  const uint32_t qfull = bars + 16 * RING, sfull = qfull + 8, pfull = qfull + 24, ofull = qfull + 32,
-                 oempty = qfull + 40, done = qfull + 48;
-  const uint32_t tmem = *slot;
+  const uint32_t qfull = bars + 16 * RING, sfull = qfull + 8, pfull = qfull + 24, ofull = qfull + 32, done = qfull + 48;
+  constexpr uint32_t tmem = 0;  // all of it was allocated
   const int order = blockIdx.x / a.heads, head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
   const int t = a.by_queries[order];
   const int4 tile = a.tile[t];
   const int n = tile.z + 1;  // key blocks
-  const int64_t kplane = (int64_t)(a.heads + kv_head) * a.tiles + tile.w;
+  const int64_t kplane = (int64_t)(a.heads + kv_head) * a.tiles + first_tile(tile, t);
   const int64_t vplane = kplane + (int64_t)a.kv_heads * a.tiles;
   const int64_t qblock = (int64_t)head * a.tiles + t;
   const int warp = threadIdx.x >> 5;
-  if (warp == 0) {
-    if ((threadIdx.x & 31) == 0) {
-      Ring ring{base + L::kRing, bars, bars + 8 * RING, RING};
+  if (warp < 4) {
+    W::few();
+    if (warp == 0 && (threadIdx.x & 31) == 0) {
+      Ring<DP, RING> ring{base + L::kRing, bars};
       Waiter wait(1);
       mbar_expect_tx(qfull, block_bytes<DP>());
       bulk_load(base, sp.blocks + qblock * block_bytes<DP>(), block_bytes<DP>(), qfull);
-      feed<DP>(ring, wait, sp.blocks + kplane * block_bytes<DP>(), false);
+      feed(ring, wait, sp.blocks + kplane * block_bytes<DP>());
       for (int j = 0; j < n; ++j) {
-        if (j + 1 < n) feed<DP>(ring, wait, sp.blocks + (kplane + j + 1) * block_bytes<DP>(), false);
-        feed<DP>(ring, wait, sp.blocks + (vplane + j) * block_bytes<DP>(), true);
+        if (j + 1 < n) feed(ring, wait, sp.blocks + (kplane + j + 1) * block_bytes<DP>());
+        feed(ring, wait, sp.blocks + (vplane + j) * block_bytes<DP>());
       }
       feed_done(ring);
       Waiter last(32);
       last(qfull, 0);
-    }
-  } else if (warp == 1) {
-    if ((threadIdx.x & 31) == 0) {
-      Ring ring{base + L::kRing, bars, bars + 8 * RING, RING};
-      Waiter wait(2);
-      wait(qfull, 0);
-      mma_columns<DP>(tmem, base, ring, wait);
-      mma_commit(sfull);
-      for (int j = 0; j < n && wait.ok; ++j) {
-        if (j + 1 < n) {
-          mma_columns<DP>(tmem + ((j + 1) & 1) * 128, base, ring, wait);
-          mma_commit(sfull + 8 * ((j + 1) & 1));
-        }
-        wait(pfull, j & 1);
-        wait(oempty, (j & 1) ^ 1);
-        tc_fence_after();
-        if (wait.ok) mma_rows<DP>(tmem + 256, tmem + (j & 1) * 128, ring, wait);
-        mma_commit(ofull);
+    } else if (warp == 1) {
+    Issuer<DP, RING> mma(base + L::kRing, bars, 2);
+    const auto nothing = [] {};
+    mma.wait_for(qfull, 0);
+    mma.columns(tmem, base, nothing);
+    commit(sfull);
+    for (int j = 0; j < n && mma.wait.ok; ++j) {
+      // block j's weights; that they are there also says that block j - 2's product is drained
+      bool weights = false;
+      if (j + 1 < n) {
+        mma.columns(tmem + ((j + 1) & 1) * 128, base, [&] { weights = mma.test(pfull, j & 1); });
+        commit(sfull + 8 * ((j + 1) & 1));
       }
-      Waiter last(33);  // nothing of this CTA is in flight when it ends
-      mma_commit(done);
-      last(done, 0);
+      if (!weights) mma.wait_for(pfull, j & 1);
+      else tc_fence_after();
+      if (mma.wait.ok) mma.rows(tmem + 256 + (j & 1) * 128, tmem + (j & 1) * 128, nothing);
+      commit(ofull + 8 * (j & 1));
+    }
+    Waiter last(33);  // nothing of this CTA is in flight when it ends
+    commit(done);
+    last(done, 0);
     }
   } else {
-    const Who me(2);
+    W::many();
+    constexpr int C = DP / PARTS;
+    const Who<PARTS> me(4);
     Waiter wait(3);
-    float acc[DP / 2], m = -INFINITY, l = 0.f, alpha = 0.f, of = 0.f;
+    float acc[C], m = -INFINITY, l = 0.f, alpha = 0.f, of = 0.f;
 #pragma unroll
-    for (int i = 0; i < DP / 2; ++i) acc[i] = 0.f;
+    for (int i = 0; i < C; ++i) acc[i] = 0.f;
     const int eq = sp.expo[qblock];
     int ek = sp.expo[kplane], ev = sp.expo[vplane];
-    const uint32_t own = tmem + me.lanes + me.half * 64, oown = tmem + 256 + me.lanes + me.half * (DP / 2);
+    // of the last block a row sees columns low..row, low its sequence's first:
+    // this thread's column i if unsigned(col0 + i) < span
+    const int low = a.low_of(tile, me.row), col0 = me.part * COLS - low;
+    const unsigned span = me.row - low + 1;
+    const uint32_t own = tmem + me.lanes + me.part * COLS, oown = tmem + 256 + me.lanes + me.part * C;
     for (int j = 0; j < n; ++j) {
       const float c = ldexpf(a.scale * kLog2e, -(eq + ek));
       const float f = two_to(-ev);
       if (j + 1 < n) ek = sp.expo[kplane + j + 1], ev = sp.expo[vplane + j + 1];
       const uint32_t s = own + (j & 1) * 128;
-      // columns this row sees: all but in the last block, where column <= row
       const bool diag = j + 1 == n;
-      const int see = diag ? me.row - me.half * 64 + 1 : 64;
       warp_wait(wait, sfull + 8 * (j & 1), (j >> 1) & 1);
+      uint32_t r[COLS / 16][16];
+#pragma unroll
+      for (int k = 0; k < COLS / 16; ++k) tmem_ld16_issue(s + 16 * k, r[k]);
+      tmem_ld_wait();
       float mx = -INFINITY;
 #pragma unroll
-      for (int k = 0; k < 64; k += 32) {
-        uint32_t r[16], u[16];
-        tmem_ld16_issue(s + k, r);
-        tmem_ld16_issue(s + k + 16, u);
-        tmem_ld_wait();
-        tmem_regs_ready(r);
-        tmem_regs_ready(u);
-        if (!diag) {
+      for (int k = 0; k < COLS / 16; ++k) {
+        tmem_regs_ready(r[k]);
+        if (diag) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(r[i]), __uint_as_float(u[i])));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (k + i < see) mx = fmaxf(mx, __uint_as_float(r[i]));
-            if (k + 16 + i < see) mx = fmaxf(mx, __uint_as_float(u[i]));
-          }
+          for (int i = 0; i < 16; ++i)
+            if (unsigned(col0 + 16 * k + i) >= span) r[k][i] = 0xff800000u;  // -inf
         }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, __uint_as_float(r[k][i]));
       }
-      float* x = xch + (j & 1) * 256;
-      x[me.half * 128 + me.row] = mx;
-      compute_sync();
-      mx = fmaxf(mx, x[(me.half ^ 1) * 128 + me.row]);
-      const float mn = fmaxf(m, mx * c);  // finite: every row sees key 0 of the first block
+      float* x = xch + (j & 1) * (128 * PARTS) + me.row;
+      x[me.part * 128] = mx;
+      compute_sync<WARPS>();
+#pragma unroll
+      for (int k = 0; k < PARTS; ++k) mx = fmaxf(mx, x[k * 128]);
+      const float mn = fmaxf(m, mx * c);  // finite: the first block has a key for every row
       const float next = exp2_fast(m - mn), bias = kWeightBits - mn;
       float sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < 64; k += 16) {
-        uint32_t r[16], w[16];
-        tmem_ld16_issue(s + k, r);
-        tmem_ld_wait();
-        tmem_regs_ready(r);
+      for (int k = 0; k < COLS / 16; ++k) {
+        uint32_t w[16];
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          float p0 = exp2_fast(fmaf(__uint_as_float(r[i]), c, bias));
-          float p1 = exp2_fast(fmaf(__uint_as_float(r[i + 1]), c, bias));
-          if (diag) {
-            if (k + i >= see) p0 = 0.f;
-            if (k + i + 1 >= see) p1 = 0.f;
+          float p0 = exp2_fast(fmaf(__uint_as_float(r[k][i]), c, bias));
+          float p1 = exp2_fast(fmaf(__uint_as_float(r[k][i + 1]), c, bias));
+          if (diag) {  // by index: a scale of 0 makes NaN of -inf
+            if (unsigned(col0 + 16 * k + i) >= span) p0 = 0.f;
+            if (unsigned(col0 + 16 * k + i + 1) >= span) p1 = 0.f;
           }
           sum += p0 + p1;
           split2(p0, p1, w[i / 2], w[8 + i / 2]);
         }
-        tmem_st16(s + k, w);
+        tmem_st16(s + 16 * k, w);
       }
       tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(pfull);
+      warp_arrive(pfull);
       l = l * next + sum;
       m = mn;
       if (j > 0) {
-        warp_wait(wait, ofull, (j - 1) & 1);
-        drain<DP>(oown, acc, alpha, of);
-        tc_fence_before();
-        mbar_arrive(oempty);
+        warp_wait(wait, ofull + 8 * ((j - 1) & 1), ((j - 1) >> 1) & 1);
+        drain<C>(oown + ((j - 1) & 1) * 128, acc, alpha, of);
       }
       alpha = next;
       of = f;
     }
-    warp_wait(wait, ofull, (n - 1) & 1);
-    drain<DP>(oown, acc, alpha, of);
-    float* x = xch + (n & 1) * 256;
-    x[me.half * 128 + me.row] = l;
-    compute_sync();
-    l = x[me.row] + x[128 + me.row];
+    warp_wait(wait, ofull + 8 * ((n - 1) & 1), ((n - 1) >> 1) & 1);
+    drain<C>(oown + ((n - 1) & 1) * 128, acc, alpha, of);
+    float* x = xch + (n & 1) * (128 * PARTS) + me.row;
+    x[me.part * 128] = l;
+    compute_sync<WARPS>();
+    l = 0.f;
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) l += x[k * 128];
     const int row = tile.z * kTileRows + me.row;
     if (row < tile.y && wait.ok) {
       const int64_t at = tile.x + row;
-      store_row<DP>(a.out + (at * a.heads + head) * a.dim, acc, me.half, a.dim, __frcp_rn(l), vec_out);
-      if (me.half == 0) a.lse[(int64_t)head * a.tokens + at] = (m + log2f(l) - kWeightBits) * kLn2;
+      store_row<C>(a.out + (at * a.heads + head) * a.dim, acc, me.part * C, a.dim, __frcp_rn(l), vec_out);
+      if (me.part == 0) a.lse[(int64_t)head * a.tokens + at] = (m + log2f(l) - kWeightBits) * kLn2;
     }
   }
   teardown(tmem);
@@ -646,79 +722,83 @@ __device__ __forceinline__ DsScale ds_scale(float gnorm, float vnorm, float dmax
 // with k in [384, 384 + DP).  Block j + 1's scores run while the computing
 // warps turn block j's scores and dP into dS.
 template <int DP>
-__global__ void __launch_bounds__(kThreads, 1) dq_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
+__global__ void __launch_bounds__(Warps8::kThreads, 1) dq_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
   extern __shared__ __align__(1024) unsigned char smem[];
   using L = BackwardLayout<DP>;
+  using W = Warps8;
+  constexpr int WARPS = W::kWarps, PARTS = W::kParts, COLS = W::kCols;
   constexpr int RING = backward_ring<DP>();
   const uint32_t base = smem_u32(smem), bars = base + L::kBarsAt;
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + L::kBarsAt + kBars * 8);
   // q and grad, scores and dP, dS, product, product drained, end
-  const int counts[6] = {1, 1, 256, 1, 256, 1};
+  const int counts[6] = {1, 1, WARPS, 1, WARPS, 1};
   if (!setup(smem, bars, slot, RING, counts, 6)) return;
   const uint32_t resident = bars + 16 * RING, spfull = resident + 8, dsfull = resident + 16, ofull = resident + 24,
                  oempty = resident + 32, done = resident + 40;
-  const uint32_t tmem = *slot;
+  constexpr uint32_t tmem = 0;  // all of it was allocated
   const int order = blockIdx.x / a.heads, head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
   const int t = a.by_queries[order];
   const int4 tile = a.tile[t];
   const int n = tile.z + 1;  // key blocks
-  const int64_t kplane = (int64_t)(a.heads + kv_head) * a.tiles + tile.w;
+  const int64_t kplane = (int64_t)(a.heads + kv_head) * a.tiles + first_tile(tile, t);
   const int64_t vplane = kplane + (int64_t)a.kv_heads * a.tiles;
   const int64_t qblock = (int64_t)head * a.tiles + t;
   const int64_t gblock = qblock + (int64_t)(a.heads + 2 * a.kv_heads) * a.tiles;
   const int warp = threadIdx.x >> 5;
   constexpr int64_t BB = block_bytes<DP>();
-  if (warp == 0) {
-    if ((threadIdx.x & 31) == 0) {
-      Ring ring{base + L::kRing, bars, bars + 8 * RING, RING};
+  if (warp < 4) {
+    W::few();
+    if (warp == 0 && (threadIdx.x & 31) == 0) {
+      Ring<DP, RING> ring{base + L::kRing, bars};
       Waiter wait(11);
       mbar_expect_tx(resident, 2 * BB);
       bulk_load(base, sp.blocks + qblock * BB, BB, resident);
       bulk_load(base + BB, sp.blocks + gblock * BB, BB, resident);
-      feed<DP>(ring, wait, sp.blocks + kplane * BB, false);
-      feed<DP>(ring, wait, sp.blocks + vplane * BB, false);
+      feed(ring, wait, sp.blocks + kplane * BB);
+      feed(ring, wait, sp.blocks + vplane * BB);
       for (int j = 0; j < n; ++j) {
         if (j + 1 < n) {
-          feed<DP>(ring, wait, sp.blocks + (kplane + j + 1) * BB, false);
-          feed<DP>(ring, wait, sp.blocks + (vplane + j + 1) * BB, false);
+          feed(ring, wait, sp.blocks + (kplane + j + 1) * BB);
+          feed(ring, wait, sp.blocks + (vplane + j + 1) * BB);
         }
-        feed<DP>(ring, wait, sp.blocks + (kplane + j) * BB, true);
+        feed(ring, wait, sp.blocks + (kplane + j) * BB);
       }
       feed_done(ring);
       Waiter last(32);
       last(resident, 0);
-    }
-  } else if (warp == 1) {
-    if ((threadIdx.x & 31) == 0) {
-      Ring ring{base + L::kRing, bars, bars + 8 * RING, RING};
-      Waiter wait(12);
-      wait(resident, 0);
-      mma_columns<DP>(tmem, base, ring, wait);
-      mma_columns<DP>(tmem + 256, base + BB, ring, wait);
-      mma_commit(spfull);
-      for (int j = 0; j < n && wait.ok; ++j) {
-        if (j + 1 < n) mma_columns<DP>(tmem + ((j + 1) & 1) * 128, base, ring, wait);
-        wait(dsfull, j & 1);
-        tc_fence_after();
-        if (j + 1 < n && wait.ok) {
-          mma_columns<DP>(tmem + 256, base + BB, ring, wait);
-          mma_commit(spfull);
-        }
-        wait(oempty, (j & 1) ^ 1);
-        tc_fence_after();
-        if (wait.ok) mma_rows<DP>(tmem + 384, tmem + (j & 1) * 128, ring, wait);
-        mma_commit(ofull);
+    } else if (warp == 1) {
+    Issuer<DP, RING> mma(base + L::kRing, bars, 12);
+    const auto nothing = [] {};
+    mma.wait_for(resident, 0);
+    mma.columns(tmem, base, nothing);
+    mma.columns(tmem + 256, base + BB, nothing);
+    commit(spfull);
+    for (int j = 0; j < n && mma.wait.ok; ++j) {
+      bool ds = false, drained = false;
+      if (j + 1 < n) mma.columns(tmem + ((j + 1) & 1) * 128, base, [&] { ds = mma.test(dsfull, j & 1); });
+      if (!ds) mma.wait_for(dsfull, j & 1);
+      else tc_fence_after();
+      if (j + 1 < n && mma.wait.ok) {
+        mma.columns(tmem + 256, base + BB, [&] { drained = mma.test(oempty, (j & 1) ^ 1); });
+        commit(spfull);
       }
-      Waiter last(33);
-      mma_commit(done);
-      last(done, 0);
+      if (!drained) mma.wait_for(oempty, (j & 1) ^ 1);
+      else tc_fence_after();
+      if (mma.wait.ok) mma.rows(tmem + 384, tmem + (j & 1) * 128, nothing);
+      commit(ofull);
+    }
+    Waiter last(33);
+    commit(done);
+    last(done, 0);
     }
   } else {
-    const Who me(2);
+    W::many();
+    constexpr int C = DP / PARTS;
+    const Who<PARTS> me(4);
     Waiter wait(13);
-    float acc[DP / 2], of = 0.f;
+    float acc[C], of = 0.f;
 #pragma unroll
-    for (int i = 0; i < DP / 2; ++i) acc[i] = 0.f;
+    for (int i = 0; i < C; ++i) acc[i] = 0.f;
     const int row = tile.z * kTileRows + me.row;
     const int64_t at = (int64_t)head * a.tokens + tile.x + row;
     const float lse = row < tile.y ? a.lse[at] * kLog2e : INFINITY;  // rows behind the sequence: no weight
@@ -727,7 +807,9 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const AttentionArgs a, 
     const float gnorm = sp.norm[gblock], dmax = sp.dmax[gblock];
     int ek = sp.expo[kplane], ev = sp.expo[vplane];
     float vnorm = sp.norm[vplane];
-    const uint32_t own = tmem + me.lanes + me.half * 64, oown = tmem + 384 + me.lanes + me.half * (DP / 2);
+    const int low = a.low_of(tile, me.row), col0 = me.part * COLS - low;
+    const unsigned span = me.row - low + 1;
+    const uint32_t own = tmem + me.lanes + me.part * COLS, oown = tmem + 384 + me.lanes + me.part * C;
     for (int j = 0; j < n; ++j) {
       const float c = ldexpf(a.scale * kLog2e, -(eq + ek));
       const DsScale ds = ds_scale(gnorm, vnorm, dmax, eg, ev, 0.f);
@@ -735,10 +817,9 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const AttentionArgs a, 
       if (j + 1 < n) ek = sp.expo[kplane + j + 1], ev = sp.expo[vplane + j + 1], vnorm = sp.norm[vplane + j + 1];
       const uint32_t s = own + (j & 1) * 128, dp = own + 256;
       const bool diag = j + 1 == n;
-      const int see = me.row - me.half * 64 + 1;
       warp_wait(wait, spfull, j & 1);
 #pragma unroll
-      for (int k = 0; k < 64; k += 16) {
+      for (int k = 0; k < COLS; k += 16) {
         uint32_t r[16], u[16], w[16];
         tmem_ld16_issue(s + k, r);
         tmem_ld16_issue(dp + k, u);
@@ -750,131 +831,141 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const AttentionArgs a, 
           float d0 = exp2_fast(fmaf(__uint_as_float(r[i]), c, -lse)) * fmaf(__uint_as_float(u[i]), ds.dp, -dd);
           float d1 = exp2_fast(fmaf(__uint_as_float(r[i + 1]), c, -lse)) * fmaf(__uint_as_float(u[i + 1]), ds.dp, -dd);
           if (diag) {
-            if (k + i >= see) d0 = 0.f;
-            if (k + i + 1 >= see) d1 = 0.f;
+            if (unsigned(col0 + k + i) >= span) d0 = 0.f;
+            if (unsigned(col0 + k + i + 1) >= span) d1 = 0.f;
           }
           split2(d0, d1, w[i / 2], w[8 + i / 2]);
         }
         tmem_st16(s + k, w);
       }
       tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(dsfull);
+      warp_arrive(dsfull);
       if (j > 0) {
         warp_wait(wait, ofull, (j - 1) & 1);
-        drain<DP>(oown, acc, 1.f, of);
-        tc_fence_before();
-        mbar_arrive(oempty);
+        drain<C>(oown, acc, 1.f, of);
+        warp_arrive(oempty);
       }
       of = f;
     }
     warp_wait(wait, ofull, (n - 1) & 1);
-    drain<DP>(oown, acc, 1.f, of);
+    drain<C>(oown, acc, 1.f, of);
     if (row < tile.y && wait.ok)
-      store_row<DP>(a.dq + ((int64_t)(tile.x + row) * a.heads + head) * a.dim, acc, me.half, a.dim, 1.f, vec_out);
+      store_row<C>(a.dq + ((int64_t)(tile.x + row) * a.heads + head) * a.dim, acc, me.part * C, a.dim, 1.f, vec_out);
   }
   teardown(tmem);
 }
 
 // dk and dv of one key tile and key/value head, over the group's query heads
-// and their tiles from the diagonal on.  Rows are keys, columns queries.
+// and their tiles from the diagonal on: one list of blocks, of which split s of
+// a.splits takes its share (a share may be empty).  With more than one split
+// the shares go to a.part, one after the other [splits, 2, tokens, kv_heads,
+// dim], which join_kernel adds in their order.  Rows are keys, columns queries.
 // TMEM: scores in columns [0, 128), overwritten by the weights; dP in
 // [128, 256), overwritten by dS; the block's shares of dv and dk in
 // [256, 256 + DP) and [384, 384 + DP).  The MMAs of a block run scores, dP,
 // dv, dk: weights are computed under dP, dS under dv.
 //
-// Both running sums are held in registers, 2 x DP / 2 a thread.  12 warps of
-// 168 registers are launched; the first four keep 88 so that the
-// computing eight can have 208 (128 x 88 + 256 x 208 = 384 x 168).
-constexpr int kThreadsKV = 384;
-
+// Both running sums are held in registers, 2 x DP / 2 a thread.
 template <int DP>
-__global__ void __launch_bounds__(kThreadsKV, 1) dkv_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
+__global__ void __launch_bounds__(Warps8::kThreads, 1) dkv_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
   extern __shared__ __align__(1024) unsigned char smem[];
   using L = BackwardLayout<DP>;
+  using W = Warps8;
+  constexpr int WARPS = W::kWarps, PARTS = W::kParts, COLS = W::kCols;
   constexpr int RING = backward_ring<DP>();
   const uint32_t base = smem_u32(smem), bars = base + L::kBarsAt;
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + L::kBarsAt + kBars * 8);
   float* stat = reinterpret_cast<float*>(smem + L::kScratch);  // [2][2][128]: weight offset, scaled delta
   // k and v, scores, dP, weights, dS, dv, dv drained, dk, dk drained, end
-  const int counts[10] = {1, 1, 1, 256, 256, 1, 256, 1, 256, 1};
+  const int counts[10] = {1, 1, 1, WARPS, WARPS, 1, WARPS, 1, WARPS, 1};
   if (!setup(smem, bars, slot, RING, counts, 10)) return;
   const uint32_t resident = bars + 16 * RING, sfull = resident + 8, dpfull = resident + 16, pfull = resident + 24,
                  dsfull = resident + 32, vfull = resident + 40, vempty = resident + 48, kfull = resident + 56,
                  kempty = resident + 64, done = resident + 72;
-  const uint32_t tmem = *slot;
-  const int order = blockIdx.x / a.kv_heads, kv_head = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
+  constexpr uint32_t tmem = 0;  // all of it was allocated
+  const int per_order = a.kv_heads * a.splits, order = blockIdx.x / per_order, kv_head = blockIdx.x % per_order / a.splits;
+  const int split = blockIdx.x % a.splits, group = a.heads / a.kv_heads;
   const int t = a.by_keys[order];
   const int4 tile = a.tile[t];
-  const int per_head = (tile.y + kTileRows - 1) / kTileRows - tile.z, n = per_head * group;  // query blocks
+  const int per_head = (tile.y + kTileRows - 1) / kTileRows - tile.z;  // query blocks of a head
+  const int first = (int)((int64_t)per_head * group * split / a.splits);
+  const int n = (int)((int64_t)per_head * group * (split + 1) / a.splits) - first;
   const int64_t kblock = (int64_t)(a.heads + kv_head) * a.tiles + t;
   const int64_t vblock = kblock + (int64_t)a.kv_heads * a.tiles;
   const int64_t gplanes = (int64_t)(a.heads + 2 * a.kv_heads) * a.tiles;
-  // block i: query head and tile, as a block index of the q planes
-  auto qblock = [&](int i) { return (int64_t)(kv_head * group + i / per_head) * a.tiles + t + i % per_head; };
+  // block i of this share: query head and tile, as a block index of the q planes
+  auto qblock = [&](int i) {
+    return (int64_t)(kv_head * group + (first + i) / per_head) * a.tiles + t + (first + i) % per_head;
+  };
   const int warp = threadIdx.x >> 5;
   constexpr int64_t BB = block_bytes<DP>();
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    W::few();
     if (warp == 0 && (threadIdx.x & 31) == 0) {
-      Ring ring{base + L::kRing, bars, bars + 8 * RING, RING};
+      Ring<DP, RING> ring{base + L::kRing, bars};
       Waiter wait(21);
       mbar_expect_tx(resident, 2 * BB);
       bulk_load(base, sp.blocks + kblock * BB, BB, resident);
       bulk_load(base + BB, sp.blocks + vblock * BB, BB, resident);
       for (int i = 0; i < n; ++i) {
         const unsigned char *q = sp.blocks + qblock(i) * BB, *g = q + gplanes * BB;
-        feed<DP>(ring, wait, q, false);
-        feed<DP>(ring, wait, g, false);
-        feed<DP>(ring, wait, g, true);
-        feed<DP>(ring, wait, q, true);
+        feed(ring, wait, q);
+        feed(ring, wait, g);
+        feed(ring, wait, g);
+        feed(ring, wait, q);
       }
       feed_done(ring);
       Waiter last(32);
       last(resident, 0);
-    } else if (warp == 1 && (threadIdx.x & 31) == 0) {
-      Ring ring{base + L::kRing, bars, bars + 8 * RING, RING};
-      Waiter wait(22);
-      wait(resident, 0);
-      for (int i = 0; i < n && wait.ok; ++i) {
-        mma_columns<DP>(tmem, base, ring, wait);
-        mma_commit(sfull);
-        mma_columns<DP>(tmem + 128, base + BB, ring, wait);
-        mma_commit(dpfull);
-        wait(pfull, i & 1);
-        wait(vempty, (i & 1) ^ 1);
+    } else if (warp == 1) {
+      Issuer<DP, RING> mma(base + L::kRing, bars, 22);
+      const auto nothing = [] {};
+      mma.wait_for(resident, 0);
+      for (int i = 0; i < n && mma.wait.ok; ++i) {
+        bool p = false, v = false, ds = false, k = false;
+        mma.columns(tmem, base, nothing);
+        commit(sfull);
+        mma.columns(tmem + 128, base + BB, [&] { p = mma.test(pfull, i & 1), v = mma.test(vempty, (i & 1) ^ 1); });
+        commit(dpfull);
+        if (!p) mma.wait_for(pfull, i & 1);
+        if (!v) mma.wait_for(vempty, (i & 1) ^ 1);
         tc_fence_after();
-        if (wait.ok) mma_rows<DP>(tmem + 256, tmem, ring, wait);
-        mma_commit(vfull);
-        wait(dsfull, i & 1);
-        wait(kempty, (i & 1) ^ 1);
+        if (mma.wait.ok) mma.rows(tmem + 256, tmem, [&] { ds = mma.test(dsfull, i & 1), k = mma.test(kempty, (i & 1) ^ 1); });
+        commit(vfull);
+        if (!ds) mma.wait_for(dsfull, i & 1);
+        if (!k) mma.wait_for(kempty, (i & 1) ^ 1);
         tc_fence_after();
-        if (wait.ok) mma_rows<DP>(tmem + 384, tmem + 128, ring, wait);
-        mma_commit(kfull);
+        if (mma.wait.ok) mma.rows(tmem + 384, tmem + 128, nothing);
+        commit(kfull);
       }
       Waiter last(33);
-      mma_commit(done);
+      commit(done);
       last(done, 0);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const Who me(4);
+    W::many();
+    constexpr int C = DP / PARTS;
+    const Who<PARTS> me(4);
     Waiter wait(23);
-    float dk[DP / 2], dv[DP / 2], fk = 0.f;
+    float dk[C], dv[C], fk = 0.f;
 #pragma unroll
-    for (int i = 0; i < DP / 2; ++i) dk[i] = dv[i] = 0.f;
+    for (int i = 0; i < C; ++i) dk[i] = dv[i] = 0.f;
     const int ek = sp.expo[kblock], ev = sp.expo[vblock];
     const float vnorm = sp.norm[vblock];
-    const uint32_t own = tmem + me.lanes + me.half * 64, oown = tmem + 256 + me.lanes + me.half * (DP / 2);
+    // in the diagonal block a key is seen by queries row..high - 1, high its
+    // sequence's end: by this thread's column i if unsigned(col0 + i) < span
+    const int col0 = me.part * COLS - me.row;
+    const unsigned span = a.high_of(tile, me.row) - me.row;
+    const uint32_t own = tmem + me.lanes + me.part * COLS, oown = tmem + 256 + me.lanes + me.part * C;
     // one value of the next block's row statistics a thread: lse (first half) or delta
     const int tid = threadIdx.x - 128;
     const float* source = tid < 128 ? a.lse : a.delta;
     auto fetch = [&](int i) {
-      const int r = (tile.z + i % per_head) * kTileRows + (tid & 127);
-      const int64_t at = (int64_t)(kv_head * group + i / per_head) * a.tokens + tile.x + r;
+      const int r = (tile.z + (first + i) % per_head) * kTileRows + (tid & 127);
+      const int64_t at = (int64_t)(kv_head * group + (first + i) / per_head) * a.tokens + tile.x + r;
       return r < tile.y ? __ldg(source + at) : tid < 128 ? INFINITY : 0.f;
     };
-    float next = fetch(0);
+    float next = n ? fetch(0) : 0.f;
     for (int i = 0; i < n; ++i) {
       const int64_t qb = qblock(i), gb = qb + gplanes;
       const int eq = sp.expo[qb], eg = sp.expo[gb];
@@ -882,15 +973,14 @@ __global__ void __launch_bounds__(kThreadsKV, 1) dkv_kernel(const AttentionArgs 
       const DsScale ds = ds_scale(sp.norm[gb], vnorm, sp.dmax[gb], eg, ev, kWeightBits);
       float* st = stat + (i & 1) * 256;
       st[tid] = tid < 128 ? kWeightBits - next * kLog2e : next * ds.d;
-      compute_sync();
+      compute_sync<WARPS>();
       if (i + 1 < n) next = fetch(i + 1);
-      const bool diag = i % per_head == 0;
-      const int from = me.row - me.half * 64;  // on the diagonal, queries from this column on see the key
-      const float4* bias = reinterpret_cast<const float4*>(st + me.half * 64);
-      const float4* dd = reinterpret_cast<const float4*>(st + 128 + me.half * 64);
+      const bool diag = (first + i) % per_head == 0;
+      const float4* bias = reinterpret_cast<const float4*>(st + me.part * COLS);
+      const float4* dd = reinterpret_cast<const float4*>(st + 128 + me.part * COLS);
       warp_wait(wait, sfull, i & 1);
 #pragma unroll
-      for (int k = 0; k < 64; k += 16) {
+      for (int k = 0; k < COLS; k += 16) {
         uint32_t r[16], w[16];
         tmem_ld16_issue(own + k, r);
         tmem_ld_wait();
@@ -903,7 +993,7 @@ __global__ void __launch_bounds__(kThreadsKV, 1) dkv_kernel(const AttentionArgs 
           if (diag) {
 #pragma unroll
             for (int x = 0; x < 4; ++x)
-              if (k + j + x < from) p[x] = 0.f;
+              if (unsigned(col0 + k + j + x) >= span) p[x] = 0.f;
           }
           split2(p[0], p[1], w[j / 2], w[8 + j / 2]);
           split2(p[2], p[3], w[j / 2 + 1], w[8 + j / 2 + 1]);
@@ -911,17 +1001,15 @@ __global__ void __launch_bounds__(kThreadsKV, 1) dkv_kernel(const AttentionArgs 
         tmem_st16(own + k, w);
       }
       tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(pfull);
+      warp_arrive(pfull);
       if (i > 0) {
         warp_wait(wait, kfull, (i - 1) & 1);
-        drain<DP>(oown + 128, dk, 1.f, fk);
-        tc_fence_before();
-        mbar_arrive(kempty);
+        drain<C>(oown + 128, dk, 1.f, fk);
+        warp_arrive(kempty);
       }
       warp_wait(wait, dpfull, i & 1);
 #pragma unroll
-      for (int k = 0; k < 64; k += 16) {
+      for (int k = 0; k < COLS; k += 16) {
         uint32_t r[16], u[16], w[16];
         tmem_ld16_issue(own + k, r);
         tmem_ld16_issue(own + 128 + k, u);
@@ -946,24 +1034,37 @@ __global__ void __launch_bounds__(kThreadsKV, 1) dkv_kernel(const AttentionArgs 
         tmem_st16(own + 128 + k, w);
       }
       tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(dsfull);
+      warp_arrive(dsfull);
       warp_wait(wait, vfull, i & 1);
-      drain<DP>(oown, dv, 1.f, two_to(-(int)kWeightBits - eg));
-      tc_fence_before();
-      mbar_arrive(vempty);
+      drain<C>(oown, dv, 1.f, two_to(-(int)kWeightBits - eg));
+      warp_arrive(vempty);
       fk = ldexpf(a.scale, -(ds.e + eq));
     }
-    warp_wait(wait, kfull, (n - 1) & 1);
-    drain<DP>(oown + 128, dk, 1.f, fk);
+    if (n) {
+      warp_wait(wait, kfull, (n - 1) & 1);
+      drain<C>(oown + 128, dk, 1.f, fk);
+    }
     const int row = tile.z * kTileRows + me.row;
     if (row < tile.y && wait.ok) {
       const int64_t at = ((int64_t)(tile.x + row) * a.kv_heads + kv_head) * a.dim;
-      store_row<DP>(a.dk + at, dk, me.half, a.dim, 1.f, vec_out);
-      store_row<DP>(a.dv + at, dv, me.half, a.dim, 1.f, vec_out);
+      const int64_t values = a.tokens * a.kv_heads * a.dim;
+      store_row<C>((a.part ? a.part + 2 * split * values : a.dk) + at, dk, me.part * C, a.dim, 1.f, vec_out);
+      store_row<C>((a.part ? a.part + (2 * split + 1) * values : a.dv) + at, dv, me.part * C, a.dim, 1.f, vec_out);
     }
   }
   teardown(tmem);
+}
+
+// dk and dv from the splits' shares, in their order: `used` values each (the
+// tokens of the sequences) of `values`.
+__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part, float* __restrict__ dk,
+                                                   float* __restrict__ dv, int64_t used, int64_t values, int splits) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= used) return;
+  const float* p = part + blockIdx.y * values + i;
+  float s = p[0];
+  for (int k = 1; k < splits; ++k) s += p[2 * k * values];
+  (blockIdx.y ? dv : dk)[i] = s;
 }
 
 // ------------------------------------------------------------ host side
@@ -977,12 +1078,13 @@ lmpb_status allow_smem(K kernel, int bytes) {
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // One allocation for the split blocks and what goes with them.
-lmpb_status make_split(const AttentionArgs& a, bool backward, int dp, Split& s, float** delta, void** ws, cudaStream_t st) {
+lmpb_status make_split(AttentionArgs& a, bool backward, int dp, Split& s, float** delta, void** ws, cudaStream_t st) {
   auto up = [](size_t b) { return (b + 255) / 256 * 256; };
   const size_t planes = (size_t)(backward ? 2 : 1) * a.heads + 2 * a.kv_heads, n = planes * a.tiles;
   const size_t blocks = n * (dp == 64 ? block_bytes<64>() : block_bytes<128>());
   const size_t dbytes = backward ? up((size_t)a.tokens * a.heads * 4) : 0;
-  LMPB_CUDA_TRY(stream_alloc(ws, blocks + 3 * up(4 * n) + up(n) + dbytes, st));
+  const size_t pbytes = a.splits > 1 ? (size_t)a.splits * 2 * a.tokens * a.kv_heads * a.dim * 4 : 0;
+  LMPB_CUDA_TRY(stream_alloc(ws, blocks + 3 * up(4 * n) + up(n) + dbytes + pbytes, st));
   unsigned char* p = static_cast<unsigned char*>(*ws);
   s.blocks = p;
   s.expo = reinterpret_cast<int*>(p + blocks);
@@ -990,6 +1092,7 @@ lmpb_status make_split(const AttentionArgs& a, bool backward, int dp, Split& s, 
   s.dmax = reinterpret_cast<float*>(p + blocks + 2 * up(4 * n));
   s.flags = p + blocks + 3 * up(4 * n);
   *delta = reinterpret_cast<float*>(s.flags + up(n));
+  if (pbytes) a.part = reinterpret_cast<float*>(s.flags + up(n) + dbytes);
   return LMPB_OK;
 }
 
@@ -1008,7 +1111,7 @@ lmpb_status forward(const AttentionArgs& a, const Split& s, cudaStream_t st) {
   if (r == LMPB_OK) r = allow_smem(forward_kernel<DP>, ForwardLayout<DP>::kBytes);
   if (r != LMPB_OK) return r;
   const bool vec = a.dim % 4 == 0 && aligned16(a.out);
-  forward_kernel<DP><<<(unsigned)(a.tiles * a.heads), kThreads, ForwardLayout<DP>::kBytes, st>>>(a, s, vec);
+  forward_kernel<DP><<<(unsigned)(a.tiles * a.heads), ForwardWarps<DP>::kThreads, ForwardLayout<DP>::kBytes, st>>>(a, s, vec);
   return launch_status("attention");
 }
 
@@ -1019,15 +1122,20 @@ lmpb_status backward(const AttentionArgs& a, const Split& s, float* delta, cudaS
   if (r == LMPB_OK && a.dk) {
     r = allow_smem(dkv_kernel<DP>, bytes);
     if (r != LMPB_OK) return r;
-    const bool vec = a.dim % 4 == 0 && aligned16(a.dk) && aligned16(a.dv);
-    dkv_kernel<DP><<<(unsigned)(a.tiles * a.kv_heads), kThreadsKV, bytes, st>>>(a, s, vec);
+    const bool vec = a.dim % 4 == 0 && (a.part ? aligned16(a.part) : aligned16(a.dk) && aligned16(a.dv));
+    dkv_kernel<DP><<<(unsigned)(a.tiles * a.kv_heads * a.splits), Warps8::kThreads, bytes, st>>>(a, s, vec);
     r = launch_status("attention_backward (dk, dv)");
+    if (r == LMPB_OK && a.part) {
+      const int64_t row = (int64_t)a.kv_heads * a.dim, used = a.used * row;
+      join_kernel<<<dim3((unsigned)((used + 255) / 256), 2), 256, 0, st>>>(a.part, a.dk, a.dv, used, a.tokens * row, a.splits);
+      r = launch_status("attention_backward (join)");
+    }
   }
   if (r == LMPB_OK && a.dq) {
     r = allow_smem(dq_kernel<DP>, bytes);
     if (r != LMPB_OK) return r;
     const bool vec = a.dim % 4 == 0 && aligned16(a.dq);
-    dq_kernel<DP><<<(unsigned)(a.tiles * a.heads), kThreads, bytes, st>>>(a, s, vec);
+    dq_kernel<DP><<<(unsigned)(a.tiles * a.heads), Warps8::kThreads, bytes, st>>>(a, s, vec);
     r = launch_status("attention_backward (dq)");
   }
   return r;
@@ -1036,10 +1144,21 @@ lmpb_status backward(const AttentionArgs& a, const Split& s, float* delta, cudaS
 }  // namespace
 
 bool attention_fits_sm100(const AttentionArgs& a) {
-  return (int64_t)a.tiles * a.heads <= 0x7fffffff && 2 * a.heads + 2 * a.kv_heads <= 65535;
+  return (int64_t)a.tiles * a.heads * kMaxSplits <= 0x7fffffff && 2 * a.heads + 2 * a.kv_heads <= 65535;
 }
 
-lmpb_status attention_sm100(const AttentionArgs& args, cudaStream_t st) {
+// Into how many shares the dk, dv work of a key tile is cut: until the
+// largest share is at most half of what an SM gets on average, so that the
+// last CTAs do not run alone (one key/value head, or a long sequence), but
+// not below 6 blocks, where starting a CTA costs as much as its work.
+int dkv_splits(const AttentionArgs& a) {
+  const int64_t group = a.heads / a.kv_heads;
+  const double average = (double)a.pair_tiles * a.heads / sm_count();
+  const int64_t share = std::max<int64_t>(6, (int64_t)(average / 2));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, (a.longest_tiles * group + share - 1) / share));
+}
+
+lmpb_status attention_sm100(const AttentionArgs& args, const lmpb_sequences_s* seqs, cudaStream_t st) {
   AttentionArgs a = args;
   Split s{};
   float* unused = nullptr;
@@ -1049,6 +1168,7 @@ lmpb_status attention_sm100(const AttentionArgs& args, cudaStream_t st) {
   if (r != LMPB_OK) return r;
   r = dp == 64 ? forward<64>(a, s, st) : forward<128>(a, s, st);
   a.flags = s.flags;
+  use_tiles(a, seqs, seqs->plain);  // the fp32 kernels for what was flagged
   if (r == LMPB_OK) r = attention_simt(a, st);
   const cudaError_t e = cudaFreeAsync(ws, st);
   if (r == LMPB_OK && e != cudaSuccess)
@@ -1056,17 +1176,19 @@ lmpb_status attention_sm100(const AttentionArgs& args, cudaStream_t st) {
   return r;
 }
 
-lmpb_status attention_sm100_backward(const AttentionArgs& args, cudaStream_t st) {
+lmpb_status attention_sm100_backward(const AttentionArgs& args, const lmpb_sequences_s* seqs, cudaStream_t st) {
   AttentionArgs a = args;
   Split s{};
   float* delta = nullptr;
   void* ws = nullptr;
   const int dp = a.dim <= 64 ? 64 : 128;
+  a.splits = a.dk ? dkv_splits(a) : 1;
   lmpb_status r = make_split(a, true, dp, s, &delta, &ws, st);
   if (r != LMPB_OK) return r;
   a.delta = delta;
   r = dp == 64 ? backward<64>(a, s, delta, st) : backward<128>(a, s, delta, st);
   a.flags = s.flags;
+  use_tiles(a, seqs, seqs->plain);  // the fp32 kernels for what was flagged
   if (r == LMPB_OK) r = attention_simt_backward(a, st);
   const cudaError_t e = cudaFreeAsync(ws, st);
   if (r == LMPB_OK && e != cudaSuccess)

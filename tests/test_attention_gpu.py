@@ -12,6 +12,11 @@ Tolerances, per element, from what is added (magnitudes M below):
   value is rounded to fp32): within 2 E + 2^-23 |lse| + 2^-21 of itself.
 * what sums weights times values has the same 3 * 2^-22 a product, and at most
   2^-23 a product and block of additions that follow one another: L 2^-23.
+* the fp16 parts have a smallest step of 2^-24, so of an operand scaled to have
+  its largest value (of a 128-row tile), a weight 1, or dS its bound
+  B = max|g| max|v| + max|delta| at 2^14 or more, the two parts are within
+  max(2^-22 |x|, 2^-25) of x in that scale: an absolute 2^-39 of that largest
+  value.  Where all of a sum's terms are tiny against it, this is what is left.
 Each bound is the sum of these times the magnitudes added, in 64 bits."""
 from __future__ import annotations
 
@@ -27,7 +32,12 @@ CASES = [  # lengths, heads, kv_heads, head_dim, rows behind the last sequence
     ([128, 127, 129, 1], 4, 1, 128, 5), ([300, 17, 513], 6, 2, 80, 0), ([0, 0], 2, 2, 16, 3), ([], 2, 1, 4, 4),
     ([1030], 3, 3, 96, 1), ([255, 256, 257], 8, 1, 16, 0), ([2049], 4, 2, 128, 0), ([1500, 31, 700, 1], 4, 2, 64, 0),
     ([1] * 40, 3, 1, 31, 0), ([640] * 3, 2, 2, 65, 130),
+    ([5, 60, 30, 40, 1, 0, 128, 3, 127, 1, 64, 64, 2, 70], 4, 2, 64, 0),  # several sequences in a 128-row tile
+    ([90, 20, 18, 90, 38, 0, 0, 1, 300, 5], 6, 1, 128, 9),
 ]
+
+
+FLOOR = 2.0 ** -39
 
 
 def _inputs(torch, rng, case, scale=1.0):
@@ -64,24 +74,33 @@ def _reference(torch, x, lengths, scale=None):
             S = (scale * Q @ K.T).masked_fill(~mask, -math.inf)
             lse = torch.logsumexp(S, 1, keepdim=True)
             P = torch.exp(S - lse)
-            E = ((3 + d / 2) * w * scale * (Q.abs() @ K.abs().T)).masked_fill(~mask, 0)
+            top = {a: float(b.abs().max()) for a, b in (("q", Q), ("k", K), ("v", V), ("g", G))}
+            q1, k1, v1, g1 = (a.abs().sum(1) for a in (Q, K, V, G))
+            E = (3 + d / 2) * w * scale * (Q.abs() @ K.abs().T) + scale * FLOOR * (top["k"] * q1[:, None] + top["q"] * k1)
+            E = E.masked_fill(~mask, 0)
             rel = 2 * E.amax(1, keepdim=True) + w * (lse.abs() / 2 + 2)  # of a weight
             sums = (3 + n / 2) * w
             O = P @ V
-            out["out"][0][rows, h], out["out"][1][rows, h] = O, (rel + sums) * (P @ V.abs())
+            seen = mask.double()
+            out["out"][0][rows, h] = O
+            out["out"][1][rows, h] = (rel + sums) * (P @ V.abs()) + FLOOR * (seen @ V.abs() + top["v"])
             dP = G @ V.T
             delta = (G * O).sum(1, keepdim=True)
             dS = P * (dP - delta)
             # dP and delta: D products each, delta with the output's own error
             size = (G.abs() @ V.abs().T) + (G.abs() * (P @ V.abs())).sum(1, keepdim=True)
             dSt = (rel + (3 + d / 2) * w + sums) * P * size + rel * dS.abs()
+            dSt = dSt + P * FLOOR * (top["v"] * g1[:, None] + top["g"] * v1 + (G.abs() @ V.abs().sum(0)[:, None] + top["v"] * g1[:, None]))
+            bound = float(G.norm(dim=1).max() * V.norm(dim=1).max() + delta.abs().max())
+            dSt = dSt + FLOOR * bound * seen
             dSm = P * size
             out["dq"][0][rows, h] = scale * dS @ K
-            out["dq"][1][rows, h] = scale * (dSt @ K.abs() + sums * (dSm @ K.abs()))
+            out["dq"][1][rows, h] = scale * (dSt @ K.abs() + sums * (dSm @ K.abs()) + FLOOR * top["k"] * dSm.sum(1, keepdim=True))
             out["dk"][0][rows, j] += scale * dS.T @ Q
-            out["dk"][1][rows, j] += scale * (dSt.T @ Q.abs() + sums * (dSm.T @ Q.abs()))
+            out["dk"][1][rows, j] += scale * (dSt.T @ Q.abs() + sums * (dSm.T @ Q.abs()) + FLOOR * top["q"] * dSm.sum(0)[:, None])
             out["dv"][0][rows, j] += P.T @ G
             out["dv"][1][rows, j] += (rel * P).T @ G.abs() + sums * (P.T @ G.abs())
+            out["dv"][1][rows, j] += FLOOR * (seen.T @ G.abs() + top["g"] * P.sum(0)[:, None])
     return {n: (a.cpu().numpy(), b.cpu().numpy()) for n, (a, b) in out.items()}
 
 
