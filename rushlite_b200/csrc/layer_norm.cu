@@ -11,8 +11,8 @@
 // x + y and the backward x + g + dx and nothing twice.  The centred second
 // pass costs no traffic and has no cancellation for a large mean.
 //
-// A row of up to 1024 values (512 in float64) belongs to one warp (8 rows a
-// CTA, no barrier); a row of up to 8192 to a CTA of 256 or 1024 threads.
+// A row of up to 512 values, or 1024 in float32, belongs to one warp (8 rows a
+// CTA, no barrier); a row of up to 8192 to a CTA of 256 to 1024 threads.
 // Longer rows are walked in memory (the *_long kernels).  The backward's CTAs stay resident and walk
 // rows with a stride; each thread keeps its columns' share of dw and db in
 // registers, writes it once at its end as one row of a partial table, and a
@@ -142,25 +142,39 @@ __global__ void __launch_bounds__(block_of(TPR))
   }
 }
 
-// part: [gridDim.x, 2, F] of dw and db; null when neither is wanted.
+// CTAs an SM must hold of a tile of E values a thread: two where the four
+// tiles of a row (x and g, and the next row's) and the two running sums leave
+// room for it in registers.
+template <typename T, int E, int TPR>
+constexpr int resident() { return TPR <= 256 && E * sizeof(T) <= 64 ? 2 : 1; }
+
+// part: [gridDim.x, 2, F] of dw and db, or with one CTA the results
+// themselves; null when neither is wanted.  The next row's x and g are loaded
+// before this row's sums are awaited (without that, 82 us instead of 62 for
+// [8192, 4096]; the same rows fetched by bulk copies into a ring in shared
+// memory: 104, since fewer threads are then there to add).
 template <typename T, int VEC, int NV, int TPR>
-__global__ void __launch_bounds__(block_of(TPR))
+__global__ void __launch_bounds__(block_of(TPR), resident<T, NV * VEC, TPR>())
     backward_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ mean,
                     const T* __restrict__ rstd, const T* __restrict__ g, T* __restrict__ dx, T* __restrict__ part,
-                    int64_t rows, int F, T inv_f) {
+                    T* __restrict__ dw_out, T* __restrict__ db_out, int64_t rows, int F, T inv_f) {
   constexpr int RPC = block_of(TPR) / TPR, E = NV * VEC;
   __shared__ T red[4 * (TPR / 32)];
   extern __shared__ __align__(16) unsigned char fold_raw[];  // at most 8 rows of 4 KB
   const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   int phase = 0;
-  T dw[E], db[E];
+  T dw[E], db[E], h[E], a[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) dw[i] = db[i] = T(0);
-  for (int64_t row = (int64_t)blockIdx.x * RPC + sub; row < rows; row += (int64_t)gridDim.x * RPC) {
-    T h[E], a[E];
+  const int64_t step = (int64_t)gridDim.x * RPC;
+  int64_t row = (int64_t)blockIdx.x * RPC + sub;
+  T mu = T(0), rs = T(0);
+  if (row < rows) {
     load_row<T, VEC, NV, TPR>(x + row * F, lane, F, h);
     load_row<T, VEC, NV, TPR>(g + row * F, lane, F, a);
-    const T mu = mean[row], rs = rstd[row];
+    mu = mean[row], rs = rstd[row];
+  }
+  for (; row < rows; row += step) {
     T s[2] = {T(0), T(0)};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -179,21 +193,32 @@ __global__ void __launch_bounds__(block_of(TPR))
         s[1] += a[k] * h[k];
       }
     }
-    if (!dx) continue;  // uniform
-    row_sum<T, TPR, 2>(s, red, phase);
-    const T m0 = s[0] * inv_f, m1 = s[1] * inv_f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * VEC;
-      if (c >= F) continue;
-      Packet<T, VEC> u;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) u.v[j] = rs * (a[i * VEC + j] - m0 - h[i * VEC + j] * m1);
-      *reinterpret_cast<Packet<T, VEC>*>(dx + row * F + c) = u;
+    T nh[E], na[E], nmu = T(0), nrs = T(0);
+    const int64_t next = row + step;
+    if (next < rows) {
+      load_row<T, VEC, NV, TPR>(x + next * F, lane, F, nh);
+      load_row<T, VEC, NV, TPR>(g + next * F, lane, F, na);
+      nmu = mean[next], nrs = rstd[next];
     }
+    if (dx) {  // uniform
+      row_sum<T, TPR, 2>(s, red, phase);
+      const T m0 = s[0] * inv_f, m1 = s[1] * inv_f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * TPR + lane) * VEC;
+        if (c >= F) continue;
+        Packet<T, VEC> u;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) u.v[j] = rs * (a[i * VEC + j] - m0 - h[i * VEC + j] * m1);
+        *reinterpret_cast<Packet<T, VEC>*>(dx + row * F + c) = u;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) h[i] = nh[i], a[i] = na[i];
+    mu = nmu, rs = nrs;
   }
-  if (!part) return;
-  T* prow = part + (int64_t)blockIdx.x * 2 * F;
+  T* const prow[2] = {part ? part + (int64_t)blockIdx.x * 2 * F : dw_out, part ? part + ((int64_t)blockIdx.x * 2 + 1) * F : db_out};
+  if (!prow[0] && !prow[1]) return;
   if constexpr (RPC == 1) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -201,14 +226,15 @@ __global__ void __launch_bounds__(block_of(TPR))
       if (c >= F) continue;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        prow[c + j] = dw[i * VEC + j];
-        prow[F + c + j] = db[i * VEC + j];
+        if (prow[0]) prow[0][c + j] = dw[i * VEC + j];
+        if (prow[1]) prow[1][c + j] = db[i * VEC + j];
       }
     }
   } else {  // the CTA's rows' owners, added in their order
     T* fold = reinterpret_cast<T*>(fold_raw);  // [RPC, F]
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
+      if (!prow[which]) continue;  // uniform
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = (i * TPR + lane) * VEC;
@@ -221,31 +247,32 @@ __global__ void __launch_bounds__(block_of(TPR))
         T t = fold[c];
 #pragma unroll
         for (int r = 1; r < RPC; ++r) t += fold[r * F + c];
-        prow[which * F + c] = t;
+        prow[which][c] = t;
       }
       __syncthreads();
     }
   }
 }
 
-// out[c] = sum over the table's rows of column c: 32 columns a CTA, 8 row
-// lanes folded in order.  Columns [0, F) go to dw, [F, 2F) to db.
+// out[c] = sum over the table's rows of column c: 32 columns a CTA, 32 row
+// lanes folded in order (8 lanes of four times the rows waited 13 us for
+// [296, 2 x 4096]).  Columns [0, F) go to dw, [F, 2F) to db.
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(1024)
     fold_kernel(const T* __restrict__ part, int rows, int F, T* __restrict__ dw, T* __restrict__ db) {
-  __shared__ T s[8][33];
+  __shared__ T s[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t col = (int64_t)blockIdx.x * 32 + tx, W = 2 * (int64_t)F;
   T t = T(0);
   if (col < W) {
-#pragma unroll 4
-    for (int r = ty; r < rows; r += 8) t += part[r * W + col];
+#pragma unroll 5
+    for (int r = ty; r < rows; r += 32) t += part[r * W + col];
   }
   s[ty][tx] = t;
   __syncthreads();
   if (ty == 0 && col < W) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) t += s[k][tx];
+    for (int k = 1; k < 32; ++k) t += s[k][tx];
     T* out = col < F ? dw : db;
     if (out) out[col < F ? col : col - F] = t;
   }
@@ -336,27 +363,44 @@ unsigned grid_of(int64_t rows, int rows_per_cta, int ctas_per_sm) {
   return (unsigned)std::max<int64_t>(1, std::min<int64_t>(need, (int64_t)sm_count() * ctas_per_sm));
 }
 
-// Calls f.run<VEC, NV, TPR>() for the smallest register tile that holds a
-// row of F values; false when none does.  A thread holds at most 128 bytes
-// of a row: the backward keeps four such tiles in registers.
-template <typename T, int VEC, typename F>
-bool with_tile(int64_t features, F&& f) {
-  constexpr int big = 128 / sizeof(T);  // 32 floats, 16 doubles
-  if (features <= 32 * 4) f.template run<VEC, 4 / VEC, 32>();
-  else if (features <= 32 * 8) f.template run<VEC, 8 / VEC, 32>();
-  else if (features <= 32 * 16) f.template run<VEC, 16 / VEC, 32>();
-  else if (features <= 32 * big) f.template run<VEC, big / VEC, 32>();
-  else if (features <= 256 * 4) f.template run<VEC, 4 / VEC, 256>();
-  else if (features <= 256 * 8) f.template run<VEC, 8 / VEC, 256>();
-  else if (features <= 256 * 16) f.template run<VEC, 16 / VEC, 256>();
-  else if (features <= 1024 * 8) f.template run<VEC, 8 / VEC, 1024>();
-  else return false;
-  return true;
+// Whether a warp walks a row.  Up to 512 values always; up to 1024 floats
+// where there are rows for 8 warps of 8 CTAs on every SM, otherwise a CTA a
+// row is there sooner (forward: [16384, 1024] 27 us by warps, 41 by CTAs;
+// [1023, 1001] 10.8 and 6.9).
+template <typename T>
+bool by_warps(int64_t rows, int64_t features) {
+  return features <= 512 || (sizeof(T) == 4 && features <= 1024 && rows > 8 * (int64_t)sm_count());
 }
 
-// Rows a CTA of that tile walks at once.
-template <typename T>
-int rows_per_cta(int64_t features) { return features <= 32 * (128 / (int)sizeof(T)) ? kThreads / 32 : 1; }
+// Calls f.run<VEC, NV, TPR>() for the tile that holds a row of F values;
+// false when none does.  `wide`: doubles spread over 512 threads, which
+// leaves the backward's sums in registers ([2048, 4096]: 50 us, 62 over 256;
+// the forward has less to hold: 33 and 29).
+template <typename T, int VEC, typename F>
+bool with_tile(int64_t rows, int64_t features, bool wide, F&& f) {
+  if (by_warps<T>(rows, features)) {
+    if (features <= 32 * 4) f.template run<VEC, 4 / VEC, 32>();
+    else if (features <= 32 * 8) f.template run<VEC, 8 / VEC, 32>();
+    else if (features <= 32 * 16) f.template run<VEC, 16 / VEC, 32>();
+    else if constexpr (sizeof(T) == 4) f.template run<VEC, 32 / VEC, 32>();
+  } else if (features <= 256 * 4) {
+    f.template run<VEC, 4 / VEC, 256>();
+  } else if (sizeof(T) == 8 && wide && features <= 512 * 8) {
+    if constexpr (sizeof(T) == 8) {
+      if (features <= 512 * 4) f.template run<VEC, 4 / VEC, 512>();
+      else f.template run<VEC, 8 / VEC, 512>();
+    }
+  } else if (features <= 256 * 8) {
+    f.template run<VEC, 8 / VEC, 256>();
+  } else if (features <= 256 * 16) {
+    f.template run<VEC, 16 / VEC, 256>();
+  } else if (features <= 1024 * 8) {
+    f.template run<VEC, 8 / VEC, 1024>();
+  } else {
+    return false;
+  }
+  return true;
+}
 
 template <typename T>
 struct Forward {
@@ -376,14 +420,14 @@ struct Forward {
 template <typename T>
 struct Backward {
   const T *x, *w, *mean, *rstd, *g;
-  T *dx, *part;
+  T *dx, *part, *dw, *db;
   int64_t rows, F;
   unsigned grid;
   cudaStream_t st;
   template <int VEC, int NV, int TPR>
   void run() const {
-    const size_t fold = TPR == 32 && part ? (size_t)(kThreads / 32) * F * sizeof(T) : 0;
-    backward_kernel<T, VEC, NV, TPR><<<grid, block_of(TPR), fold, st>>>(x, w, mean, rstd, g, dx, part, rows, (int)F,
+    const size_t fold = TPR == 32 && (dw || db) ? (size_t)(kThreads / 32) * F * sizeof(T) : 0;
+    backward_kernel<T, VEC, NV, TPR><<<grid, block_of(TPR), fold, st>>>(x, w, mean, rstd, g, dx, part, dw, db, rows, (int)F,
                                                                         T(1.0 / (double)F));
   }
 };
@@ -394,7 +438,7 @@ lmpb_status forward(const void* x, const void* w, const void* b, int64_t rows, i
   constexpr int V = 16 / sizeof(T);
   Forward<T> f{(const T*)x, (const T*)w, (const T*)b, (T*)y, (T*)mean, (T*)rstd, rows, F, eps, st};
   const bool vec = F % V == 0 && aligned16(x) && aligned16(y) && aligned16(w) && aligned16(b);
-  if (!(vec ? with_tile<T, V>(F, f) : with_tile<T, 1>(F, f)))
+  if (!(vec ? with_tile<T, V>(rows, F, false, f) : with_tile<T, 1>(rows, F, false, f)))
     forward_long_kernel<T><<<grid_of(rows, 1, 8), kThreads, 0, st>>>(f.x, f.w, f.b, f.y, f.mean, f.rstd, rows, F,
                                                                      T(1.0 / (double)F), T(eps));
   return launch_status("layer_norm");
@@ -405,17 +449,20 @@ lmpb_status backward(const void* x, const void* w, const void* mean, const void*
                      int64_t F, void* dx, void* dw, void* db, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const bool columns = dw || db, lng = F > 8192;
-  const unsigned grid = grid_of(rows, rows_per_cta<T>(F), 2);
+  const bool vec = F % V == 0 && aligned16(x) && aligned16(g) && aligned16(dx) && aligned16(w);
+  // a few rows: one CTA, whose sums over rows are the results (32 x 256: one launch instead of two)
+  const unsigned grid = !lng && rows * F <= 8192 ? 1 : grid_of(rows, by_warps<T>(rows, F) ? kThreads / 32 : 1, 2);
+  const bool table = columns && (lng || grid > 1);
   const int64_t chunk = std::max<int64_t>(32, (rows + 63) / 64);
   const int prows = lng ? (int)((rows + chunk - 1) / chunk) : (int)grid;
   T* part = nullptr;
-  if (columns) LMPB_CUDA_TRY(stream_alloc((void**)&part, (size_t)prows * 2 * F * sizeof(T), st));
+  if (table) LMPB_CUDA_TRY(stream_alloc((void**)&part, (size_t)prows * 2 * F * sizeof(T), st));
   lmpb_status s = LMPB_OK;
   if (!lng) {
-    Backward<T> f{(const T*)x, (const T*)w, (const T*)mean, (const T*)rstd, (const T*)g, (T*)dx, part, rows, F, grid, st};
-    const bool vec = F % V == 0 && aligned16(x) && aligned16(g) && aligned16(dx) && aligned16(w);
-    if (vec) with_tile<T, V>(F, f);
-    else with_tile<T, 1>(F, f);
+    Backward<T> f{(const T*)x, (const T*)w, (const T*)mean, (const T*)rstd, (const T*)g,
+                  (T*)dx,      part,        (T*)dw,         (T*)db,         rows, F, grid, st};
+    if (vec) with_tile<T, V>(rows, F, true, f);
+    else with_tile<T, 1>(rows, F, true, f);
     s = launch_status("layer_norm_backward");
   } else {
     if (dx) {
@@ -430,8 +477,8 @@ lmpb_status backward(const void* x, const void* w, const void* mean, const void*
       s = launch_status("layer_norm_backward (columns)");
     }
   }
-  if (s == LMPB_OK && columns) {
-    fold_kernel<T><<<(unsigned)((2 * F + 31) / 32), kThreads, 0, st>>>(part, prows, (int)F, (T*)dw, (T*)db);
+  if (s == LMPB_OK && table) {
+    fold_kernel<T><<<(unsigned)((2 * F + 31) / 32), 1024, 0, st>>>(part, prows, (int)F, (T*)dw, (T*)db);
     s = launch_status("layer_norm_backward (fold)");
   }
   if (part) {
@@ -451,6 +498,7 @@ lmpb_status check(const char* what, int dtype, int64_t rows, int64_t features) {
 }
 
 }  // namespace
+
 }  // namespace lmpb
 
 extern "C" lmpb_status lmpb_layer_norm(int dtype, const void* x, const void* weight, const void* bias, int64_t rows,
