@@ -27,9 +27,6 @@
 
 #include "attention.cuh"
 
-#ifndef TENSOR_MIN
-#define TENSOR_MIN 64
-#endif
 namespace lmpb {
 namespace {
 
@@ -435,10 +432,20 @@ lmpb_status check(const char* what, int64_t tokens, int heads, int kv_heads, int
   return LMPB_OK;
 }
 
-// Sequences of under 65 tokens leave half of every 128-row tile empty.
-bool on_tensor_cores(const AttentionArgs& a, const lmpb_sequences_s* seqs) {
-  static const bool off = getenv("LMPB_ATTENTION_SIMT") != nullptr;  // A/B switch
-  return !off && seqs->longest > TENSOR_MIN && attention_fits_sm100(a);
+// Which kernels: the short ones where one CTA a sequence and head is there
+// first, the tensor cores' otherwise.
+enum class Path { kShort, kTensor, kSimt };
+
+Path path_of(const AttentionArgs& a, const lmpb_sequences_s* seqs) {
+  static const char* force = getenv("LMPB_ATTENTION");  // A/B switch: simt, tensor or short
+  const bool fits = attention_fits_sm100(a), brief = seqs->longest <= kShortRows;
+  if (force && !strcmp(force, "simt")) return Path::kSimt;
+  if (force && !strcmp(force, "tensor") && fits) return Path::kTensor;
+  if (force && !strcmp(force, "short") && brief) return Path::kShort;
+  // About where they meet ([32] x 150, 8 heads of 64: 42 + 88 us short, 39 + 87 on tensor cores; [20] x 10:
+  // 8.4 + 11 and 21 + 37; [16] x 1000: 130 + 273 and 98 + 208).
+  if (brief && (double)seqs->plain.count * a.heads * seqs->longest * seqs->longest <= 8192.0 * sm_count()) return Path::kShort;
+  return fits ? Path::kTensor : Path::kSimt;
 }
 
 // Rows behind the last sequence belong to nobody: 0.
@@ -575,10 +582,12 @@ extern "C" lmpb_status lmpb_attention(const float* q, const float* k, const floa
   AttentionArgs a{};
   a.q = q, a.k = k, a.v = v, a.out = out, a.lse = lse;
   a.tokens = tokens, a.heads = heads, a.kv_heads = kv_heads, a.dim = head_dim, a.scale = scale;
-  a.used = seqs->tokens, a.pair_tiles = seqs->pair_tiles, a.longest_tiles = (seqs->longest + kTileRows - 1) / kTileRows, a.splits = 1;
+  a.pair_tiles = seqs->pair_tiles, a.longest_tiles = (seqs->longest + kTileRows - 1) / kTileRows, a.splits = 1, a.share = 1 << 30;
   use_tiles(a, seqs, seqs->packed);
-  if (on_tensor_cores(a, seqs)) return attention_sm100(a, seqs, st);
+  const Path path = path_of(a, seqs);
+  if (path == Path::kTensor) return attention_sm100(a, seqs, st);
   use_tiles(a, seqs, seqs->plain);
+  if (path == Path::kShort) return attention_short(a, (int)seqs->longest, st);
   return attention_simt(a, st);
 }
 
@@ -601,10 +610,12 @@ extern "C" lmpb_status lmpb_attention_backward(const float* q, const float* k, c
   a.q = q, a.k = k, a.v = v, a.out = const_cast<float*>(out), a.lse = const_cast<float*>(lse), a.grad = grad;
   a.dq = dq, a.dk = dk, a.dv = dv;
   a.tokens = tokens, a.heads = heads, a.kv_heads = kv_heads, a.dim = head_dim, a.scale = scale;
-  a.used = seqs->tokens, a.pair_tiles = seqs->pair_tiles, a.longest_tiles = (seqs->longest + kTileRows - 1) / kTileRows, a.splits = 1;
+  a.pair_tiles = seqs->pair_tiles, a.longest_tiles = (seqs->longest + kTileRows - 1) / kTileRows, a.splits = 1, a.share = 1 << 30;
   use_tiles(a, seqs, seqs->packed);
-  if (on_tensor_cores(a, seqs)) return attention_sm100_backward(a, seqs, st);
+  const Path path = path_of(a, seqs);
+  if (path == Path::kTensor) return attention_sm100_backward(a, seqs, st);
   use_tiles(a, seqs, seqs->plain);
+  if (path == Path::kShort) return attention_short_backward(a, (int)seqs->longest, st);
   float* delta = nullptr;
   LMPB_CUDA_TRY(stream_alloc((void**)&delta, (size_t)tokens * heads * 4, st));
   const int64_t rows = seqs->tokens * heads;

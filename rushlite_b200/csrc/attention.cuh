@@ -44,11 +44,10 @@ struct AttentionArgs {
   const int *by_queries, *by_keys;
   int tiles;
   const uchar2* pack;
-  int64_t used;           // tokens of the sequences
   int64_t pair_tiles;     // query tile, key tile pairs
   int64_t longest_tiles;  // of one sequence
-  // dk, dv work of a key tile cut into `splits`, whose results go to `part`.
-  int splits;
+  // dk, dv work of a key tile in shares of `share` blocks, `splits` at most.
+  int splits, share;
   float* part;
   // Per head plane and tile: not 0 where the tensor-core path's fp16 split
   // cannot carry the tile's values.  Null: every tile is computed here.
@@ -67,6 +66,11 @@ lmpb_status attention_sm100(const AttentionArgs& a, const lmpb_sequences_s* seqs
 lmpb_status attention_sm100_backward(const AttentionArgs& a, const lmpb_sequences_s* seqs, cudaStream_t st);
 // Points `a` at one of the sequences' lists of tiles.
 void use_tiles(AttentionArgs& a, const lmpb_sequences_s* seqs, const lmpb_sequences_s::Tiles& t);
+
+// A few sequences of at most kShortRows tokens (attention_short.cu).
+constexpr int kShortRows = 32;
+lmpb_status attention_short(const AttentionArgs& a, int longest, cudaStream_t st);
+lmpb_status attention_short_backward(const AttentionArgs& a, int longest, cudaStream_t st);  // computes delta itself
 
 // fp32 kernels for any values and lengths (attention.cu).
 lmpb_status attention_simt(const AttentionArgs& a, cudaStream_t st);

@@ -35,8 +35,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <mutex>
-#include <vector>
+#include <type_traits>
 
 #include "attention.cuh"
 #include "tcgen05.cuh"
@@ -84,22 +83,62 @@ struct Split {
 
 // ------------------------------------------------------------ split pass
 
+// Two floats in one 64-bit register: sm_100 multiplies and adds them in one
+// instruction, and the computing warps are bound by instructions and by the
+// power that these take.
+struct Two {
+  unsigned long long v;
+  __device__ __forceinline__ Two() {}
+  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ explicit Two(float a) : Two(a, a) {}
+  __device__ __forceinline__ float2 get() const {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+  }
+};
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ Two bits2(uint32_t a, uint32_t b) { return Two(__uint_as_float(a), __uint_as_float(b)); }
+
 // hi and lo of two values, packed.
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(a, b);
+__device__ __forceinline__ void split2(Two x, uint32_t& hi, uint32_t& lo) {
+  const float2 a = x.get();
+  const __half2 h = __floats2half2_rn(a.x, a.y);
   const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(__fsub_rn(a, f.x), __fsub_rn(b, f.y));
+  const float2 d = fma2(Two(f.x, f.y), Two(-1.f), x).get();  // x - hi, exact
+  const __half2 l = __floats2half2_rn(d.x, d.y);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
 __device__ __forceinline__ float two_to(int e) { return __int_as_float((e + 127) << 23); }  // e in [-126, 127]
 
-// Grid: tiles x planes, 256 threads, a warp per 16 rows.  Lane l holds
-// columns 4 l.. of a row (DP = 128), or lanes l and l + 16 hold one of two rows (DP = 64).
+// Grid: tiles x planes; a warp holds 8 rows (DP = 128) or 16 in registers.
+// Lane l holds columns 4 l.. of a row (DP = 128), or lanes l and l + 16 hold
+// one of two rows (DP = 64).  Bound by HBM and, one tile a CTA, by latency:
+// 32 warps an SM are needed ([1500, 31, 700, 1, 1865] x 24 planes of 128: 27
+// us with 16 rows a warp, 25 with 8; 40 planes of the backward: 64 and 50).
 template <int DP>
-__global__ void __launch_bounds__(256) split_kernel(const AttentionArgs a, const Split o, float* __restrict__ delta, bool vec) {
-  constexpr int RPS = 128 / DP, STEPS = 16 / RPS, LANES = 32 / RPS;  // rows a step, steps, lanes a row
+constexpr int split_warps() { return DP / 8; }
+
+template <int DP>
+__global__ void __launch_bounds__(32 * split_warps<DP>(), 2048 / (64 * split_warps<DP>())) split_kernel(const AttentionArgs a, const Split o, float* __restrict__ delta, bool vec) {
+  constexpr int WARPS = split_warps<DP>(), ROWS = 128 / WARPS;  // of a warp
+  constexpr int RPS = 128 / DP, STEPS = ROWS / RPS, LANES = 32 / RPS;  // rows a step, steps, lanes a row
   const int64_t plane = blockIdx.y;
   const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int4 tile = a.tile[t];
@@ -128,7 +167,7 @@ __global__ void __launch_bounds__(256) split_kernel(const AttentionArgs a, const
   };
   float4 v[STEPS];
 #pragma unroll
-  for (int i = 0; i < STEPS; ++i) v[i] = load4(base, warp * 16 + i * RPS + sub);
+  for (int i = 0; i < STEPS; ++i) v[i] = load4(base, warp * ROWS + i * RPS + sub);
   float mx = 0.f, mn = INFINITY, nrm = 0.f, dmx = 0.f;
   bool bad = false;
 #pragma unroll
@@ -141,7 +180,7 @@ __global__ void __launch_bounds__(256) split_kernel(const AttentionArgs a, const
     if (m > 0.f) mn = fminf(mn, m);
     if (is_v || is_g) {
       float q = v[i].x * v[i].x + v[i].y * v[i].y + v[i].z * v[i].z + v[i].w * v[i].w, d = 0.f;
-      const int r = warp * 16 + i * RPS + sub;
+      const int r = warp * ROWS + i * RPS + sub;
       if (is_g) {
         const float4 u = load4(obase, r);
         d = v[i].x * u.x + v[i].y * u.y + v[i].z * u.z + v[i].w * u.w;
@@ -156,7 +195,7 @@ __global__ void __launch_bounds__(256) split_kernel(const AttentionArgs a, const
       if (is_g && lane % LANES == 0 && r < rows) delta[(int64_t)head * a.tokens + first + r] = d;
     }
   }
-  __shared__ float red[4][8];
+  __shared__ float red[4][WARPS];
 #pragma unroll
   for (int s = 16; s; s >>= 1) {
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
@@ -167,7 +206,7 @@ __global__ void __launch_bounds__(256) split_kernel(const AttentionArgs a, const
   if (lane == 0) red[0][warp] = mx, red[1][warp] = mn, red[2][warp] = nrm, red[3][warp] = dmx;
   const int bads = __syncthreads_or(bad);
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
+  for (int w = 0; w < WARPS; ++w) {
     mx = fmaxf(mx, red[0][w]);
     mn = fminf(mn, red[1][w]);
     nrm = fmaxf(nrm, red[2][w]);
@@ -190,10 +229,10 @@ __global__ void __launch_bounds__(256) split_kernel(const AttentionArgs a, const
   unsigned char* out = o.blocks + block * block_bytes<DP>();
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
-    const int r = warp * 16 + i * RPS + sub;
+    const int r = warp * ROWS + i * RPS + sub;
     uint2 hi, lo;
-    split2(v[i].x * s, v[i].y * s, hi.x, lo.x);
-    split2(v[i].z * s, v[i].w * s, hi.y, lo.y);
+    split2(Two(v[i].x * s, v[i].y * s), hi.x, lo.x);
+    split2(Two(v[i].z * s, v[i].w * s), hi.y, lo.y);
     // 16-byte chunk c of row r sits at chunk c ^ (r & 7) of its 128 bytes
     const int byte = (col & 63) * 2, at = (col >> 6) * 16384 + r * 128 + ((((byte >> 4) ^ (r & 7)) << 4) | (byte & 15));
     *reinterpret_cast<uint2*>(out + at) = hi;
@@ -259,6 +298,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+__device__ __forceinline__ Two exp2_fast(Two x) {
+  const float2 f = x.get();
+  return Two(exp2_fast(f.x), exp2_fast(f.y));
+}
+
 // A computing warp's wait: all its lanes go on together, with what the
 // barrier orders before them visible to their tcgen05 operations.
 __device__ __forceinline__ void warp_wait(Waiter& wait, uint32_t bar, uint32_t parity) {
@@ -267,7 +311,7 @@ __device__ __forceinline__ void warp_wait(Waiter& wait, uint32_t bar, uint32_t p
   tc_fence_after();
 }
 
-// Barrier of the computing warps.
+// Barrier of the WARPS computing warps.
 template <int WARPS>
 __device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); }
 
@@ -329,7 +373,7 @@ template <int DP, int N>
 struct Issuer {
   Ring<DP, N> ring;
   Waiter wait;
-  bool landed = false;  // the ring's next part, as far as is known
+  bool landed = false;  // what take() waits for, as far as is known
 
   __device__ __forceinline__ Issuer(uint32_t parts, uint32_t bars, unsigned code) : ring{parts, bars}, wait(code) {}
 
@@ -343,63 +387,90 @@ struct Issuer {
   __device__ __forceinline__ bool test(uint32_t bar, uint32_t parity) const {
     return __all_sync(0xffffffffu, mbar_test(bar, parity));
   }
+  // The next operand: with DP = 64 both its parts, else the first.
   __device__ __forceinline__ bool take() {
     if (landed) tc_fence_after();
     else if (!wait_for(ring.full(), ring.phase)) return false;
+    if (DP == 64 && !landed) {
+      Ring<DP, N> second = ring;
+      second.next();
+      if (!wait_for(second.full(), second.phase)) return false;
+    }
     landed = false;
     return true;
   }
 
   // D[128, 128] = A (shared, resident block) . B^T, B the ring's next tile.
+  // `done`, if not 0, is signalled when this and all products before are done.
   template <typename Ahead>
-  __device__ __forceinline__ void columns(uint32_t d, uint32_t a_block, Ahead ahead) {
+  __device__ __forceinline__ void columns(uint32_t d, uint32_t a_block, uint32_t done, Ahead ahead) {
     constexpr uint32_t idesc = idesc_of(128, false);
     constexpr int U = DP / 64;
     const uint32_t ah = desc_lo(a_block, 16), al = ah + (part_bytes<DP>() >> 4);
     product<4 * U>([&](uint32_t b, int k, bool lo_a, uint32_t acc) {  // 16 columns = 32 bytes a step, 64 a swizzle atom
       const uint32_t o = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
       mma_ss(d, (lo_a ? al : ah) + o, b + o, idesc, acc);
-    }, 16, ahead);
+    }, 16, done, ahead);
   }
 
   // D[128, DP] = W . B, W the split weights in TMEM (16 columns for 16
   // tokens: 8 of hi, 8 of lo), B the ring's next tile.
   template <typename Ahead>
-  __device__ __forceinline__ void rows(uint32_t d, uint32_t w, Ahead ahead) {
+  __device__ __forceinline__ void rows(uint32_t d, uint32_t w, uint32_t done, Ahead ahead) {
     constexpr uint32_t idesc = idesc_of(DP, true);
     product<8>([&](uint32_t b, int k, bool lo_w, uint32_t acc) {  // 16 rows = 2048 bytes a step
       mma_ts(d, w + k * 16 + (lo_w ? 8 : 0), b + k * (2048 >> 4), idesc, acc);
-    }, 16384, ahead);
+    }, 16384, done, ahead);
   }
 
+  // With DP = 64 a product is 768 clocks of MMAs, against which three separate
+  // runs of the issuing lane weigh too much: both parts are awaited at once.
+  // With DP = 128 it is 1,536, and the ring is too short to hold them so long.
   template <int STEPS, typename Mma, typename Ahead>
-  __device__ __forceinline__ void product(Mma mma, uint32_t lbo, Ahead ahead) {
+  __device__ __forceinline__ void product(Mma mma, uint32_t lbo, uint32_t done, Ahead ahead) {
     if (!take()) return;
-    uint32_t b = desc_lo(ring.part(), lbo);
-    if (elect_one()) {
-#pragma unroll
-      for (int k = 0; k < STEPS; ++k) mma(b, k, false, k != 0);
-      mma_commit(ring.empty());
-    }
-    __syncwarp();
+    const uint32_t lo = desc_lo(ring.part(), lbo), lo_free = ring.empty();
     ring.next();
-    if (!wait_for(ring.full(), ring.phase)) return;
-    b = desc_lo(ring.part(), lbo);
-    if (elect_one()) {
+    if (DP == 128) {
+      if (elect_one()) {
 #pragma unroll
-      for (int k = 0; k < STEPS; ++k) mma(b, k, true, 1);
+        for (int k = 0; k < STEPS; ++k) mma(lo, k, false, k != 0);
+        mma_commit(lo_free);
+      }
+      __syncwarp();
+      if (!wait_for(ring.full(), ring.phase)) return;
     }
-    __syncwarp();
-    const uint32_t free_bar = ring.empty();
+    const uint32_t hi = desc_lo(ring.part(), lbo), hi_free = ring.empty();
     ring.next();
-    landed = test(ring.full(), ring.phase);
-    ahead();
-    if (elect_one()) {
+    if (DP == 128) {
+      if (elect_one()) {
 #pragma unroll
-      for (int k = 0; k < STEPS; ++k) mma(b, k, false, 1);
-      mma_commit(free_bar);
+        for (int k = 0; k < STEPS; ++k) mma(hi, k, true, 1);
+      }
+      __syncwarp();
+      landed = test(ring.full(), ring.phase);
+      ahead();
+    }
+    if (elect_one()) {
+      if (DP == 64) {
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) mma(lo, k, false, k != 0);
+        mma_commit(lo_free);
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) mma(hi, k, true, 1);
+      }
+#pragma unroll
+      for (int k = 0; k < STEPS; ++k) mma(hi, k, false, 1);
+      mma_commit(hi_free);
+      if (done) mma_commit(done);
     }
     __syncwarp();
+    if (DP == 64) {
+      Ring<DP, N> second = ring;
+      second.next();
+      landed = test(ring.full(), ring.phase) && test(second.full(), second.phase);
+      ahead();
+    }
   }
 };
 
@@ -425,10 +496,13 @@ struct Warps {
   static __device__ __forceinline__ void many() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(HIGH)); }
 };
 using Warps8 = Warps<8, 168, 88, 208>;
-using Warps16 = Warps<16, 96, 56, 104>;
-// Forward with DP = 64, where the weights' arithmetic bounds: 16 warps, 0.446
-// ms for [8192] x 16 heads (8 warps: 0.467); with DP = 128, where the tensor
-// core does, 8 warps: 1.24 ms for [16384] x 8 (16: 1.25; that backward: 4.94, 5.10).
+template <int DP>
+using WarpsKV = std::conditional_t<DP == 64, Warps<8, 168, 104, 200>, Warps8>;
+using Warps16 = Warps<16, 96, 64, 104>;
+// Forward with DP = 64, where the weights' arithmetic weighs as much as the
+// MMAs: 16 warps (0.390 ms for [8192] x 16 heads; 8 warps 0.44, two
+// pipelines of 8 warps that take the key blocks in turn 0.42).  With DP = 128,
+// where the MMAs outweigh it, 8 warps of twice the registers.
 template <int DP>
 using ForwardWarps = std::conditional_t<DP == 64, Warps16, Warps8>;
 
@@ -512,8 +586,8 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar) {
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
-// acc = acc * alpha + f * this thread's C columns of a drained block.
-template <int C>
+// acc = acc (* alpha) + f * this thread's C columns of a drained block.
+template <int C, bool RESCALE>
 __device__ __forceinline__ void drain(uint32_t taddr, float (&acc)[C], float alpha, float f) {
 #pragma unroll
   for (int c = 0; c < C; c += 16) {
@@ -522,7 +596,11 @@ __device__ __forceinline__ void drain(uint32_t taddr, float (&acc)[C], float alp
     tmem_ld_wait();
     tmem_regs_ready(r);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[c + i] = fmaf(__uint_as_float(r[i]), f, acc[c + i] * alpha);
+    for (int i = 0; i < 16; i += 2) {
+      const Two x(acc[c + i], acc[c + i + 1]);
+      const float2 s = fma2(bits2(r[i], r[i + 1]), Two(f), RESCALE ? mul2(x, Two(alpha)) : x).get();
+      acc[c + i] = s.x, acc[c + i + 1] = s.y;
+    }
   }
 }
 
@@ -556,11 +634,11 @@ __global__ void __launch_bounds__(ForwardWarps<DP>::kThreads, 1) forward_kernel(
   constexpr int RING = forward_ring<DP>();
   const uint32_t base = smem_u32(smem), bars = base + L::kBarsAt;
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + L::kBarsAt + kBars * 8);
-  float* xch = reinterpret_cast<float*>(smem + L::kScratch);  // [2][PARTS][128]
   // q, scores of each parity, weights, product of each parity, end
   const int counts[7] = {1, 1, 1, WARPS, 1, 1, 1};
   if (!setup(smem, bars, slot, RING, counts, 7)) return;
   const uint32_t qfull = bars + 16 * RING, sfull = qfull + 8, pfull = qfull + 24, ofull = qfull + 32, done = qfull + 48;
+  const auto phase2 = [](int j) { return (uint32_t)(j >> 1) & 1; };  // of a barrier that every other block uses
   constexpr uint32_t tmem = 0;  // all of it was allocated
   const int order = blockIdx.x / a.heads, head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
   const int t = a.by_queries[order];
@@ -572,40 +650,37 @@ __global__ void __launch_bounds__(ForwardWarps<DP>::kThreads, 1) forward_kernel(
   const int warp = threadIdx.x >> 5;
   if (warp < 4) {
     W::few();
+    const unsigned char *kblocks = sp.blocks + kplane * block_bytes<DP>(), *vblocks = sp.blocks + vplane * block_bytes<DP>();
     if (warp == 0 && (threadIdx.x & 31) == 0) {
       Ring<DP, RING> ring{base + L::kRing, bars};
       Waiter wait(1);
       mbar_expect_tx(qfull, block_bytes<DP>());
       bulk_load(base, sp.blocks + qblock * block_bytes<DP>(), block_bytes<DP>(), qfull);
-      feed(ring, wait, sp.blocks + kplane * block_bytes<DP>());
+      feed(ring, wait, kblocks);
       for (int j = 0; j < n; ++j) {
-        if (j + 1 < n) feed(ring, wait, sp.blocks + (kplane + j + 1) * block_bytes<DP>());
-        feed(ring, wait, sp.blocks + (vplane + j) * block_bytes<DP>());
+        if (j + 1 < n) feed(ring, wait, kblocks + (j + 1) * block_bytes<DP>());
+        feed(ring, wait, vblocks + j * block_bytes<DP>());
       }
       feed_done(ring);
       Waiter last(32);
       last(qfull, 0);
     } else if (warp == 1) {
-    Issuer<DP, RING> mma(base + L::kRing, bars, 2);
-    const auto nothing = [] {};
-    mma.wait_for(qfull, 0);
-    mma.columns(tmem, base, nothing);
-    commit(sfull);
-    for (int j = 0; j < n && mma.wait.ok; ++j) {
-      // block j's weights; that they are there also says that block j - 2's product is drained
-      bool weights = false;
-      if (j + 1 < n) {
-        mma.columns(tmem + ((j + 1) & 1) * 128, base, [&] { weights = mma.test(pfull, j & 1); });
-        commit(sfull + 8 * ((j + 1) & 1));
+      Issuer<DP, RING> mma(base + L::kRing, bars, 2);
+      const auto nothing = [] {};
+      mma.wait_for(qfull, 0);
+      mma.columns(tmem, base, sfull, nothing);
+      for (int j = 0; j < n && mma.wait.ok; ++j) {
+        // block j's weights; that they are there also says that block j - 2's product is drained
+        bool weights = false;
+        if (j + 1 < n)
+          mma.columns(tmem + ((j + 1) & 1) * 128, base, sfull + 8 * ((j + 1) & 1), [&] { weights = mma.test(pfull, j & 1); });
+        if (!weights) mma.wait_for(pfull, j & 1);
+        else tc_fence_after();
+        if (mma.wait.ok) mma.rows(tmem + 256 + (j & 1) * 128, tmem + (j & 1) * 128, ofull + 8 * (j & 1), nothing);
       }
-      if (!weights) mma.wait_for(pfull, j & 1);
-      else tc_fence_after();
-      if (mma.wait.ok) mma.rows(tmem + 256 + (j & 1) * 128, tmem + (j & 1) * 128, nothing);
-      commit(ofull + 8 * (j & 1));
-    }
-    Waiter last(33);  // nothing of this CTA is in flight when it ends
-    commit(done);
-    last(done, 0);
+      Waiter last(33);  // nothing of this CTA is in flight when it ends
+      commit(done);
+      last(done, 0);
     }
   } else {
     W::many();
@@ -622,67 +697,71 @@ __global__ void __launch_bounds__(ForwardWarps<DP>::kThreads, 1) forward_kernel(
     const int low = a.low_of(tile, me.row), col0 = me.part * COLS - low;
     const unsigned span = me.row - low + 1;
     const uint32_t own = tmem + me.lanes + me.part * COLS, oown = tmem + 256 + me.lanes + me.part * C;
-    for (int j = 0; j < n; ++j) {
+    float* xch = reinterpret_cast<float*>(smem + L::kScratch) + me.row;  // [2][PARTS][128]
+    const auto drain_block = [&](int j) {
+      warp_wait(wait, ofull + 8 * (j & 1), phase2(j));
+      drain<C, true>(oown + (j & 1) * 128, acc, alpha, of);
+    };
+    const auto block = [&](int j, auto diagonal) {
+      constexpr bool diag = decltype(diagonal)::value;
       const float c = ldexpf(a.scale * kLog2e, -(eq + ek));
       const float f = two_to(-ev);
       if (j + 1 < n) ek = sp.expo[kplane + j + 1], ev = sp.expo[vplane + j + 1];
       const uint32_t s = own + (j & 1) * 128;
-      const bool diag = j + 1 == n;
-      warp_wait(wait, sfull + 8 * (j & 1), (j >> 1) & 1);
-      uint32_t r[COLS / 16][16];
-#pragma unroll
-      for (int k = 0; k < COLS / 16; ++k) tmem_ld16_issue(s + 16 * k, r[k]);
-      tmem_ld_wait();
-      float mx = -INFINITY;
-#pragma unroll
-      for (int k = 0; k < COLS / 16; ++k) {
-        tmem_regs_ready(r[k]);
+      warp_wait(wait, sfull + 8 * (j & 1), phase2(j));
+      // scores are read twice, for the maximum and for the weights: kept, they
+      // would spill, and with all of L1 given to shared memory that costs more
+            float mx = -INFINITY;
+#pragma unroll 2
+      for (int k = 0; k < COLS; k += 16) {
+        uint32_t r[16];
+        tmem_ld16(s + k, r);
         if (diag) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (unsigned(col0 + 16 * k + i) >= span) r[k][i] = 0xff800000u;  // -inf
+            if (unsigned(col0 + k + i) >= span) r[i] = 0xff800000u;  // -inf
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, __uint_as_float(r[k][i]));
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
       }
-      float* x = xch + (j & 1) * (128 * PARTS) + me.row;
+      float* x = xch + (j & 1) * (128 * PARTS);
       x[me.part * 128] = mx;
       compute_sync<WARPS>();
 #pragma unroll
       for (int k = 0; k < PARTS; ++k) mx = fmaxf(mx, x[k * 128]);
-      const float mn = fmaxf(m, mx * c);  // finite: the first block has a key for every row
+      const float mn = fmaxf(m, mx * c);  // finite: every row sees a key of every block
       const float next = exp2_fast(m - mn), bias = kWeightBits - mn;
-      float sum = 0.f;
-#pragma unroll
-      for (int k = 0; k < COLS / 16; ++k) {
-        uint32_t w[16];
+      Two sums(0.f);
+#pragma unroll 2
+      for (int k = 0; k < COLS; k += 16) {
+        uint32_t r[16], w[16];
+        tmem_ld16(s + k, r);
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          float p0 = exp2_fast(fmaf(__uint_as_float(r[k][i]), c, bias));
-          float p1 = exp2_fast(fmaf(__uint_as_float(r[k][i + 1]), c, bias));
+          Two p = exp2_fast(fma2(bits2(r[i], r[i + 1]), Two(c), Two(bias)));
           if (diag) {  // by index: a scale of 0 makes NaN of -inf
-            if (unsigned(col0 + 16 * k + i) >= span) p0 = 0.f;
-            if (unsigned(col0 + 16 * k + i + 1) >= span) p1 = 0.f;
+            float2 q = p.get();
+            if (unsigned(col0 + k + i) >= span) q.x = 0.f;
+            if (unsigned(col0 + k + i + 1) >= span) q.y = 0.f;
+            p = Two(q.x, q.y);
           }
-          sum += p0 + p1;
-          split2(p0, p1, w[i / 2], w[8 + i / 2]);
+          sums = add2(sums, p);
+          split2(p, w[i / 2], w[8 + i / 2]);
         }
-        tmem_st16(s + 16 * k, w);
+        tmem_st16(s + k, w);
       }
       tmem_st_wait();
       warp_arrive(pfull);
-      l = l * next + sum;
+      l = l * next + (sums.get().x + sums.get().y);
       m = mn;
-      if (j > 0) {
-        warp_wait(wait, ofull + 8 * ((j - 1) & 1), ((j - 1) >> 1) & 1);
-        drain<C>(oown + ((j - 1) & 1) * 128, acc, alpha, of);
-      }
+      if (j > 0) drain_block(j - 1);
       alpha = next;
       of = f;
-    }
-    warp_wait(wait, ofull + 8 * ((n - 1) & 1), ((n - 1) >> 1) & 1);
-    drain<C>(oown + ((n - 1) & 1) * 128, acc, alpha, of);
-    float* x = xch + (n & 1) * (128 * PARTS) + me.row;
+    };
+    for (int j = 0; j + 1 < n; ++j) block(j, std::false_type{});
+    block(n - 1, std::true_type{});
+    drain_block(n - 1);
+    float* x = xch + (n & 1) * (128 * PARTS);
     x[me.part * 128] = l;
     compute_sync<WARPS>();
     l = 0.f;
@@ -770,22 +849,19 @@ __global__ void __launch_bounds__(Warps8::kThreads, 1) dq_kernel(const Attention
     Issuer<DP, RING> mma(base + L::kRing, bars, 12);
     const auto nothing = [] {};
     mma.wait_for(resident, 0);
-    mma.columns(tmem, base, nothing);
-    mma.columns(tmem + 256, base + BB, nothing);
-    commit(spfull);
+    mma.columns(tmem, base, 0, nothing);
+    mma.columns(tmem + 256, base + BB, spfull, nothing);
     for (int j = 0; j < n && mma.wait.ok; ++j) {
       bool ds = false, drained = false;
-      if (j + 1 < n) mma.columns(tmem + ((j + 1) & 1) * 128, base, [&] { ds = mma.test(dsfull, j & 1); });
+      if (j + 1 < n) mma.columns(tmem + ((j + 1) & 1) * 128, base, 0, [&] { ds = mma.test(dsfull, j & 1); });
       if (!ds) mma.wait_for(dsfull, j & 1);
       else tc_fence_after();
       if (j + 1 < n && mma.wait.ok) {
-        mma.columns(tmem + 256, base + BB, [&] { drained = mma.test(oempty, (j & 1) ^ 1); });
-        commit(spfull);
+        mma.columns(tmem + 256, base + BB, spfull, [&] { drained = mma.test(oempty, (j & 1) ^ 1); });
       }
       if (!drained) mma.wait_for(oempty, (j & 1) ^ 1);
       else tc_fence_after();
-      if (mma.wait.ok) mma.rows(tmem + 384, tmem + (j & 1) * 128, nothing);
-      commit(ofull);
+      if (mma.wait.ok) mma.rows(tmem + 384, tmem + (j & 1) * 128, ofull, nothing);
     }
     Waiter last(33);
     commit(done);
@@ -810,13 +886,13 @@ __global__ void __launch_bounds__(Warps8::kThreads, 1) dq_kernel(const Attention
     const int low = a.low_of(tile, me.row), col0 = me.part * COLS - low;
     const unsigned span = me.row - low + 1;
     const uint32_t own = tmem + me.lanes + me.part * COLS, oown = tmem + 384 + me.lanes + me.part * C;
-    for (int j = 0; j < n; ++j) {
+    const auto block = [&](int j, auto diagonal) {
+      constexpr bool diag = decltype(diagonal)::value;
       const float c = ldexpf(a.scale * kLog2e, -(eq + ek));
       const DsScale ds = ds_scale(gnorm, vnorm, dmax, eg, ev, 0.f);
       const float f = ldexpf(a.scale, -(ds.e + ek)), dd = delta * ds.d;
       if (j + 1 < n) ek = sp.expo[kplane + j + 1], ev = sp.expo[vplane + j + 1], vnorm = sp.norm[vplane + j + 1];
       const uint32_t s = own + (j & 1) * 128, dp = own + 256;
-      const bool diag = j + 1 == n;
       warp_wait(wait, spfull, j & 1);
 #pragma unroll
       for (int k = 0; k < COLS; k += 16) {
@@ -828,13 +904,15 @@ __global__ void __launch_bounds__(Warps8::kThreads, 1) dq_kernel(const Attention
         tmem_regs_ready(u);
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          float d0 = exp2_fast(fmaf(__uint_as_float(r[i]), c, -lse)) * fmaf(__uint_as_float(u[i]), ds.dp, -dd);
-          float d1 = exp2_fast(fmaf(__uint_as_float(r[i + 1]), c, -lse)) * fmaf(__uint_as_float(u[i + 1]), ds.dp, -dd);
+          const Two p = exp2_fast(fma2(bits2(r[i], r[i + 1]), Two(c), Two(-lse)));
+          Two d = mul2(p, fma2(bits2(u[i], u[i + 1]), Two(ds.dp), Two(-dd)));
           if (diag) {
-            if (unsigned(col0 + k + i) >= span) d0 = 0.f;
-            if (unsigned(col0 + k + i + 1) >= span) d1 = 0.f;
+            float2 q = d.get();
+            if (unsigned(col0 + k + i) >= span) q.x = 0.f;
+            if (unsigned(col0 + k + i + 1) >= span) q.y = 0.f;
+            d = Two(q.x, q.y);
           }
-          split2(d0, d1, w[i / 2], w[8 + i / 2]);
+          split2(d, w[i / 2], w[8 + i / 2]);
         }
         tmem_st16(s + k, w);
       }
@@ -842,13 +920,15 @@ __global__ void __launch_bounds__(Warps8::kThreads, 1) dq_kernel(const Attention
       warp_arrive(dsfull);
       if (j > 0) {
         warp_wait(wait, ofull, (j - 1) & 1);
-        drain<C>(oown, acc, 1.f, of);
+        drain<C, false>(oown, acc, 1.f, of);
         warp_arrive(oempty);
       }
       of = f;
-    }
+    };
+    for (int j = 0; j + 1 < n; ++j) block(j, std::false_type{});
+    block(n - 1, std::true_type{});
     warp_wait(wait, ofull, (n - 1) & 1);
-    drain<C>(oown, acc, 1.f, of);
+    drain<C, false>(oown, acc, 1.f, of);
     if (row < tile.y && wait.ok)
       store_row<C>(a.dq + ((int64_t)(tile.x + row) * a.heads + head) * a.dim, acc, me.part * C, a.dim, 1.f, vec_out);
   }
@@ -856,26 +936,40 @@ __global__ void __launch_bounds__(Warps8::kThreads, 1) dq_kernel(const Attention
 }
 
 // dk and dv of one key tile and key/value head, over the group's query heads
-// and their tiles from the diagonal on: one list of blocks, of which split s of
-// a.splits takes its share (a share may be empty).  With more than one split
-// the shares go to a.part, one after the other [splits, 2, tokens, kv_heads,
-// dim], which join_kernel adds in their order.  Rows are keys, columns queries.
+// and their tiles from the diagonal on: one list of blocks, cut into shares of
+// about a.share blocks.  Where a tile has more than one share, their results
+// go to a.part [splits, 2, tokens, kv_heads, dim], which join_kernel adds in
+// their order.  Rows are keys, columns queries.
 // TMEM: scores in columns [0, 128), overwritten by the weights; dP in
 // [128, 256), overwritten by dS; the block's shares of dv and dk in
 // [256, 256 + DP) and [384, 384 + DP).  The MMAs of a block run scores, dP,
 // dv, dk: weights are computed under dP, dS under dv.
 //
 // Both running sums are held in registers, 2 x DP / 2 a thread.
+// Shares of a key tile whose head has `per_head` query blocks; a.splits at most.
+__device__ __forceinline__ int shares_of(const AttentionArgs& a, int per_head) {
+  return min(a.splits, (per_head * (a.heads / a.kv_heads) + a.share - 1) / a.share);
+}
+
 template <int DP>
-__global__ void __launch_bounds__(Warps8::kThreads, 1) dkv_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
+__global__ void __launch_bounds__(WarpsKV<DP>::kThreads, 1) dkv_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
   extern __shared__ __align__(1024) unsigned char smem[];
   using L = BackwardLayout<DP>;
-  using W = Warps8;
+  using W = WarpsKV<DP>;
   constexpr int WARPS = W::kWarps, PARTS = W::kParts, COLS = W::kCols;
   constexpr int RING = backward_ring<DP>();
   const uint32_t base = smem_u32(smem), bars = base + L::kBarsAt;
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + L::kBarsAt + kBars * 8);
-  float* stat = reinterpret_cast<float*>(smem + L::kScratch);  // [2][2][128]: weight offset, scaled delta
+  float* stat = reinterpret_cast<float*>(smem + L::kScratch);  // [2][2][128]: weight offset, -scaled delta
+  const int per_order = a.kv_heads * a.splits, order = blockIdx.x / per_order, kv_head = blockIdx.x % per_order / a.splits;
+  const int split = blockIdx.x % a.splits, group = a.heads / a.kv_heads;
+  const int t = a.by_keys[order];
+  const int4 tile = a.tile[t];
+  const int per_head = (tile.y + kTileRows - 1) / kTileRows - tile.z;  // query blocks of a head
+  const int shares = shares_of(a, per_head);
+  if (split >= shares) return;
+  const int first = (int)((int64_t)per_head * group * split / shares);
+  const int n = (int)((int64_t)per_head * group * (split + 1) / shares) - first;
   // k and v, scores, dP, weights, dS, dv, dv drained, dk, dk drained, end
   const int counts[10] = {1, 1, 1, WARPS, WARPS, 1, WARPS, 1, WARPS, 1};
   if (!setup(smem, bars, slot, RING, counts, 10)) return;
@@ -883,13 +977,6 @@ __global__ void __launch_bounds__(Warps8::kThreads, 1) dkv_kernel(const Attentio
                  dsfull = resident + 32, vfull = resident + 40, vempty = resident + 48, kfull = resident + 56,
                  kempty = resident + 64, done = resident + 72;
   constexpr uint32_t tmem = 0;  // all of it was allocated
-  const int per_order = a.kv_heads * a.splits, order = blockIdx.x / per_order, kv_head = blockIdx.x % per_order / a.splits;
-  const int split = blockIdx.x % a.splits, group = a.heads / a.kv_heads;
-  const int t = a.by_keys[order];
-  const int4 tile = a.tile[t];
-  const int per_head = (tile.y + kTileRows - 1) / kTileRows - tile.z;  // query blocks of a head
-  const int first = (int)((int64_t)per_head * group * split / a.splits);
-  const int n = (int)((int64_t)per_head * group * (split + 1) / a.splits) - first;
   const int64_t kblock = (int64_t)(a.heads + kv_head) * a.tiles + t;
   const int64_t vblock = kblock + (int64_t)a.kv_heads * a.tiles;
   const int64_t gplanes = (int64_t)(a.heads + 2 * a.kv_heads) * a.tiles;
@@ -923,20 +1010,16 @@ __global__ void __launch_bounds__(Warps8::kThreads, 1) dkv_kernel(const Attentio
       mma.wait_for(resident, 0);
       for (int i = 0; i < n && mma.wait.ok; ++i) {
         bool p = false, v = false, ds = false, k = false;
-        mma.columns(tmem, base, nothing);
-        commit(sfull);
-        mma.columns(tmem + 128, base + BB, [&] { p = mma.test(pfull, i & 1), v = mma.test(vempty, (i & 1) ^ 1); });
-        commit(dpfull);
+        mma.columns(tmem, base, sfull, nothing);
+        mma.columns(tmem + 128, base + BB, dpfull, [&] { p = mma.test(pfull, i & 1), v = mma.test(vempty, (i & 1) ^ 1); });
         if (!p) mma.wait_for(pfull, i & 1);
         if (!v) mma.wait_for(vempty, (i & 1) ^ 1);
         tc_fence_after();
-        if (mma.wait.ok) mma.rows(tmem + 256, tmem, [&] { ds = mma.test(dsfull, i & 1), k = mma.test(kempty, (i & 1) ^ 1); });
-        commit(vfull);
+        if (mma.wait.ok) mma.rows(tmem + 256, tmem, vfull, [&] { ds = mma.test(dsfull, i & 1), k = mma.test(kempty, (i & 1) ^ 1); });
         if (!ds) mma.wait_for(dsfull, i & 1);
         if (!k) mma.wait_for(kempty, (i & 1) ^ 1);
         tc_fence_after();
-        if (mma.wait.ok) mma.rows(tmem + 384, tmem + 128, nothing);
-        commit(kfull);
+        if (mma.wait.ok) mma.rows(tmem + 384, tmem + 128, kfull, nothing);
       }
       Waiter last(33);
       commit(done);
@@ -965,46 +1048,53 @@ __global__ void __launch_bounds__(Warps8::kThreads, 1) dkv_kernel(const Attentio
       const int64_t at = (int64_t)(kv_head * group + (first + i) / per_head) * a.tokens + tile.x + r;
       return r < tile.y ? __ldg(source + at) : tid < 128 ? INFINITY : 0.f;
     };
-    float next = n ? fetch(0) : 0.f;
+    float next = fetch(0);
     for (int i = 0; i < n; ++i) {
       const int64_t qb = qblock(i), gb = qb + gplanes;
       const int eq = sp.expo[qb], eg = sp.expo[gb];
       const float c = ldexpf(a.scale * kLog2e, -(eq + ek));
       const DsScale ds = ds_scale(sp.norm[gb], vnorm, sp.dmax[gb], eg, ev, kWeightBits);
       float* st = stat + (i & 1) * 256;
-      st[tid] = tid < 128 ? kWeightBits - next * kLog2e : next * ds.d;
+      st[tid] = tid < 128 ? kWeightBits - next * kLog2e : -next * ds.d;
       compute_sync<WARPS>();
       if (i + 1 < n) next = fetch(i + 1);
       const bool diag = (first + i) % per_head == 0;
       const float4* bias = reinterpret_cast<const float4*>(st + me.part * COLS);
       const float4* dd = reinterpret_cast<const float4*>(st + 128 + me.part * COLS);
       warp_wait(wait, sfull, i & 1);
+      const auto weights = [&](auto diagonal) {
 #pragma unroll
-      for (int k = 0; k < COLS; k += 16) {
-        uint32_t r[16], w[16];
-        tmem_ld16_issue(own + k, r);
-        tmem_ld_wait();
-        tmem_regs_ready(r);
+        for (int k = 0; k < COLS; k += 16) {
+          uint32_t r[16], w[16];
+          tmem_ld16_issue(own + k, r);
+          tmem_ld_wait();
+          tmem_regs_ready(r);
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-          const float4 b = bias[(k + j) / 4];
-          float p[4] = {exp2_fast(fmaf(__uint_as_float(r[j]), c, b.x)), exp2_fast(fmaf(__uint_as_float(r[j + 1]), c, b.y)),
-                        exp2_fast(fmaf(__uint_as_float(r[j + 2]), c, b.z)), exp2_fast(fmaf(__uint_as_float(r[j + 3]), c, b.w))};
-          if (diag) {
+          for (int j = 0; j < 16; j += 4) {
+            const float4 b = bias[(k + j) / 4];
+            Two p[2] = {exp2_fast(fma2(bits2(r[j], r[j + 1]), Two(c), Two(b.x, b.y))),
+                        exp2_fast(fma2(bits2(r[j + 2], r[j + 3]), Two(c), Two(b.z, b.w)))};
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              if (unsigned(col0 + k + j + x) >= span) p[x] = 0.f;
+            for (int x = 0; x < 2; ++x) {
+              if (decltype(diagonal)::value) {
+                float2 q = p[x].get();
+                if (unsigned(col0 + k + j + 2 * x) >= span) q.x = 0.f;
+                if (unsigned(col0 + k + j + 2 * x + 1) >= span) q.y = 0.f;
+                p[x] = Two(q.x, q.y);
+              }
+              split2(p[x], w[j / 2 + x], w[8 + j / 2 + x]);
+            }
           }
-          split2(p[0], p[1], w[j / 2], w[8 + j / 2]);
-          split2(p[2], p[3], w[j / 2 + 1], w[8 + j / 2 + 1]);
+          tmem_st16(own + k, w);
         }
-        tmem_st16(own + k, w);
-      }
+      };
+      if (diag) weights(std::true_type{});
+      else weights(std::false_type{});
       tmem_st_wait();
       warp_arrive(pfull);
       if (i > 0) {
         warp_wait(wait, kfull, (i - 1) & 1);
-        drain<C>(oown + 128, dk, 1.f, fk);
+        drain<C, false>(oown + 128, dk, 1.f, fk);
         warp_arrive(kempty);
       }
       warp_wait(wait, dpfull, i & 1);
@@ -1019,52 +1109,57 @@ __global__ void __launch_bounds__(Warps8::kThreads, 1) dkv_kernel(const Attentio
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
           const float4 d = dd[(k + j) / 4];
-          const float dx[4] = {d.x, d.y, d.z, d.w};
-          float v[4];
+          const Two nd[2] = {Two(d.x, d.y), Two(d.z, d.w)};
 #pragma unroll
-          for (int x = 0; x < 4; x += 2) {  // the weight is exactly hi + lo
-            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&r[(j + x) / 2]));
-            const float2 l = __half22float2(*reinterpret_cast<const __half2*>(&r[8 + (j + x) / 2]));
-            v[x] = (h.x + l.x) * fmaf(__uint_as_float(u[j + x]), ds.dp, -dx[x]);
-            v[x + 1] = (h.y + l.y) * fmaf(__uint_as_float(u[j + x + 1]), ds.dp, -dx[x + 1]);
+          for (int x = 0; x < 2; ++x) {  // the weight is exactly hi + lo
+            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&r[j / 2 + x]));
+            const float2 l = __half22float2(*reinterpret_cast<const __half2*>(&r[8 + j / 2 + x]));
+            const Two p = add2(Two(h.x, h.y), Two(l.x, l.y));
+            split2(mul2(p, fma2(bits2(u[j + 2 * x], u[j + 2 * x + 1]), Two(ds.dp), nd[x])), w[j / 2 + x], w[8 + j / 2 + x]);
           }
-          split2(v[0], v[1], w[j / 2], w[8 + j / 2]);
-          split2(v[2], v[3], w[j / 2 + 1], w[8 + j / 2 + 1]);
         }
         tmem_st16(own + 128 + k, w);
       }
       tmem_st_wait();
       warp_arrive(dsfull);
       warp_wait(wait, vfull, i & 1);
-      drain<C>(oown, dv, 1.f, two_to(-(int)kWeightBits - eg));
+      drain<C, false>(oown, dv, 1.f, two_to(-(int)kWeightBits - eg));
       warp_arrive(vempty);
       fk = ldexpf(a.scale, -(ds.e + eq));
     }
-    if (n) {
-      warp_wait(wait, kfull, (n - 1) & 1);
-      drain<C>(oown + 128, dk, 1.f, fk);
-    }
+    warp_wait(wait, kfull, (n - 1) & 1);
+    drain<C, false>(oown + 128, dk, 1.f, fk);
     const int row = tile.z * kTileRows + me.row;
     if (row < tile.y && wait.ok) {
       const int64_t at = ((int64_t)(tile.x + row) * a.kv_heads + kv_head) * a.dim;
       const int64_t values = a.tokens * a.kv_heads * a.dim;
-      store_row<C>((a.part ? a.part + 2 * split * values : a.dk) + at, dk, me.part * C, a.dim, 1.f, vec_out);
-      store_row<C>((a.part ? a.part + (2 * split + 1) * values : a.dv) + at, dv, me.part * C, a.dim, 1.f, vec_out);
+      store_row<C>((shares > 1 ? a.part + 2 * split * values : a.dk) + at, dk, me.part * C, a.dim, 1.f, vec_out);
+      store_row<C>((shares > 1 ? a.part + (2 * split + 1) * values : a.dv) + at, dv, me.part * C, a.dim, 1.f, vec_out);
     }
   }
   teardown(tmem);
 }
 
-// dk and dv from the splits' shares, in their order: `used` values each (the
-// tokens of the sequences) of `values`.
-__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part, float* __restrict__ dk,
-                                                   float* __restrict__ dv, int64_t used, int64_t values, int splits) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= used) return;
-  const float* p = part + blockIdx.y * values + i;
-  float s = p[0];
-  for (int k = 1; k < splits; ++k) s += p[2 * k * values];
-  (blockIdx.y ? dv : dk)[i] = s;
+// dk and dv of the tiles that have several shares, added in their order.
+// Grid: tiles x key/value heads, and eighths of a tile's rows.
+__global__ void __launch_bounds__(256) join_kernel(const AttentionArgs a) {
+  const int t = blockIdx.x / a.kv_heads, kv_head = blockIdx.x % a.kv_heads;
+  const int4 tile = a.tile[t];
+  const int shares = shares_of(a, (tile.y + kTileRows - 1) / kTileRows - tile.z);
+  if (shares == 1) return;
+  const int row0 = blockIdx.y * (kTileRows / 8), rows = min(kTileRows / 8, tile.y - tile.z * kTileRows - row0);
+  const int64_t values = a.tokens * a.kv_heads * a.dim;
+  for (int i = threadIdx.x; i < rows * a.dim; i += 256) {
+    const int64_t at = ((int64_t)(tile.x + tile.z * kTileRows + row0 + i / a.dim) * a.kv_heads + kv_head) * a.dim + i % a.dim;
+    float k = 0.f, v = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < shares; ++s) {
+      k += a.part[2 * s * values + at];
+      v += a.part[(2 * s + 1) * values + at];
+    }
+    a.dk[at] = k;
+    a.dv[at] = v;
+  }
 }
 
 // ------------------------------------------------------------ host side
@@ -1101,7 +1196,7 @@ lmpb_status split(const AttentionArgs& a, const Split& s, float* delta, cudaStre
   const unsigned planes = (a.grad ? 2 : 1) * a.heads + 2 * a.kv_heads;
   const bool vec = a.dim % 4 == 0 && aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.grad) &&
                    (!a.grad || aligned16(a.out));
-  split_kernel<DP><<<dim3((unsigned)a.tiles, planes), 256, 0, st>>>(a, s, delta, vec);
+  split_kernel<DP><<<dim3((unsigned)a.tiles, planes), 32 * split_warps<DP>(), 0, st>>>(a, s, delta, vec);
   return launch_status("attention (split)");
 }
 
@@ -1122,12 +1217,11 @@ lmpb_status backward(const AttentionArgs& a, const Split& s, float* delta, cudaS
   if (r == LMPB_OK && a.dk) {
     r = allow_smem(dkv_kernel<DP>, bytes);
     if (r != LMPB_OK) return r;
-    const bool vec = a.dim % 4 == 0 && (a.part ? aligned16(a.part) : aligned16(a.dk) && aligned16(a.dv));
+    const bool vec = a.dim % 4 == 0 && aligned16(a.dk) && aligned16(a.dv) && (!a.part || a.tokens * a.kv_heads * a.dim % 4 == 0);
     dkv_kernel<DP><<<(unsigned)(a.tiles * a.kv_heads * a.splits), Warps8::kThreads, bytes, st>>>(a, s, vec);
     r = launch_status("attention_backward (dk, dv)");
-    if (r == LMPB_OK && a.part) {
-      const int64_t row = (int64_t)a.kv_heads * a.dim, used = a.used * row;
-      join_kernel<<<dim3((unsigned)((used + 255) / 256), 2), 256, 0, st>>>(a.part, a.dk, a.dv, used, a.tokens * row, a.splits);
+    if (r == LMPB_OK && a.splits > 1) {
+      join_kernel<<<dim3((unsigned)(a.tiles * a.kv_heads), 8), 256, 0, st>>>(a);
       r = launch_status("attention_backward (join)");
     }
   }
@@ -1147,15 +1241,18 @@ bool attention_fits_sm100(const AttentionArgs& a) {
   return (int64_t)a.tiles * a.heads * kMaxSplits <= 0x7fffffff && 2 * a.heads + 2 * a.kv_heads <= 65535;
 }
 
-// Into how many shares the dk, dv work of a key tile is cut: until the
-// largest share is at most half of what an SM gets on average, so that the
-// last CTAs do not run alone (one key/value head, or a long sequence), but
-// not below 6 blocks, where starting a CTA costs as much as its work.
-int dkv_splits(const AttentionArgs& a) {
-  const int64_t group = a.heads / a.kv_heads;
+// Cuts the dk, dv work of the key tiles into shares of at most what an SM gets
+// on average, so that the last CTAs do not run alone (one key/value head, or a
+// long sequence), but not of under 6 blocks, where starting a CTA costs as
+// much as its work.  Where an SM gets few blocks, three quarters of that:
+// [1500, 31, 700, 1, 1865] x 16 heads (4) of 128: 427 us, 475 with whole
+// averages; [16384] x 8 (2): 5.14 ms and 4.91.
+void cut_dkv(AttentionArgs& a) {
+  const int64_t group = a.heads / a.kv_heads, most = a.longest_tiles * group;
   const double average = (double)a.pair_tiles * a.heads / sm_count();
-  const int64_t share = std::max<int64_t>(6, (int64_t)(average / 2));
-  return (int)std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, (a.longest_tiles * group + share - 1) / share));
+  a.share = (int)std::max<int64_t>(6, std::min<int64_t>(most, (int64_t)(average < 64 ? average * 0.75 : average)));
+  a.share = (int)std::max<int64_t>(a.share, (most + kMaxSplits - 1) / kMaxSplits);
+  a.splits = (int)((most + a.share - 1) / a.share);
 }
 
 lmpb_status attention_sm100(const AttentionArgs& args, const lmpb_sequences_s* seqs, cudaStream_t st) {
@@ -1182,7 +1279,7 @@ lmpb_status attention_sm100_backward(const AttentionArgs& args, const lmpb_seque
   float* delta = nullptr;
   void* ws = nullptr;
   const int dp = a.dim <= 64 ? 64 : 128;
-  a.splits = a.dk ? dkv_splits(a) : 1;
+  if (a.dk) cut_dkv(a);
   lmpb_status r = make_split(a, true, dp, s, &delta, &ws, st);
   if (r != LMPB_OK) return r;
   a.delta = delta;
