@@ -330,9 +330,14 @@ lmpb_status lmpb_sequences_release(lmpb_sequences handle);
  * [tokens, kv_heads, head_dim], lse [heads, tokens].  Token i of a sequence
  * sees that sequence's tokens j <= i; query head h reads key/value head
  * h / (heads / kv_heads):
- *   out = softmax(scale * q k^T) v,  lse = log(sum(exp(scale * q k^T)))
- * Tokens behind the last sequence get 0 (their lse is not written).
- * head_dim <= 128, heads a multiple of kv_heads, scale > 0. */
+ *   out = softmax(scale * q k^T) v,  lse = log2(sum(exp(scale * q k^T)))
+ * lse is what the backward wants back.  Tokens behind the last sequence get 0
+ * (their lse is not written) and are not read.  head_dim <= 128, heads a
+ * multiple of kv_heads, 0 < scale <= 2^64.  Products are fp32-accurate on the
+ * tensor cores; sequences and head groups whose values these cannot carry
+ * (infinities, NaN, scores past 2^14, rows over 2^18 apart within 128 tokens)
+ * are computed in plain fp32, several times slower.  A value that a row does
+ * not see never reaches it, whatever it is. */
 lmpb_status lmpb_attention(const float* q, const float* k, const float* v, float* out, float* lse, int64_t tokens,
                            int heads, int kv_heads, int head_dim, float scale, lmpb_sequences sequences,
                            void* stream);

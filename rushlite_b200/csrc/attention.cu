@@ -2,7 +2,7 @@
 // packed-sequence handle and the fp32 kernels.
 //
 //   S = scale * q k^T,  row i of a sequence sees its keys j <= i
-//   P = exp(S - lse),  lse = log(sum_j exp(S)),  o = P v
+//   P = exp(S) / sum_j exp(S),  o = P v;  kept for the backward: lse = log2(sum_j exp(S))
 //   backward, with delta_i = sum(grad_i * o_i):
 //   dP = grad v^T,  dS = P * (dP - delta),  dq = scale * dS k,  dk = scale * dS^T q,  dv = P^T grad
 //
@@ -34,7 +34,6 @@ constexpr int kB = 64;        // rows and columns of an S tile
 constexpr int kThreads = 256;  // 16 x 16, a 4 x 4 block of S each
 constexpr int kPad = 4;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 // Rows [row0, row0 + 64) of head `head` of a [*, heads, dim] tensor, zero
 // behind `n` rows and `dim` columns.
@@ -207,7 +206,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const AttentionArgs a
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const bool see = !diag || tx + 16 * j <= 4 * ty + i;
-          z[i][j] = see ? z[i][j] * c : -INFINITY;
+          z[i][j] = see ? __fmul_rn(z[i][j], c) : -INFINITY;  // rounded as in the backward, so that a weight of 1 is 1
           mx = fmaxf(mx, z[i][j]);  // drops a NaN: exp2f below keeps it in the row's sum
         }
         const float mn = fmaxf(m[i], over16(mx, true));
@@ -240,7 +239,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const AttentionArgs a
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k)
         if (column<DP>(tx, k) < a.dim) o[column<DP>(tx, k)] = __fdiv_rn(acc[i][k], l[i]);
-      if (tx == 0) a.lse[(int64_t)head * a.tokens + t.x + row] = (m[i] + log2f(l[i])) * kLn2;
+      if (tx == 0) a.lse[(int64_t)head * a.tokens + t.x + row] = m[i] + log2f(l[i]);
     }
   });
 }
@@ -276,6 +275,7 @@ __device__ __forceinline__ void probabilities(const AttentionArgs& a, BackwardSm
   float z[4][4], d[4][4];
   dot_tile<DP>(s.q, s.k, ty, tx, z);
   dot_tile<DP>(s.g, s.v, ty, tx, d);
+  const float c = a.scale * kLog2e;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = q0 + 4 * ty + i;
@@ -286,7 +286,7 @@ __device__ __forceinline__ void probabilities(const AttentionArgs& a, BackwardSm
     for (int j = 0; j < 4; ++j) {
       const int key = k0 + tx + 16 * j;
       const bool see = in && key <= row;
-      const float p = see ? exp2f((z[i][j] * a.scale - lse) * kLog2e) : 0.f;
+      const float p = see ? exp2f(__fsub_rn(__fmul_rn(z[i][j], c), lse)) : 0.f;
       if (kWithP) s.p[4 * ty + i][tx + 16 * j] = p;
       s.ds[4 * ty + i][tx + 16 * j] = see ? p * (d[i][j] - delta) : 0.f;
     }
@@ -420,7 +420,7 @@ lmpb_status check(const char* what, int64_t tokens, int heads, int kv_heads, int
   LMPB_CHECK_ARG(dim <= 128, w + ": head_dim " + std::to_string(dim) + " is over 128");
   LMPB_CHECK_ARG(heads % kv_heads == 0, w + ": heads must be a multiple of kv_heads");
   LMPB_CHECK_ARG(heads <= 65535, w + ": at most 65535 heads");
-  LMPB_CHECK_ARG(std::isfinite(scale) && scale > 0.f, w + ": scale must be finite and positive");
+  LMPB_CHECK_ARG(scale > 0.f && scale <= 0x1p64f, w + ": scale must be positive and at most 2^64");
   LMPB_CHECK_ARG(seqs->tokens <= tokens, w + ": the sequences have " + std::to_string(seqs->tokens) +
                                              " tokens, the tensors " + std::to_string(tokens));
   int dev = 0;

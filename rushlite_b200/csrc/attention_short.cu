@@ -22,7 +22,6 @@ namespace {
 constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kRows = kShortRows / kWarps;  // of a warp, at most
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -99,7 +98,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const AttentionArgs a
   const int lane = threadIdx.x & 31, col = 4 * lane;
   const float c = a.scale * kLog2e;
   for (int i = threadIdx.x >> 5; i < n; i += kWarps) {
-    const float s = lane <= i ? dot(q + i * pitch, k + lane * pitch, width) * c : -INFINITY;
+    const float s = lane <= i ? __fmul_rn(dot(q + i * pitch, k + lane * pitch, width), c) : -INFINITY;
     float m = s;
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -113,7 +112,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const AttentionArgs a
     }
     float* out = a.out + ((int64_t)(t.x + i) * a.heads + head) * a.dim;
     store4(out, make_float4(__fdiv_rn(o.x, l), __fdiv_rn(o.y, l), __fdiv_rn(o.z, l), __fdiv_rn(o.w, l)), col, a.dim);
-    if (lane == 0) a.lse[(int64_t)head * a.tokens + t.x + i] = (m + log2f(l)) * kLn2;
+    if (lane == 0) a.lse[(int64_t)head * a.tokens + t.x + i] = m + log2f(l);
   }
 }
 
@@ -141,7 +140,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const AttentionArgs 
       delta = warp_sum(delta);
       float w = 0.f, d = 0.f;
       if (lane <= i) {
-        w = exp2f((dot(q + i * pitch, k + lane * pitch, width) * a.scale - lse[i]) * kLog2e);
+        w = exp2f(__fsub_rn(__fmul_rn(dot(q + i * pitch, k + lane * pitch, width), a.scale * kLog2e), lse[i]));
         d = w * (dot(g + i * pitch, v + lane * pitch, width) - delta);
       }
       p[i * 33 + lane] = w;

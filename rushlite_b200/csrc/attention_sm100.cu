@@ -13,7 +13,8 @@
 // is drained into registers, where the running sums round to nearest.
 //
 // Tiles whose values that cannot carry (infinities, NaN, rows over 2^18 apart,
-// magnitudes outside [2^-60, 2^40]) are flagged by the split; the fp32 kernels
+// magnitudes outside [2^-60, 2^40], q or k so long that a score may pass 2^14,
+// where the rounding of lse moves a weight by 2^-10) are flagged by the split; the fp32 kernels
 // of attention.cu then redo the sequences and head groups that hold one.
 //
 // 1. Split pass: a CTA per tile and head plane writes the tile's hi and lo as
@@ -44,7 +45,6 @@ namespace lmpb {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kWeightBits = 14.f;  // weights enter the MMA times 2^14
 
 __device__ unsigned int g_attention_error = 0;
@@ -178,21 +178,20 @@ __global__ void __launch_bounds__(32 * split_warps<DP>(), 2048 / (64 * split_war
     for (int s = LANES / 2; s; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
     mx = fmaxf(mx, m);
     if (m > 0.f) mn = fminf(mn, m);
-    if (is_v || is_g) {
-      float q = v[i].x * v[i].x + v[i].y * v[i].y + v[i].z * v[i].z + v[i].w * v[i].w, d = 0.f;
-      const int r = warp * ROWS + i * RPS + sub;
-      if (is_g) {
-        const float4 u = load4(obase, r);
-        d = v[i].x * u.x + v[i].y * u.y + v[i].z * u.z + v[i].w * u.w;
-      }
+    float q = v[i].x * v[i].x + v[i].y * v[i].y + v[i].z * v[i].z + v[i].w * v[i].w, d = 0.f;
+    const int r = warp * ROWS + i * RPS + sub;
+    if (is_g) {
+      const float4 u = load4(obase, r);
+      d = v[i].x * u.x + v[i].y * u.y + v[i].z * u.z + v[i].w * u.w;
+    }
 #pragma unroll
-      for (int s = LANES / 2; s; s >>= 1) {
-        q += __shfl_xor_sync(0xffffffffu, q, s);
-        d += __shfl_xor_sync(0xffffffffu, d, s);
-      }
-      nrm = fmaxf(nrm, q);
+    for (int s = LANES / 2; s; s >>= 1) q += __shfl_xor_sync(0xffffffffu, q, s);
+    nrm = fmaxf(nrm, q);
+    if (is_g) {
+#pragma unroll
+      for (int s = LANES / 2; s; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
       dmx = fmaxf(dmx, fabsf(d));
-      if (is_g && lane % LANES == 0 && r < rows) delta[(int64_t)head * a.tokens + first + r] = d;
+      if (lane % LANES == 0 && r < rows) delta[(int64_t)head * a.tokens + first + r] = d;
     }
   }
   __shared__ float red[4][WARPS];
@@ -214,7 +213,8 @@ __global__ void __launch_bounds__(32 * split_warps<DP>(), 2048 / (64 * split_war
   }
   // a gradient's small rows only ever add to larger sums: no limit on their range
   const bool range = mx > 0.f && (mx > 0x1p40f || mx < 0x1p-60f || (!is_g && mn < mx * 0x1p-18f));
-  const bool flag = bads || range || !(dmx < INFINITY);
+  const bool far = !is_v && !is_g && !(nrm * a.scale <= 0x1p14f);  // so |q| |k| scale <= 2^14 of unflagged tiles
+  const bool flag = bads || range || far || !(dmx < INFINITY);
   const int e = flag ? 0 : row_exp(mx);
   const int64_t block = plane * a.tiles + t;
   if (threadIdx.x == 0) {
@@ -771,7 +771,7 @@ __global__ void __launch_bounds__(ForwardWarps<DP>::kThreads, 1) forward_kernel(
     if (row < tile.y && wait.ok) {
       const int64_t at = tile.x + row;
       store_row<C>(a.out + (at * a.heads + head) * a.dim, acc, me.part * C, a.dim, __frcp_rn(l), vec_out);
-      if (me.part == 0) a.lse[(int64_t)head * a.tokens + at] = (m + log2f(l) - kWeightBits) * kLn2;
+      if (me.part == 0) a.lse[(int64_t)head * a.tokens + at] = m + (log2f(l) - kWeightBits);
     }
   }
   teardown(tmem);
@@ -877,7 +877,7 @@ __global__ void __launch_bounds__(Warps8::kThreads, 1) dq_kernel(const Attention
     for (int i = 0; i < C; ++i) acc[i] = 0.f;
     const int row = tile.z * kTileRows + me.row;
     const int64_t at = (int64_t)head * a.tokens + tile.x + row;
-    const float lse = row < tile.y ? a.lse[at] * kLog2e : INFINITY;  // rows behind the sequence: no weight
+    const float lse = row < tile.y ? a.lse[at] : INFINITY;  // rows behind the sequence: no weight
     const float delta = row < tile.y ? a.delta[at] : 0.f;
     const int eq = sp.expo[qblock], eg = sp.expo[gblock];
     const float gnorm = sp.norm[gblock], dmax = sp.dmax[gblock];
@@ -1055,7 +1055,7 @@ __global__ void __launch_bounds__(WarpsKV<DP>::kThreads, 1) dkv_kernel(const Att
       const float c = ldexpf(a.scale * kLog2e, -(eq + ek));
       const DsScale ds = ds_scale(sp.norm[gb], vnorm, sp.dmax[gb], eg, ev, kWeightBits);
       float* st = stat + (i & 1) * 256;
-      st[tid] = tid < 128 ? kWeightBits - next * kLog2e : -next * ds.d;
+      st[tid] = tid < 128 ? kWeightBits - next : -next * ds.d;
       compute_sync<WARPS>();
       if (i + 1 < n) next = fetch(i + 1);
       const bool diag = (first + i) % per_head == 0;

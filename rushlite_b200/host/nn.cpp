@@ -220,7 +220,7 @@ Variable causal_attention(const Variable& q, const Variable& k, const Variable& 
   LMP_CHECK(s[2] >= 1 && s[2] <= 128, "causal_attention: head_dim must lie in [1, 128], got " << s[2]);
   LMP_CHECK((size_t)seqs->tokens <= s[0], "causal_attention: the sequences have " << seqs->tokens << " tokens, q has " << s[0]);
   const float sc = scale ? (float)*scale : (float)(1.0 / std::sqrt((double)s[2]));
-  LMP_CHECK(std::isfinite(sc) && sc > 0, "causal_attention: scale must be finite and positive");
+  LMP_CHECK(sc > 0 && sc <= 0x1p64f, "causal_attention: scale must be positive and at most 2^64");
   variable_list in{q, k, v};
   const bool rg = records(in);
   const float *pq = (const float*)ptr(q.data()), *pk = (const float*)ptr(k.data()), *pv = (const float*)ptr(v.data());

@@ -9,7 +9,8 @@ Tolerances, per element, from what is added (magnitudes M below):
   D * 2^-23 at most.  Plain fp32 loses at most D * 2^-24.  So a score is within
   E = (3 + D / 2) * 2^-22 * scale * |q| . |k|.
 * a weight P is exp of a difference of two such scores (or score and lse, whose
-  value is rounded to fp32): within 2 E + 2^-23 |lse| + 2^-21 of itself.
+  value is rounded to fp32, as a base-2 logarithm): within 2 E + 2^-23 |lse| +
+  2^-21 of itself.
 * what sums weights times values has the same 3 * 2^-22 a product, and at most
   2^-23 a product and block of additions that follow one another: L 2^-23.
 * the fp16 parts have a smallest step of 2^-24, so of an operand scaled to have
@@ -195,6 +196,62 @@ def test_what_a_row_does_not_see_does_not_reach_it(cuda, bad, dim):
     for name in ("dk", "dv"):
         _check(name, got[name][:, 0], tuple(a[:, 0] for a in ref[name]))
         _check(name, got[name][p + 1:, 1], tuple(a[p + 1:, 1] for a in ref[name]))
+
+
+@pytest.mark.parametrize("lengths", [[20, 7], [300, 9, 100]])
+@pytest.mark.parametrize("size", [2.0 ** 5, 2.0 ** 12, 2.0 ** 30])
+def test_scores_far_apart_pick_one_key(cuda, lengths, size):
+    """Keys that are powers-of-two multiples of each other's direction: every row's
+    largest score is its own key's and the next one at least size^2 / 4 below,
+    so its weight is 1 exactly and the gradients through the weights are 0."""
+    import rushlite_b200 as rsl
+
+    t, d = sum(lengths), 16
+    rng = np.random.default_rng(21)
+    v, g = (rng.standard_normal((t, 1, d)).astype(np.float32) for _ in range(2))
+    at = np.concatenate([np.arange(n) for n in lengths])
+    k = np.zeros((t, 1, d), np.float32)
+    k[:, 0, 0] = size * (1 + at / 4)  # exact
+    q = np.zeros((t, 1, d), np.float32)
+    q[:, 0, 0] = size
+    x = {"q": q, "k": k, "v": v, "g": g}
+    got = _run(rsl, {n: cuda.from_numpy(a) for n, a in x.items()}, lengths, 1.0)
+    tol = 2.0 ** -20 * np.abs(v).max()
+    assert (np.abs(got["out"] - v) <= tol).all()
+    assert (np.abs(got["dv"] - g) <= 2.0 ** -20 * np.abs(g).max()).all()
+    # dS = P (dP - delta) with P = 1: what is left is roundings of dP and delta, D products each
+    left = 2 * (d + 24) * 2.0 ** -22 * float((np.abs(g) @ np.abs(v).swapaxes(1, 2)).max()) * d
+    assert (np.abs(got["dq"][:, 0, 0]) <= left * np.abs(k).max() * max(lengths)).all()
+    assert np.isfinite(got["dk"]).all() and (np.abs(got["dk"]) <= left * size * max(lengths)).all()
+
+
+@pytest.mark.parametrize("size", [300.0, 3e4, 1e8])
+def test_large_values_stay_finite(cuda, size):
+    """Scores whose own rounding passes 1: weights are between 0 and 1 all the same."""
+    import rushlite_b200 as rsl
+
+    lengths = [260, 30]
+    x = _inputs(cuda, np.random.default_rng(22), (lengths, 2, 1, 64, 0))
+    x["q"] *= size
+    x["k"] *= size
+    got = _run(rsl, x, lengths)
+    assert all(np.isfinite(a).all() for a in got.values())
+    assert (np.abs(got["out"]) <= float(x["v"].abs().max()) * (1 + 2.0 ** -18)).all()
+
+
+def test_repeated_backward_of_one_graph(cuda):
+    import rushlite_b200 as rsl
+
+    lengths = [140, 20]
+    x = _inputs(cuda, np.random.default_rng(23), (lengths, 2, 1, 64, 0))
+    once = _run(rsl, x, lengths)
+    var = {n: rsl.Variable(x[n].numpy(), n != "g") for n in "qkvg"}
+    o = rsl.causal_attention(var["q"], var["k"], var["v"], rsl.Sequences(lengths))
+    for _ in range(3):
+        o.backward(var["g"])
+    for n in "qkv":
+        d = once["d" + n]
+        assert (var[n].grad.numpy() == (d + d) + d).all(), n
 
 
 def test_a_score_of_minus_infinity_has_no_weight(cuda):
@@ -408,7 +465,7 @@ def test_refusals(cuda):
            ((q, kv, rsl.ones([6, 2, 4]), s), "same shape"), ((q, rsl.ones([6, 3, 8]), rsl.ones([6, 3, 8]), s), "multiple"),
            ((q, rsl.ones([5, 2, 8]), rsl.ones([5, 2, 8]), s), "tokens"), ((q, kv, kv, rsl.Sequences([7])), "tokens"),
            ((rsl.ones([6, 2, 129]),) * 3 + (s,), "128"), ((q, kv, kv, s, 0.0), "scale"), ((q, kv, kv, s, -1.0), "scale"),
-           ((q, kv, kv, s, float("nan")), "scale"), ((q, kv, kv, s, float("inf")), "scale")]
+           ((q, kv, kv, s, float("nan")), "scale"), ((q, kv, kv, s, float("inf")), "scale"), ((q, kv, kv, s, 1e20), "scale")]
     for args, text in bad:
         with pytest.raises(RuntimeError, match=text):
             rsl.causal_attention(*args)
