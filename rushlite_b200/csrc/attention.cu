@@ -10,12 +10,15 @@
 // over the query heads of their group.
 //
 // The kernels here compute in plain fp32 (FFMA) with 64 x 64 tiles of S: a
-// running row maximum and sum forward; one kernel per result side backward
-// (dq by query tile; dk and dv by key tile, walking the group's heads in
-// order), so no sum depends on an order of atomics.  They serve sequences
-// too short to fill tensor-core tiles, and values that the fp16 split of the
-// tensor-core path cannot carry.  Masked positions never enter a sum, so a
-// NaN or infinity in a row that a query does not see does not reach it.
+// running row maximum and sum forward; backward dq by query tile, then dk and
+// dv by key tile, walking the group's heads in order, so no sum depends on an
+// order of atomics.  They serve the sequences and head groups whose values the
+// fp16 split of the tensor-core path cannot carry (one launch behind that
+// path's reads its flags and mostly ends there, 3 us), and more heads than its
+// grids hold.  Masked positions never enter a sum, so a NaN or infinity in a
+// row that a query does not see does not reach it.  Bound: FFMA and the
+// shared-memory loads that feed it, [16384] x 8 heads (2) of 128: forward
+// 27 ms, backward 56, against 1.15 and 4.9 on the tensor cores.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -164,7 +167,6 @@ __device__ __forceinline__ bool wanted(const AttentionArgs& a, const int4& t, in
 // of one half tile next to each other, those with the most work first.
 template <typename F>
 __device__ __forceinline__ void for_halves(const AttentionArgs& a, const int* order, int heads, F body) {
-  if (!any_flag(a)) return;
   const int64_t items = 2 * (int64_t)a.tiles * heads;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int64_t i = item / heads;
@@ -186,6 +188,7 @@ template <int DP>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const AttentionArgs a, bool vec) {
   extern __shared__ __align__(16) unsigned char raw[];
   ForwardSmem<DP>& s = *reinterpret_cast<ForwardSmem<DP>*>(raw);
+  if (!any_flag(a)) return;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const float c = a.scale * kLog2e;
   for_halves(a, a.by_queries, a.heads, [&](const int4& t, int q0, int head) {
@@ -294,9 +297,7 @@ __device__ __forceinline__ void probabilities(const AttentionArgs& a, BackwardSm
 }
 
 template <int DP>
-__global__ void __launch_bounds__(kThreads) dq_kernel(const AttentionArgs a, bool vec) {
-  extern __shared__ __align__(16) unsigned char raw[];
-  BackwardSmem<DP>& s = *reinterpret_cast<BackwardSmem<DP>*>(raw);
+__device__ __forceinline__ void dq_halves(const AttentionArgs& a, BackwardSmem<DP>& s, bool vec) {
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   for_halves(a, a.by_queries, a.heads, [&](const int4& t, int q0, int head) {
     const int kv_head = head / (a.heads / a.kv_heads);
@@ -326,9 +327,7 @@ __global__ void __launch_bounds__(kThreads) dq_kernel(const AttentionArgs a, boo
 }
 
 template <int DP>
-__global__ void __launch_bounds__(kThreads) dkv_kernel(const AttentionArgs a, bool vec) {
-  extern __shared__ __align__(16) unsigned char raw[];
-  BackwardSmem<DP>& s = *reinterpret_cast<BackwardSmem<DP>*>(raw);
+__device__ __forceinline__ void dkv_halves(const AttentionArgs& a, BackwardSmem<DP>& s, bool vec) {
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, group = a.heads / a.kv_heads;
   for_halves(a, a.by_keys, a.kv_heads, [&](const int4& t, int k0, int kv_head) {
     load_tile<DP>(s.k, a.k, t.x + k0, t.y - k0, a.kv_heads, kv_head, a.dim, vec);
@@ -364,6 +363,15 @@ __global__ void __launch_bounds__(kThreads) dkv_kernel(const AttentionArgs a, bo
   });
 }
 
+template <int DP>
+__global__ void __launch_bounds__(kThreads) backward_kernel(const AttentionArgs a, bool vec) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  BackwardSmem<DP>& s = *reinterpret_cast<BackwardSmem<DP>*>(raw);
+  if (!any_flag(a)) return;
+  if (a.dq) dq_halves<DP>(a, s, vec);
+  if (a.dk) dkv_halves<DP>(a, s, vec);
+}
+
 // A CTA per half tile and head; where flags pick the few that are wanted, no
 // more than fill the GPU once, since reading the flags is then all most do.
 template <typename K>
@@ -389,20 +397,11 @@ lmpb_status attention_simt(const AttentionArgs& a, cudaStream_t st) {
 
 lmpb_status attention_simt_backward(const AttentionArgs& a, cudaStream_t st) {
   const bool vec = a.dim % 4 == 0 && aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.grad);
-  lmpb_status s = LMPB_OK;
-  if (a.dq) {
-    const char* what = "attention_backward (dq)";
-    s = a.dim <= 32   ? launch(dq_kernel<32>, sizeof(BackwardSmem<32>), a.heads, a, vec, what, st)
-        : a.dim <= 64 ? launch(dq_kernel<64>, sizeof(BackwardSmem<64>), a.heads, a, vec, what, st)
-                      : launch(dq_kernel<128>, sizeof(BackwardSmem<128>), a.heads, a, vec, what, st);
-  }
-  if (s == LMPB_OK && a.dk) {
-    const char* what = "attention_backward (dk, dv)";
-    s = a.dim <= 32   ? launch(dkv_kernel<32>, sizeof(BackwardSmem<32>), a.kv_heads, a, vec, what, st)
-        : a.dim <= 64 ? launch(dkv_kernel<64>, sizeof(BackwardSmem<64>), a.kv_heads, a, vec, what, st)
-                      : launch(dkv_kernel<128>, sizeof(BackwardSmem<128>), a.kv_heads, a, vec, what, st);
-  }
-  return s;
+  const char* what = "attention_backward";
+  const int heads = a.dq ? a.heads : a.kv_heads;
+  if (a.dim <= 32) return launch(backward_kernel<32>, sizeof(BackwardSmem<32>), heads, a, vec, what, st);
+  if (a.dim <= 64) return launch(backward_kernel<64>, sizeof(BackwardSmem<64>), heads, a, vec, what, st);
+  return launch(backward_kernel<128>, sizeof(BackwardSmem<128>), heads, a, vec, what, st);
 }
 
 void use_tiles(AttentionArgs& a, const lmpb_sequences_s* seqs, const lmpb_sequences_s::Tiles& t) {

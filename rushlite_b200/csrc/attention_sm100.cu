@@ -496,15 +496,13 @@ struct Warps {
   static __device__ __forceinline__ void many() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(HIGH)); }
 };
 using Warps8 = Warps<8, 168, 88, 208>;
-template <int DP>
-using WarpsKV = std::conditional_t<DP == 64, Warps<8, 168, 104, 200>, Warps8>;
 using Warps16 = Warps<16, 96, 64, 104>;
-// Forward with DP = 64, where the weights' arithmetic weighs as much as the
-// MMAs: 16 warps (0.390 ms for [8192] x 16 heads; 8 warps 0.44, two
-// pipelines of 8 warps that take the key blocks in turn 0.42).  With DP = 128,
-// where the MMAs outweigh it, 8 warps of twice the registers.
+// With DP = 64, where the weights' arithmetic weighs as much as the MMAs, 16
+// warps ([8192] x 16 heads: forward 0.390 ms, backward 1.55; 8 warps 0.44 and
+// 1.63; a forward of two pipelines of 8 that take the key blocks in turn 0.42).
+// With DP = 128, where the MMAs outweigh it, 8 warps of twice the registers.
 template <int DP>
-using ForwardWarps = std::conditional_t<DP == 64, Warps16, Warps8>;
+using WarpsOf = std::conditional_t<DP == 64, Warps16, Warps8>;
 
 template <int DP, int RESIDENT, int RING, int SCRATCH>
 struct Layout {
@@ -520,7 +518,7 @@ constexpr int forward_ring() { return DP == 64 ? 8 : 5; }
 template <int DP>
 constexpr int backward_ring() { return DP == 64 ? 8 : 3; }
 template <int DP>
-using ForwardLayout = Layout<DP, 1, forward_ring<DP>(), 2 * ForwardWarps<DP>::kParts * 128 * 4>;
+using ForwardLayout = Layout<DP, 1, forward_ring<DP>(), 2 * WarpsOf<DP>::kParts * 128 * 4>;
 template <int DP>
 using BackwardLayout = Layout<DP, 2, backward_ring<DP>(), 2048>;
 
@@ -626,10 +624,10 @@ __device__ __forceinline__ void store_row(float* p, const float (&acc)[C], int c
 // turn block j's scores into weights, the MMAs of block j + 1's scores run.
 
 template <int DP>
-__global__ void __launch_bounds__(ForwardWarps<DP>::kThreads, 1) forward_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
+__global__ void __launch_bounds__(WarpsOf<DP>::kThreads, 1) forward_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
   extern __shared__ __align__(1024) unsigned char smem[];
   using L = ForwardLayout<DP>;
-  using W = ForwardWarps<DP>;
+  using W = WarpsOf<DP>;
   constexpr int WARPS = W::kWarps, PARTS = W::kParts, COLS = W::kCols;
   constexpr int RING = forward_ring<DP>();
   const uint32_t base = smem_u32(smem), bars = base + L::kBarsAt;
@@ -801,10 +799,10 @@ __device__ __forceinline__ DsScale ds_scale(float gnorm, float vnorm, float dmax
 // with k in [384, 384 + DP).  Block j + 1's scores run while the computing
 // warps turn block j's scores and dP into dS.
 template <int DP>
-__global__ void __launch_bounds__(Warps8::kThreads, 1) dq_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
+__global__ void __launch_bounds__(WarpsOf<DP>::kThreads, 1) dq_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
   extern __shared__ __align__(1024) unsigned char smem[];
   using L = BackwardLayout<DP>;
-  using W = Warps8;
+  using W = WarpsOf<DP>;
   constexpr int WARPS = W::kWarps, PARTS = W::kParts, COLS = W::kCols;
   constexpr int RING = backward_ring<DP>();
   const uint32_t base = smem_u32(smem), bars = base + L::kBarsAt;
@@ -952,10 +950,10 @@ __device__ __forceinline__ int shares_of(const AttentionArgs& a, int per_head) {
 }
 
 template <int DP>
-__global__ void __launch_bounds__(WarpsKV<DP>::kThreads, 1) dkv_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
+__global__ void __launch_bounds__(WarpsOf<DP>::kThreads, 1) dkv_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
   extern __shared__ __align__(1024) unsigned char smem[];
   using L = BackwardLayout<DP>;
-  using W = WarpsKV<DP>;
+  using W = WarpsOf<DP>;
   constexpr int WARPS = W::kWarps, PARTS = W::kParts, COLS = W::kCols;
   constexpr int RING = backward_ring<DP>();
   const uint32_t base = smem_u32(smem), bars = base + L::kBarsAt;
@@ -980,10 +978,15 @@ __global__ void __launch_bounds__(WarpsKV<DP>::kThreads, 1) dkv_kernel(const Att
   const int64_t kblock = (int64_t)(a.heads + kv_head) * a.tiles + t;
   const int64_t vblock = kblock + (int64_t)a.kv_heads * a.tiles;
   const int64_t gplanes = (int64_t)(a.heads + 2 * a.kv_heads) * a.tiles;
-  // block i of this share: query head and tile, as a block index of the q planes
-  auto qblock = [&](int i) {
-    return (int64_t)(kv_head * group + (first + i) / per_head) * a.tiles + t + (first + i) % per_head;
+  // the blocks of this share: query head and tile, counted from the diagonal
+  struct Walk {
+    int head, x, per_head;
+    __device__ __forceinline__ void next() {
+      if (++x == per_head) x = 0, ++head;
+    }
   };
+  const Walk begin{kv_head * group + first / per_head, first % per_head, per_head};
+  const auto qblock = [&](const Walk& w) { return (int64_t)w.head * a.tiles + t + w.x; };  // of the q planes
   const int warp = threadIdx.x >> 5;
   constexpr int64_t BB = block_bytes<DP>();
   if (warp < 4) {
@@ -994,8 +997,9 @@ __global__ void __launch_bounds__(WarpsKV<DP>::kThreads, 1) dkv_kernel(const Att
       mbar_expect_tx(resident, 2 * BB);
       bulk_load(base, sp.blocks + kblock * BB, BB, resident);
       bulk_load(base + BB, sp.blocks + vblock * BB, BB, resident);
-      for (int i = 0; i < n; ++i) {
-        const unsigned char *q = sp.blocks + qblock(i) * BB, *g = q + gplanes * BB;
+      Walk at = begin;
+      for (int i = 0; i < n; ++i, at.next()) {
+        const unsigned char *q = sp.blocks + qblock(at) * BB, *g = q + gplanes * BB;
         feed(ring, wait, q);
         feed(ring, wait, g);
         feed(ring, wait, g);
@@ -1043,22 +1047,23 @@ __global__ void __launch_bounds__(WarpsKV<DP>::kThreads, 1) dkv_kernel(const Att
     // one value of the next block's row statistics a thread: lse (first half) or delta
     const int tid = threadIdx.x - 128;
     const float* source = tid < 128 ? a.lse : a.delta;
-    auto fetch = [&](int i) {
-      const int r = (tile.z + (first + i) % per_head) * kTileRows + (tid & 127);
-      const int64_t at = (int64_t)(kv_head * group + (first + i) / per_head) * a.tokens + tile.x + r;
-      return r < tile.y ? __ldg(source + at) : tid < 128 ? INFINITY : 0.f;
+    const auto fetch = [&](const Walk& w) {
+      const int r = (tile.z + w.x) * kTileRows + (tid & 127);
+      return tid < 256 && r < tile.y ? __ldg(source + (int64_t)w.head * a.tokens + tile.x + r) : tid < 128 ? INFINITY : 0.f;
     };
-    float next = fetch(0);
-    for (int i = 0; i < n; ++i) {
-      const int64_t qb = qblock(i), gb = qb + gplanes;
+    Walk at = begin, ahead = begin;
+    float next = fetch(ahead);
+    for (int i = 0; i < n; ++i, at.next()) {
+      const int64_t qb = qblock(at), gb = qb + gplanes;
       const int eq = sp.expo[qb], eg = sp.expo[gb];
       const float c = ldexpf(a.scale * kLog2e, -(eq + ek));
       const DsScale ds = ds_scale(sp.norm[gb], vnorm, sp.dmax[gb], eg, ev, kWeightBits);
       float* st = stat + (i & 1) * 256;
-      st[tid] = tid < 128 ? kWeightBits - next : -next * ds.d;
+      if (tid < 256) st[tid] = tid < 128 ? kWeightBits - next : -next * ds.d;
       compute_sync<WARPS>();
-      if (i + 1 < n) next = fetch(i + 1);
-      const bool diag = (first + i) % per_head == 0;
+      ahead.next();
+      if (i + 1 < n) next = fetch(ahead);
+      const bool diag = at.x == 0;
       const float4* bias = reinterpret_cast<const float4*>(st + me.part * COLS);
       const float4* dd = reinterpret_cast<const float4*>(st + 128 + me.part * COLS);
       warp_wait(wait, sfull, i & 1);
@@ -1131,10 +1136,10 @@ __global__ void __launch_bounds__(WarpsKV<DP>::kThreads, 1) dkv_kernel(const Att
     drain<C, false>(oown + 128, dk, 1.f, fk);
     const int row = tile.z * kTileRows + me.row;
     if (row < tile.y && wait.ok) {
-      const int64_t at = ((int64_t)(tile.x + row) * a.kv_heads + kv_head) * a.dim;
+      const int64_t to = ((int64_t)(tile.x + row) * a.kv_heads + kv_head) * a.dim;
       const int64_t values = a.tokens * a.kv_heads * a.dim;
-      store_row<C>((shares > 1 ? a.part + 2 * split * values : a.dk) + at, dk, me.part * C, a.dim, 1.f, vec_out);
-      store_row<C>((shares > 1 ? a.part + (2 * split + 1) * values : a.dv) + at, dv, me.part * C, a.dim, 1.f, vec_out);
+      store_row<C>((shares > 1 ? a.part + 2 * split * values : a.dk) + to, dk, me.part * C, a.dim, 1.f, vec_out);
+      store_row<C>((shares > 1 ? a.part + (2 * split + 1) * values : a.dv) + to, dv, me.part * C, a.dim, 1.f, vec_out);
     }
   }
   teardown(tmem);
@@ -1206,7 +1211,7 @@ lmpb_status forward(const AttentionArgs& a, const Split& s, cudaStream_t st) {
   if (r == LMPB_OK) r = allow_smem(forward_kernel<DP>, ForwardLayout<DP>::kBytes);
   if (r != LMPB_OK) return r;
   const bool vec = a.dim % 4 == 0 && aligned16(a.out);
-  forward_kernel<DP><<<(unsigned)(a.tiles * a.heads), ForwardWarps<DP>::kThreads, ForwardLayout<DP>::kBytes, st>>>(a, s, vec);
+  forward_kernel<DP><<<(unsigned)(a.tiles * a.heads), WarpsOf<DP>::kThreads, ForwardLayout<DP>::kBytes, st>>>(a, s, vec);
   return launch_status("attention");
 }
 
@@ -1218,7 +1223,7 @@ lmpb_status backward(const AttentionArgs& a, const Split& s, float* delta, cudaS
     r = allow_smem(dkv_kernel<DP>, bytes);
     if (r != LMPB_OK) return r;
     const bool vec = a.dim % 4 == 0 && aligned16(a.dk) && aligned16(a.dv) && (!a.part || a.tokens * a.kv_heads * a.dim % 4 == 0);
-    dkv_kernel<DP><<<(unsigned)(a.tiles * a.kv_heads * a.splits), Warps8::kThreads, bytes, st>>>(a, s, vec);
+    dkv_kernel<DP><<<(unsigned)(a.tiles * a.kv_heads * a.splits), WarpsOf<DP>::kThreads, bytes, st>>>(a, s, vec);
     r = launch_status("attention_backward (dk, dv)");
     if (r == LMPB_OK && a.splits > 1) {
       join_kernel<<<dim3((unsigned)(a.tiles * a.kv_heads), 8), 256, 0, st>>>(a);
@@ -1229,7 +1234,7 @@ lmpb_status backward(const AttentionArgs& a, const Split& s, float* delta, cudaS
     r = allow_smem(dq_kernel<DP>, bytes);
     if (r != LMPB_OK) return r;
     const bool vec = a.dim % 4 == 0 && aligned16(a.dq);
-    dq_kernel<DP><<<(unsigned)(a.tiles * a.heads), Warps8::kThreads, bytes, st>>>(a, s, vec);
+    dq_kernel<DP><<<(unsigned)(a.tiles * a.heads), WarpsOf<DP>::kThreads, bytes, st>>>(a, s, vec);
     r = launch_status("attention_backward (dq)");
   }
   return r;
