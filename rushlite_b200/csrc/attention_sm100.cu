@@ -799,7 +799,7 @@ __device__ __forceinline__ DsScale ds_scale(float gnorm, float vnorm, float dmax
 // with k in [384, 384 + DP).  Block j + 1's scores run while the computing
 // warps turn block j's scores and dP into dS.
 template <int DP>
-__global__ void __launch_bounds__(WarpsOf<DP>::kThreads, 1) dq_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
+__device__ __forceinline__ void dq_tile(const AttentionArgs& a, const Split& sp, int cta, bool vec_out) {
   extern __shared__ __align__(1024) unsigned char smem[];
   using L = BackwardLayout<DP>;
   using W = WarpsOf<DP>;
@@ -813,7 +813,7 @@ __global__ void __launch_bounds__(WarpsOf<DP>::kThreads, 1) dq_kernel(const Atte
   const uint32_t resident = bars + 16 * RING, spfull = resident + 8, dsfull = resident + 16, ofull = resident + 24,
                  oempty = resident + 32, done = resident + 40;
   constexpr uint32_t tmem = 0;  // all of it was allocated
-  const int order = blockIdx.x / a.heads, head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
+  const int order = cta / a.heads, head = cta % a.heads, kv_head = head / (a.heads / a.kv_heads);
   const int t = a.by_queries[order];
   const int4 tile = a.tile[t];
   const int n = tile.z + 1;  // key blocks
@@ -950,7 +950,7 @@ __device__ __forceinline__ int shares_of(const AttentionArgs& a, int per_head) {
 }
 
 template <int DP>
-__global__ void __launch_bounds__(WarpsOf<DP>::kThreads, 1) dkv_kernel(const AttentionArgs a, const Split sp, bool vec_out) {
+__device__ __forceinline__ void dkv_tile(const AttentionArgs& a, const Split& sp, int cta, bool vec_out) {
   extern __shared__ __align__(1024) unsigned char smem[];
   using L = BackwardLayout<DP>;
   using W = WarpsOf<DP>;
@@ -959,8 +959,8 @@ __global__ void __launch_bounds__(WarpsOf<DP>::kThreads, 1) dkv_kernel(const Att
   const uint32_t base = smem_u32(smem), bars = base + L::kBarsAt;
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + L::kBarsAt + kBars * 8);
   float* stat = reinterpret_cast<float*>(smem + L::kScratch);  // [2][2][128]: weight offset, -scaled delta
-  const int per_order = a.kv_heads * a.splits, order = blockIdx.x / per_order, kv_head = blockIdx.x % per_order / a.splits;
-  const int split = blockIdx.x % a.splits, group = a.heads / a.kv_heads;
+  const int per_order = a.kv_heads * a.splits, order = cta / per_order, kv_head = cta % per_order / a.splits;
+  const int split = cta % a.splits, group = a.heads / a.kv_heads;
   const int t = a.by_keys[order];
   const int4 tile = a.tile[t];
   const int per_head = (tile.y + kTileRows - 1) / kTileRows - tile.z;  // query blocks of a head
@@ -1145,6 +1145,14 @@ __global__ void __launch_bounds__(WarpsOf<DP>::kThreads, 1) dkv_kernel(const Att
   teardown(tmem);
 }
 
+// One launch for both, dk and dv's larger CTAs first.
+template <int DP>
+__global__ void __launch_bounds__(WarpsOf<DP>::kThreads, 1)
+    backward_kernel(const AttentionArgs a, const Split sp, int dkv_ctas, bool vec_dkv, bool vec_dq) {
+  if ((int)blockIdx.x < dkv_ctas) dkv_tile<DP>(a, sp, blockIdx.x, vec_dkv);
+  else dq_tile<DP>(a, sp, blockIdx.x - dkv_ctas, vec_dq);
+}
+
 // dk and dv of the tiles that have several shares, added in their order.
 // Grid: tiles x key/value heads, and eighths of a tile's rows.
 __global__ void __launch_bounds__(256) join_kernel(const AttentionArgs a) {
@@ -1219,23 +1227,16 @@ template <int DP>
 lmpb_status backward(const AttentionArgs& a, const Split& s, float* delta, cudaStream_t st) {
   lmpb_status r = split<DP>(a, s, delta, st);
   constexpr int bytes = BackwardLayout<DP>::kBytes;
-  if (r == LMPB_OK && a.dk) {
-    r = allow_smem(dkv_kernel<DP>, bytes);
-    if (r != LMPB_OK) return r;
-    const bool vec = a.dim % 4 == 0 && aligned16(a.dk) && aligned16(a.dv) && (!a.part || a.tokens * a.kv_heads * a.dim % 4 == 0);
-    dkv_kernel<DP><<<(unsigned)(a.tiles * a.kv_heads * a.splits), WarpsOf<DP>::kThreads, bytes, st>>>(a, s, vec);
-    r = launch_status("attention_backward (dk, dv)");
-    if (r == LMPB_OK && a.splits > 1) {
-      join_kernel<<<dim3((unsigned)(a.tiles * a.kv_heads), 8), 256, 0, st>>>(a);
-      r = launch_status("attention_backward (join)");
-    }
-  }
-  if (r == LMPB_OK && a.dq) {
-    r = allow_smem(dq_kernel<DP>, bytes);
-    if (r != LMPB_OK) return r;
-    const bool vec = a.dim % 4 == 0 && aligned16(a.dq);
-    dq_kernel<DP><<<(unsigned)(a.tiles * a.heads), WarpsOf<DP>::kThreads, bytes, st>>>(a, s, vec);
-    r = launch_status("attention_backward (dq)");
+  if (r == LMPB_OK) r = allow_smem(backward_kernel<DP>, bytes);
+  if (r != LMPB_OK) return r;
+  const int dkv = a.dk ? a.tiles * a.kv_heads * a.splits : 0, dq = a.dq ? a.tiles * a.heads : 0;
+  const bool vec_dkv = a.dim % 4 == 0 && aligned16(a.dk) && aligned16(a.dv) && (!a.part || a.tokens * a.kv_heads * a.dim % 4 == 0);
+  const bool vec_dq = a.dim % 4 == 0 && aligned16(a.dq);
+  backward_kernel<DP><<<(unsigned)(dkv + dq), WarpsOf<DP>::kThreads, bytes, st>>>(a, s, dkv, vec_dkv, vec_dq);
+  r = launch_status("attention_backward");
+  if (r == LMPB_OK && dkv > 0 && a.splits > 1) {
+    join_kernel<<<dim3((unsigned)(a.tiles * a.kv_heads), 8), 256, 0, st>>>(a);
+    r = launch_status("attention_backward (join)");
   }
   return r;
 }
@@ -1243,7 +1244,7 @@ lmpb_status backward(const AttentionArgs& a, const Split& s, float* delta, cudaS
 }  // namespace
 
 bool attention_fits_sm100(const AttentionArgs& a) {
-  return (int64_t)a.tiles * a.heads * kMaxSplits <= 0x7fffffff && 2 * a.heads + 2 * a.kv_heads <= 65535;
+  return (int64_t)a.tiles * a.heads * (kMaxSplits + 1) <= 0x7fffffff && 2 * a.heads + 2 * a.kv_heads <= 65535;
 }
 
 // Cuts the dk, dv work of the key tiles into shares of at most what an SM gets

@@ -5,8 +5,8 @@ The tensor-core kernels hand registers from their feeding warps to their
 computing ones (setmaxnreg), which waits for ever if the launch does not hold
 what is asked for: the launch's registers have to be exactly the 168 (12
 warps) or 96 (20 warps) that the split is computed from.  All of L1 is shared
-memory there, so a spill goes to L2: none in the forward and dq, and at most a
-few words in dk/dv with 64 columns (its loop keeps two sums and both operands' addresses)."""
+memory there, so a spill goes to L2: none, but for a few words in the backward
+with 64 columns (the loop of dk and dv keeps two sums and both operands' addresses)."""
 from __future__ import annotations
 
 import os
@@ -32,7 +32,7 @@ def test_attention_kernels_register_budget(tmp_path):
     for line in r.stderr.splitlines():
         m = re.search(r"Compiling entry function '(\S+)'", line)
         if m:
-            k = re.search(r"(forward|dq|dkv)_kernelILi(\d+)E", m.group(1))
+            k = re.search(r"(forward|backward)_kernelILi(\d+)E", m.group(1))
             current = found.setdefault((k.group(1), int(k.group(2))), {}) if k else None
         if current is None:
             continue
@@ -42,7 +42,7 @@ def test_attention_kernels_register_budget(tmp_path):
         m = re.search(r"Used (\d+) registers", line)
         if m:
             current["regs"] = int(m.group(1))
-    assert sorted(found) == [(k, d) for k in ("dkv", "dq", "forward") for d in (64, 128)]
+    assert sorted(found) == [(k, d) for k in ("backward", "forward") for d in (64, 128)]
     for (kind, dim), v in found.items():
         assert v["regs"] == (96 if dim == 64 else 168), (kind, dim, v)
-        assert v["spill"] <= (128 if (kind, dim) == ("dkv", 64) else 0), (kind, dim, v)
+        assert v["spill"] <= (128 if (kind, dim) == ("backward", 64) else 0), (kind, dim, v)
