@@ -709,7 +709,7 @@ __global__ void __launch_bounds__(WarpsOf<DP>::kThreads, 1) forward_kernel(const
       warp_wait(wait, sfull + 8 * (j & 1), phase2(j));
       // scores are read twice, for the maximum and for the weights: kept, they
       // would spill, and with all of L1 given to shared memory that costs more
-            float mx = -INFINITY;
+      float mx = -INFINITY;
 #pragma unroll 2
       for (int k = 0; k < COLS; k += 16) {
         uint32_t r[16];
@@ -1247,16 +1247,18 @@ bool attention_fits_sm100(const AttentionArgs& a) {
   return (int64_t)a.tiles * a.heads * (kMaxSplits + 1) <= 0x7fffffff && 2 * a.heads + 2 * a.kv_heads <= 65535;
 }
 
-// Cuts the dk, dv work of the key tiles into shares of at most what an SM gets
-// on average, so that the last CTAs do not run alone (one key/value head, or a
-// long sequence), but not of under 6 blocks, where starting a CTA costs as
-// much as its work.  Where an SM gets few blocks, three quarters of that:
-// [1500, 31, 700, 1, 1865] x 16 heads (4) of 128: 427 us, 475 with whole
-// averages; [16384] x 8 (2): 5.14 ms and 4.91.
+// Cuts the dk, dv work of the key tiles into shares, so that no SM ends long
+// after the others (one key/value head, or a long sequence): at most one and a
+// half times what an SM gets on average, as dq's CTAs fill what is left
+// ([1500, 31, 700, 1, 1865] x 16 heads (4) of 128: half the average 461 us, the
+// average 420, one and a half 421, two and a half 561), but not under 8 blocks,
+// where starting a CTA and joining the shares cost as much ([600, 300, 900] x
+// 12 (1) of 128: 6 blocks 138 us, 8 to 12 129, 16 139; [777, 1234] x 6 (1) of
+// 80: 87, 88 to 102, 111).
 void cut_dkv(AttentionArgs& a) {
   const int64_t group = a.heads / a.kv_heads, most = a.longest_tiles * group;
   const double average = (double)a.pair_tiles * a.heads / sm_count();
-  a.share = (int)std::max<int64_t>(6, std::min<int64_t>(most, (int64_t)(average < 64 ? average * 0.75 : average)));
+  a.share = (int)std::max<int64_t>(8, std::min<int64_t>(most, (int64_t)(1.5 * average)));
   a.share = (int)std::max<int64_t>(a.share, (most + kMaxSplits - 1) / kMaxSplits);
   a.splits = (int)((most + a.share - 1) / a.share);
 }
