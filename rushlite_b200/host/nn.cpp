@@ -70,6 +70,7 @@ Tensor empty(const std::vector<size_t>& shape, DataType dt) {
 }
 
 void* ptr(const Tensor& t) { return t.impl()->data(); }
+void* row_of(const Tensor& t, size_t i) { return static_cast<char*>(ptr(t)) + i * (t.impl()->nbytes() / t.shape()[0]); }
 
 bool on_cuda(const Variable& v) { return v.data().device() == DeviceType::CUDA; }
 
@@ -123,7 +124,7 @@ Variable output(const Tensor& t, bool rg, std::shared_ptr<Function> fn, variable
 }
 
 struct LayerNormBackward : Function {
-  Tensor mean, rstd;
+  Tensor stats;  // [2, rows]: mean, 1 / deviation
   bool has_weight = false, has_bias = false;
   void apply(const Variable& out) override {
     variable_list& in = *saved_inputs;
@@ -134,8 +135,8 @@ struct LayerNormBackward : Function {
     const void* pw = has_weight ? ptr(in[1].data()) : nullptr;
     GradOut dx(&in[0]), dw(has_weight ? &in[1] : nullptr), db(has_bias ? &in.back() : nullptr);
     const int64_t f = (int64_t)x.shape().back();
-    LMPB_OK_OR_THROW(lmpb_layer_norm_backward((int)x.type(), px, pw, ptr(mean), ptr(rstd), pg, (int64_t)x.numel() / f,
-                                              f, dx.get(), dw.get(), db.get(), tensor::current_stream()));
+    LMPB_OK_OR_THROW(lmpb_layer_norm_backward((int)x.type(), px, pw, ptr(stats), row_of(stats, 1), pg,
+                                              (int64_t)x.numel() / f, f, dx.get(), dw.get(), db.get(), tensor::current_stream()));
     dx.add(), dw.add(), db.add();
   }
 };
@@ -193,13 +194,12 @@ Variable layer_norm(const Variable& x, const Variable* weight, const Variable* b
   const size_t rows = y.numel() / s.back();
   auto fn = std::make_shared<LayerNormBackward>();
   if (rg) {
-    fn->mean = empty({rows}, dt);
-    fn->rstd = empty({rows}, dt);
+    fn->stats = empty({2, rows}, dt);
     fn->has_weight = weight != nullptr;
     fn->has_bias = bias != nullptr;
   }
   LMPB_OK_OR_THROW(lmpb_layer_norm((int)dt, px, pw, pb, (int64_t)rows, (int64_t)s.back(), eps, ptr(y),
-                                   rg ? ptr(fn->mean) : nullptr, rg ? ptr(fn->rstd) : nullptr, tensor::current_stream()));
+                                   rg ? ptr(fn->stats) : nullptr, rg ? row_of(fn->stats, 1) : nullptr, tensor::current_stream()));
   return output(y, rg, fn, std::move(in));
 }
 
