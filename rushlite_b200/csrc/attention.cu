@@ -188,6 +188,7 @@ template <int DP>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const AttentionArgs a, bool vec) {
   extern __shared__ __align__(16) unsigned char raw[];
   ForwardSmem<DP>& s = *reinterpret_cast<ForwardSmem<DP>*>(raw);
+  after_previous();
   if (!any_flag(a)) return;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const float c = a.scale * kLog2e;
@@ -367,6 +368,7 @@ template <int DP>
 __global__ void __launch_bounds__(kThreads) backward_kernel(const AttentionArgs a, bool vec) {
   extern __shared__ __align__(16) unsigned char raw[];
   BackwardSmem<DP>& s = *reinterpret_cast<BackwardSmem<DP>*>(raw);
+  after_previous();
   if (!any_flag(a)) return;
   if (a.dq) dq_halves<DP>(a, s, vec);
   if (a.dk) dkv_halves<DP>(a, s, vec);
@@ -380,6 +382,7 @@ lmpb_status launch(K kernel, size_t smem, int heads, const AttentionArgs& a, boo
   LMPB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   const int64_t items = 2 * (int64_t)a.tiles * heads;
   const int64_t grid = std::min<int64_t>(items, a.flags ? sm_count() : INT32_MAX);
+  if (a.flags) return launch_early(what, kernel, dim3((unsigned)grid), kThreads, (int)smem, st, a, vec);
   kernel<<<(unsigned)grid, kThreads, smem, st>>>(a, vec);
   return launch_status(what);
 }

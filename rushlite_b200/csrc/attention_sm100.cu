@@ -139,6 +139,7 @@ template <int DP>
 __global__ void __launch_bounds__(32 * split_warps<DP>(), 2048 / (64 * split_warps<DP>())) split_kernel(const AttentionArgs a, const Split o, float* __restrict__ delta, bool vec) {
   constexpr int WARPS = split_warps<DP>(), ROWS = 128 / WARPS;  // of a warp
   constexpr int RPS = 128 / DP, STEPS = ROWS / RPS, LANES = 32 / RPS;  // rows a step, steps, lanes a row
+  let_next_start();
   const int64_t plane = blockIdx.y;
   const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int4 tile = a.tile[t];
@@ -522,12 +523,13 @@ using ForwardLayout = Layout<DP, 1, forward_ring<DP>(), 2 * WarpsOf<DP>::kParts 
 template <int DP>
 using BackwardLayout = Layout<DP, 2, backward_ring<DP>(), 2048>;
 
-// Sets up the barriers and all of TMEM; every thread calls it.  False (for
+// Sets up the barriers and all of TMEM, then waits for the kernel ahead; every thread calls it.  False (for
 // all) when the shared memory does not start on a swizzle atom.
 __device__ __forceinline__ bool setup(unsigned char* smem, uint32_t bars, uint32_t* slot, int ring, const int* counts, int n) {
   const int warp = threadIdx.x >> 5;
   const bool aligned = (smem_u32(smem) & 1023u) == 0;
   if (!aligned) {
+    after_previous();
     if (threadIdx.x == 0) atomicCAS(&g_attention_error, 0u, 99u);
     return false;
   }
@@ -544,6 +546,8 @@ __device__ __forceinline__ bool setup(unsigned char* smem, uint32_t bars, uint32
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  let_next_start();
+  after_previous();
   if (*slot != 0) {  // 512 columns can only start at 0
     if (warp == 1)
       asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(*slot) : "memory");
@@ -965,7 +969,7 @@ __device__ __forceinline__ void dkv_tile(const AttentionArgs& a, const Split& sp
   const int4 tile = a.tile[t];
   const int per_head = (tile.y + kTileRows - 1) / kTileRows - tile.z;  // query blocks of a head
   const int shares = shares_of(a, per_head);
-  if (split >= shares) return;
+  if (split >= shares) return after_previous();
   const int first = (int)((int64_t)per_head * group * split / shares);
   const int n = (int)((int64_t)per_head * group * (split + 1) / shares) - first;
   // k and v, scores, dP, weights, dS, dv, dv drained, dk, dk drained, end
@@ -1156,6 +1160,8 @@ __global__ void __launch_bounds__(WarpsOf<DP>::kThreads, 1)
 // dk and dv of the tiles that have several shares, added in their order.
 // Grid: tiles x key/value heads, and eighths of a tile's rows.
 __global__ void __launch_bounds__(256) join_kernel(const AttentionArgs a) {
+  let_next_start();
+  after_previous();
   const int t = blockIdx.x / a.kv_heads, kv_head = blockIdx.x % a.kv_heads;
   const int4 tile = a.tile[t];
   const int shares = shares_of(a, (tile.y + kTileRows - 1) / kTileRows - tile.z);
@@ -1219,8 +1225,8 @@ lmpb_status forward(const AttentionArgs& a, const Split& s, cudaStream_t st) {
   if (r == LMPB_OK) r = allow_smem(forward_kernel<DP>, ForwardLayout<DP>::kBytes);
   if (r != LMPB_OK) return r;
   const bool vec = a.dim % 4 == 0 && aligned16(a.out);
-  forward_kernel<DP><<<(unsigned)(a.tiles * a.heads), WarpsOf<DP>::kThreads, ForwardLayout<DP>::kBytes, st>>>(a, s, vec);
-  return launch_status("attention");
+  return launch_early("attention", forward_kernel<DP>, dim3((unsigned)(a.tiles * a.heads)), WarpsOf<DP>::kThreads,
+                      ForwardLayout<DP>::kBytes, st, a, s, vec);
 }
 
 template <int DP>
@@ -1232,12 +1238,10 @@ lmpb_status backward(const AttentionArgs& a, const Split& s, float* delta, cudaS
   const int dkv = a.dk ? a.tiles * a.kv_heads * a.splits : 0, dq = a.dq ? a.tiles * a.heads : 0;
   const bool vec_dkv = a.dim % 4 == 0 && aligned16(a.dk) && aligned16(a.dv) && (!a.part || a.tokens * a.kv_heads * a.dim % 4 == 0);
   const bool vec_dq = a.dim % 4 == 0 && aligned16(a.dq);
-  backward_kernel<DP><<<(unsigned)(dkv + dq), WarpsOf<DP>::kThreads, bytes, st>>>(a, s, dkv, vec_dkv, vec_dq);
-  r = launch_status("attention_backward");
-  if (r == LMPB_OK && dkv > 0 && a.splits > 1) {
-    join_kernel<<<dim3((unsigned)(a.tiles * a.kv_heads), 8), 256, 0, st>>>(a);
-    r = launch_status("attention_backward (join)");
-  }
+  r = launch_early("attention_backward", backward_kernel<DP>, dim3((unsigned)(dkv + dq)), WarpsOf<DP>::kThreads, bytes, st, a,
+                   s, dkv, vec_dkv, vec_dq);
+  if (r == LMPB_OK && dkv > 0 && a.splits > 1)
+    r = launch_early("attention_backward (join)", join_kernel, dim3((unsigned)(a.tiles * a.kv_heads), 8), 256, 0, st, a);
   return r;
 }
 
