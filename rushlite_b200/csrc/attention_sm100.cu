@@ -1252,17 +1252,20 @@ bool attention_fits_sm100(const AttentionArgs& a) {
 }
 
 // Cuts the dk, dv work of the key tiles into shares, so that no SM ends long
-// after the others (one key/value head, or a long sequence): at most one and a
-// half times what an SM gets on average, as dq's CTAs fill what is left
-// ([1500, 31, 700, 1, 1865] x 16 heads (4) of 128: half the average 461 us, the
-// average 420, one and a half 421, two and a half 561), but not under 8 blocks,
-// where starting a CTA and joining the shares cost as much ([600, 300, 900] x
-// 12 (1) of 128: 6 blocks 138 us, 8 to 12 129, 16 139; [777, 1234] x 6 (1) of
-// 80: 87, 88 to 102, 111).
+// after the others (one key/value head, or a long sequence): five quarters of
+// what an SM gets on average, as dq's CTAs fill what is left, and 3 blocks
+// for what starting a CTA and joining the shares cost.  Backward, with
+// 3 + 1.25 / at least 8 and 1.5 / at least 2 and 2 times the average:
+//   [300] x 4 heads (1) of 64                       35 /  50 /  34 us
+//   [200, 700] x 4 (1) of 64                        42 /  51 /  46
+//   [2500] x 4 (1) of 64                            84 /  87 /  84
+//   [1024] x 4, 8 (2) of 64                         95 /  92 /  99
+//   [600, 300, 900] x 12 (1) of 128                130 / 130 / 130
+//   [1500, 31, 700, 1, 1865] x 16 (4) of 128       318 / 319 / 354
 void cut_dkv(AttentionArgs& a) {
   const int64_t group = a.heads / a.kv_heads, most = a.longest_tiles * group;
   const double average = (double)a.pair_tiles * a.heads / sm_count();
-  a.share = (int)std::max<int64_t>(8, std::min<int64_t>(most, (int64_t)(1.5 * average)));
+  a.share = (int)std::min<int64_t>(most, (int64_t)(3 + 1.25 * average));
   a.share = (int)std::max<int64_t>(a.share, (most + kMaxSplits - 1) / kMaxSplits);
   a.splits = (int)((most + a.share - 1) / a.share);
 }
