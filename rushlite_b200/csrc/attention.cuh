@@ -30,26 +30,6 @@ namespace lmpb {
 
 constexpr int kTileRows = 128;
 
-// The kernels of one call are launched so that each may start before the one
-// ahead of it has ended: it sets up its shared memory and TMEM, then
-// waits in after_previous() for that kernel's end and results.  Every
-// thread calls it before it touches what any kernel of the call reads or
-// writes, and before it leaves.  let_next_start() in the kernel ahead says
-// from when on.
-template <typename... P, typename... A>
-lmpb_status launch_early(const char* what, void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t st, A... args) {
-  cudaLaunchAttribute early{};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t c{};
-  c.gridDim = grid, c.blockDim = dim3((unsigned)threads), c.dynamicSmemBytes = (size_t)smem, c.stream = st;
-  c.attrs = &early, c.numAttrs = 1;
-  cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);  // an error is the next line's too
-  return launch_status(what);
-}
-__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // One call's arguments.  q, out, grad, dq: [tokens, heads, dim]; k, v, dk,
 // dv: [tokens, kv_heads, dim]; lse, delta: [heads, tokens].
 struct AttentionArgs {

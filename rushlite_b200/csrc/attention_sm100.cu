@@ -23,10 +23,12 @@
 //    bulk copies, no tensor maps.  Tiles never span sequences and rows
 //    behind a sequence are 0.  For v and grad it also finds the largest row
 //    norm, for grad the row sums delta = sum(grad * out).
-// 2. forward_kernel, dq_kernel, dkv_kernel: one CTA per tile and head, one
-//    CTA per SM.  Warp 0 feeds a ring of 16 KB units, warp 1 issues the
-//    MMAs, 8 or 16 warps compute.  A row of the 128 x 128 score tile lives in one
-//    TMEM lane; two or four threads of different warps share it.
+// 2. forward_kernel, backward_kernel: one CTA per tile and head (dk and dv: per
+//    share of a key tile's work), one CTA per SM.  Warp 0 feeds a ring of
+//    parts (the hi or lo half of a block, 16 or 32 KB), warp 1 issues the MMAs,
+//    8 (128 columns) or 16 (64) warps compute.  A row of the 128 x 128 score
+//    tile lives in one TMEM lane; two or four threads of different warps
+//    share it.
 //    Scores are overwritten in place by the split weights, which are then the
 //    next MMA's A operand straight from TMEM.
 //    Every mbarrier wait is bounded; after one expires the thread stops
@@ -1053,7 +1055,7 @@ __device__ __forceinline__ void dkv_tile(const AttentionArgs& a, const Split& sp
     const float* source = tid < 128 ? a.lse : a.delta;
     const auto fetch = [&](const Walk& w) {
       const int r = (tile.z + w.x) * kTileRows + (tid & 127);
-      return tid < 256 && r < tile.y ? __ldg(source + (int64_t)w.head * a.tokens + tile.x + r) : tid < 128 ? INFINITY : 0.f;
+      return tid < 256 && r < tile.y ? source[(int64_t)w.head * a.tokens + tile.x + r] : tid < 128 ? INFINITY : 0.f;
     };
     Walk at = begin, ahead = begin;
     float next = fetch(ahead);

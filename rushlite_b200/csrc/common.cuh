@@ -36,6 +36,27 @@ lmpb_status set_error(lmpb_status st, const std::string& msg);
 // Checks the launch that was just issued.
 lmpb_status launch_status(const char* what);
 
+// A kernel that may start before the one ahead of it in the stream, a kernel of
+// the same call, has ended: it sets itself up, then waits in after_previous()
+// for that kernel's end and results.  Every thread calls that before it touches
+// what a kernel of the call reads or writes, and before it leaves; what it reads
+// then are plain loads (neither __ldg nor const __restrict__, which the compiler
+// may move up).  let_next_start() in the kernel ahead says from when on; without
+// it, from when that kernel's last CTA ends.
+template <typename... P, typename... A>
+lmpb_status launch_early(const char* what, void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t st, A... args) {
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c{};
+  c.gridDim = grid, c.blockDim = dim3((unsigned)threads), c.dynamicSmemBytes = (size_t)smem, c.stream = st;
+  c.attrs = &early, c.numAttrs = 1;
+  cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);  // an error is the next line's too
+  return launch_status(what);
+}
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 bool valid_dtype(int dt);

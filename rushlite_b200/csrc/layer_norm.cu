@@ -150,9 +150,9 @@ constexpr int resident() { return TPR <= 256 && E * sizeof(T) <= 64 ? 2 : 1; }
 
 // part: [gridDim.x, 2, F] of dw and db, or with one CTA the results
 // themselves; null when neither is wanted.  The next row's x and g are loaded
-// before this row's sums are awaited (without that, 82 us instead of 62 for
-// [8192, 4096]; the same rows fetched by bulk copies into a ring in shared
-// memory: 104, since fewer threads are then there to add).
+// before this row's sums are awaited ([8192, 4096], with a slower fold than now:
+// 77.6 us, without 88, and 109 with the rows fetched by bulk copies into a
+// ring in shared memory, since fewer threads are then there to add).
 template <typename T, int VEC, int NV, int TPR>
 __global__ void __launch_bounds__(block_of(TPR), resident<T, NV * VEC, TPR>())
     backward_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __restrict__ mean,
@@ -256,11 +256,12 @@ __global__ void __launch_bounds__(block_of(TPR), resident<T, NV * VEC, TPR>())
 
 // out[c] = sum over the table's rows of column c: 32 columns a CTA, 32 row
 // lanes folded in order (8 lanes of four times the rows waited 13 us for
-// [296, 2 x 4096]).  Columns [0, F) go to dw, [F, 2F) to db.
+// [296, 2 x 4096], these 6.5).  It starts under the last rows' CTAs: 2.5 us less.  Columns [0, F) go to dw, [F, 2F) to db.
 template <typename T>
 __global__ void __launch_bounds__(1024)
-    fold_kernel(const T* __restrict__ part, int rows, int F, T* __restrict__ dw, T* __restrict__ db) {
+    fold_kernel(const T* part, int rows, int F, T* dw, T* db) {
   __shared__ T s[32][33];
+  after_previous();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t col = (int64_t)blockIdx.x * 32 + tx, W = 2 * (int64_t)F;
   T t = T(0);
@@ -478,8 +479,8 @@ lmpb_status backward(const void* x, const void* w, const void* mean, const void*
     }
   }
   if (s == LMPB_OK && table) {
-    fold_kernel<T><<<(unsigned)((2 * F + 31) / 32), 1024, 0, st>>>(part, prows, (int)F, (T*)dw, (T*)db);
-    s = launch_status("layer_norm_backward (fold)");
+    s = launch_early("layer_norm_backward (fold)", fold_kernel<T>, dim3((unsigned)((2 * F + 31) / 32)), 1024, 0, st, part, prows,
+                     (int)F, (T*)dw, (T*)db);
   }
   if (part) {
     const cudaError_t e = cudaFreeAsync(part, st);
