@@ -527,6 +527,8 @@ extern "C" lmpb_status lmpb_sequences_create(const int64_t* lengths, int count, 
       cudaError_t e = cudaGetDevice(&h->device);
       if (e == cudaSuccess) e = cudaMalloc(&h->block, bytes);
       if (e == cudaSuccess) e = cudaMemcpy(h->block, host.data(), bytes, cudaMemcpyHostToDevice);
+      // a copy from pageable memory may return with its last part under way, and the user's stream need not wait for it
+      if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
       if (e != cudaSuccess) {
         cudaGetLastError();
         if (h->block) cudaFree(h->block);

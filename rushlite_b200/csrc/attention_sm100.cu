@@ -1160,8 +1160,14 @@ __global__ void __launch_bounds__(WarpsOf<DP>::kThreads, 1)
 }
 
 // dk and dv of the tiles that have several shares, added in their order.
-// Grid: tiles x key/value heads, and eighths of a tile's rows.
+// Grid: tiles x key/value heads, and eighths of a tile's rows.  Latency bound,
+// so V = 4 floats a load where rows allow it ([4096] x 8 heads (2) of 128:
+// 9 us, 22 with one).
+template <int V>
 __global__ void __launch_bounds__(256) join_kernel(const AttentionArgs a) {
+  struct alignas(4 * V) Pack {
+    float x[V];
+  };
   let_next_start();
   after_previous();
   const int t = blockIdx.x / a.kv_heads, kv_head = blockIdx.x % a.kv_heads;
@@ -1170,16 +1176,19 @@ __global__ void __launch_bounds__(256) join_kernel(const AttentionArgs a) {
   if (shares == 1) return;
   const int row0 = blockIdx.y * (kTileRows / 8), rows = min(kTileRows / 8, tile.y - tile.z * kTileRows - row0);
   const int64_t values = a.tokens * a.kv_heads * a.dim;
-  for (int i = threadIdx.x; i < rows * a.dim; i += 256) {
-    const int64_t at = ((int64_t)(tile.x + tile.z * kTileRows + row0 + i / a.dim) * a.kv_heads + kv_head) * a.dim + i % a.dim;
-    float k = 0.f, v = 0.f;
+  const int packs = a.dim / V;
+  for (int i = threadIdx.x; i < rows * packs; i += 256) {
+    const int64_t at = ((int64_t)(tile.x + tile.z * kTileRows + row0 + i / packs) * a.kv_heads + kv_head) * a.dim + i % packs * V;
+    Pack k{}, v{};
 #pragma unroll 4
     for (int s = 0; s < shares; ++s) {
-      k += a.part[2 * s * values + at];
-      v += a.part[(2 * s + 1) * values + at];
+      const Pack x = *reinterpret_cast<const Pack*>(a.part + 2 * s * values + at);
+      const Pack y = *reinterpret_cast<const Pack*>(a.part + (2 * s + 1) * values + at);
+#pragma unroll
+      for (int c = 0; c < V; ++c) k.x[c] += x.x[c], v.x[c] += y.x[c];
     }
-    a.dk[at] = k;
-    a.dv[at] = v;
+    *reinterpret_cast<Pack*>(a.dk + at) = k;
+    *reinterpret_cast<Pack*>(a.dv + at) = v;
   }
 }
 
@@ -1243,7 +1252,7 @@ lmpb_status backward(const AttentionArgs& a, const Split& s, float* delta, cudaS
   r = launch_early("attention_backward", backward_kernel<DP>, dim3((unsigned)(dkv + dq)), WarpsOf<DP>::kThreads, bytes, st, a,
                    s, dkv, vec_dkv, vec_dq);
   if (r == LMPB_OK && dkv > 0 && a.splits > 1)
-    r = launch_early("attention_backward (join)", join_kernel, dim3((unsigned)(a.tiles * a.kv_heads), 8), 256, 0, st, a);
+    r = launch_early("attention_backward (join)", vec_dkv ? join_kernel<4> : join_kernel<1>, dim3((unsigned)(a.tiles * a.kv_heads), 8), 256, 0, st, a);
   return r;
 }
 

@@ -118,6 +118,24 @@ def test_recorded_step_counts_its_replays(cuda):
         assert (p.numpy() == q.numpy()).all()
 
 
+def test_recorded_step_outlives_the_optimizer(cuda):
+    import rushlite_b200 as rsl
+
+    rng = np.random.default_rng(6)
+    sets = [_random(rng, (300, 100), "float32")]
+    opt, twin = _optimizer(rsl, sets, "float32"), _optimizer(rsl, sets, "float32")
+    param, graph = opt.params[0], rsl.cuda.Graph()
+    with graph:
+        opt.step()
+    del opt
+    junk = [rsl.Variable(np.full((300, 100), 1e9, np.float32)) for _ in range(8)]  # over any memory given back
+    for _ in range(3):
+        graph.replay()
+        twin.step()
+    assert (param.numpy() == twin.params[0].numpy()).all()
+    assert all((j.numpy() == 1e9).all() for j in junk)
+
+
 def test_special_values_stay_where_they_are(cuda):
     import rushlite_b200 as rsl
 

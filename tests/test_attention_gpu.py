@@ -401,6 +401,44 @@ def test_two_graphs_in_turn(cuda):
             assert (var[n].grad.numpy() == want["d" + n]).all(), n
 
 
+def test_two_streams_at_once(cuda):
+    """Calls on two streams share nothing but the sequences, which are there as soon as they are made."""
+    from rushlite_b200 import capi
+
+    torch = cuda
+    lengths, h, kv, d = [700, 1, 129, 40, 500], 4, 2, 64
+    n = sum(lengths)
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    sets = []
+    for _ in range(2):
+        x = [torch.randn(n, m, d, device="cuda", generator=gen) for m in (h, kv, kv, h)]  # q, k, v, grad
+        sets.append((x, [torch.full_like(x[i], math.nan) for i in (0, 0, 1, 2)], torch.empty(h, n, device="cuda")))
+
+    def call(x, y, lse, seqs, stream):
+        p = [a.data_ptr() for a in (*x, *y, lse)]
+        capi.attention(p[0], p[1], p[2], p[4], p[8], n, h, kv, d, 0.125, seqs, stream)
+        capi.attention_backward(p[0], p[1], p[2], p[4], p[8], p[3], p[5], p[6], p[7], n, h, kv, d, 0.125, seqs, stream)
+
+    want = []
+    for x, y, lse in sets:
+        call(x, y, lse, capi.Sequences(lengths), 0)
+        torch.cuda.synchronize()
+        want.append([a.clone() for a in (*y, lse)])
+        for a in (*y, lse):
+            a.fill_(math.nan)
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    seqs = capi.Sequences(lengths)
+    for _ in range(20):
+        for s, (x, y, lse) in zip(streams, sets):
+            call(x, y, lse, seqs, s.cuda_stream)
+    torch.cuda.synchronize()
+    for (x, y, lse), w in zip(sets, want):
+        for a, b in zip((*y, lse), w):
+            assert torch.equal(a, b)
+    capi.device_error()
+
+
 def test_offsets_past_32_bits(cuda):
     """q, out and their gradients hold over 2^31 values."""
     from rushlite_b200 import capi
