@@ -1160,9 +1160,11 @@ __global__ void __launch_bounds__(WarpsOf<DP>::kThreads, 1)
 }
 
 // dk and dv of the tiles that have several shares, added in their order.
-// Grid: tiles x key/value heads, and eighths of a tile's rows.  Latency bound,
-// so V = 4 floats a load where rows allow it ([4096] x 8 heads (2) of 128:
-// 9 us, 22 with one).
+// Grid: tiles x key/value heads, and kJoin shares of a tile's rows.  Latency
+// bound, so V = 4 floats a load where rows allow it ([4096] x 8 heads (2) of
+// 128 with 8 shares of rows: 9 us, 22 with one float), and one load a thread.
+constexpr int kJoin = 16;
+
 template <int V>
 __global__ void __launch_bounds__(256) join_kernel(const AttentionArgs a) {
   struct alignas(4 * V) Pack {
@@ -1174,7 +1176,7 @@ __global__ void __launch_bounds__(256) join_kernel(const AttentionArgs a) {
   const int4 tile = a.tile[t];
   const int shares = shares_of(a, (tile.y + kTileRows - 1) / kTileRows - tile.z);
   if (shares == 1) return;
-  const int row0 = blockIdx.y * (kTileRows / 8), rows = min(kTileRows / 8, tile.y - tile.z * kTileRows - row0);
+  const int row0 = blockIdx.y * (kTileRows / kJoin), rows = min(kTileRows / kJoin, tile.y - tile.z * kTileRows - row0);
   const int64_t values = a.tokens * a.kv_heads * a.dim;
   const int packs = a.dim / V;
   for (int i = threadIdx.x; i < rows * packs; i += 256) {
@@ -1252,7 +1254,7 @@ lmpb_status backward(const AttentionArgs& a, const Split& s, float* delta, cudaS
   r = launch_early("attention_backward", backward_kernel<DP>, dim3((unsigned)(dkv + dq)), WarpsOf<DP>::kThreads, bytes, st, a,
                    s, dkv, vec_dkv, vec_dq);
   if (r == LMPB_OK && dkv > 0 && a.splits > 1)
-    r = launch_early("attention_backward (join)", vec_dkv ? join_kernel<4> : join_kernel<1>, dim3((unsigned)(a.tiles * a.kv_heads), 8), 256, 0, st, a);
+    r = launch_early("attention_backward (join)", vec_dkv ? join_kernel<4> : join_kernel<1>, dim3((unsigned)(a.tiles * a.kv_heads), kJoin), 256, 0, st, a);
   return r;
 }
 
@@ -1264,19 +1266,19 @@ bool attention_fits_sm100(const AttentionArgs& a) {
 
 // Cuts the dk, dv work of the key tiles into shares, so that no SM ends long
 // after the others (one key/value head, or a long sequence): five quarters of
-// what an SM gets on average, as dq's CTAs fill what is left, and 3 blocks
-// for what starting a CTA and joining the shares cost.  Backward, with
-// 3 + 1.25 / at least 8 and 1.5 / at least 2 and 2 times the average:
-//   [300] x 4 heads (1) of 64                       35 /  50 /  34 us
-//   [200, 700] x 4 (1) of 64                        42 /  51 /  46
-//   [2500] x 4 (1) of 64                            84 /  87 /  84
-//   [1024] x 4, 8 (2) of 64                         95 /  92 /  99
-//   [600, 300, 900] x 12 (1) of 128                130 / 130 / 130
-//   [1500, 31, 700, 1, 1865] x 16 (4) of 128       318 / 319 / 354
+// what an SM gets on average, as dq's CTAs fill what is left, and 2 blocks
+// for what starting a CTA and joining the shares cost.  Backward, us:
+//                                             2 + 1.25   2 + 1   3 + 1.25   at least 8, 1.5
+//   [300] x 4 heads (1) of 64                    28        28       31          50
+//   [2500] x 4 (1) of 64                         75        82       74          87
+//   [1024] x 4, 8 (2) of 64                      86        91       89          92
+//   [600, 300, 900] x 12 (1) of 128             102       102      103         130
+//   [1500, 31, 700, 1, 1865] x 16 (4) of 128    310       319      309         319
+// (the last column with a slower join than now)
 void cut_dkv(AttentionArgs& a) {
   const int64_t group = a.heads / a.kv_heads, most = a.longest_tiles * group;
   const double average = (double)a.pair_tiles * a.heads / sm_count();
-  a.share = (int)std::min<int64_t>(most, (int64_t)(3 + 1.25 * average));
+  a.share = (int)std::min<int64_t>(most, (int64_t)(2 + 1.25 * average));
   a.share = (int)std::max<int64_t>(a.share, (most + kMaxSplits - 1) / kMaxSplits);
   a.splits = (int)((most + a.share - 1) / a.share);
 }
