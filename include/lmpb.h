@@ -302,7 +302,8 @@ lmpb_status lmpb_reduce_allreduce(int op, int dtype, const void* in, const int64
 /* ------------------------------------------- transformer training
  *
  * Operators of a transformer block's training step.  No counterpart in the
- * reference, whose layers stop at Linear, activations and Softmax. */
+ * reference, whose layers stop at Linear, activations and Softmax.  No output
+ * may overlap an input or another output; AdamW's are in place. */
 
 /* Layer norm over the last axis of x [rows, features], FLOAT32 or FLOAT64:
  *   y = (x - mean) / sqrt(var + eps) * weight + bias
