@@ -133,14 +133,33 @@ __device__ __forceinline__ float two_to(int e) { return __int_as_float((e + 127)
 // Lane l holds columns 4 l.. of a row (DP = 128), or lanes l and l + 16 hold
 // one of two rows (DP = 64).  Bound by HBM and, one tile a CTA, by latency:
 // 32 warps an SM are needed ([1500, 31, 700, 1, 1865] x 24 planes of 128: 27
-// us with 16 rows a warp, 25 with 8; 40 planes of the backward: 64 and 50).
+// us with 16 rows a warp, 25 with 8; 40 planes of the backward: 64 and 50;
+// with fold_rows in place of a tree for each row then 21 and 45).
 template <int DP>
 constexpr int split_warps() { return DP / 8; }
+
+// Eight rows' partial results, one of each in every of their LANES lanes, into
+// one row's result a lane: of row lane % LANES / (LANES / 8).  9 shuffles
+// (LANES = 32) where a tree for each row takes 40.
+template <int LANES, typename F>
+__device__ __forceinline__ float fold_rows(float (&x)[8], int lane, F f) {
+#pragma unroll
+  for (int n = 4, off = LANES / 2; n; n >>= 1, off >>= 1) {
+    const bool upper = lane & off;
+#pragma unroll
+    for (int i = 0; i < n; ++i)
+      x[i] = f(upper ? x[i + n] : x[i], __shfl_xor_sync(0xffffffffu, upper ? x[i] : x[i + n], off));
+  }
+#pragma unroll
+  for (int off = LANES / 16; off; off >>= 1) x[0] = f(x[0], __shfl_xor_sync(0xffffffffu, x[0], off));
+  return x[0];
+}
 
 template <int DP>
 __global__ void __launch_bounds__(32 * split_warps<DP>(), 2048 / (64 * split_warps<DP>())) split_kernel(const AttentionArgs a, const Split o, float* __restrict__ delta, bool vec) {
   constexpr int WARPS = split_warps<DP>(), ROWS = 128 / WARPS;  // of a warp
   constexpr int RPS = 128 / DP, STEPS = ROWS / RPS, LANES = 32 / RPS;  // rows a step, steps, lanes a row
+  static_assert(STEPS == 8, "fold_rows");
   let_next_start();
   const int64_t plane = blockIdx.y;
   const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -171,35 +190,32 @@ __global__ void __launch_bounds__(32 * split_warps<DP>(), 2048 / (64 * split_war
   float4 v[STEPS];
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) v[i] = load4(base, warp * ROWS + i * RPS + sub);
-  float mx = 0.f, mn = INFINITY, nrm = 0.f, dmx = 0.f;
-  bool bad = false;
+  const auto more = [](float x, float y) { return fmaxf(x, y); };
+  const auto sum = [](float x, float y) { return x + y; };
+  const int r1 = warp * ROWS + lane % LANES / (LANES / 8) * RPS + sub;  // the row whose result fold_rows leaves here
+  float part[STEPS];
 #pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    float m = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
-    bad |= !(fabsf(v[i].x) < INFINITY && fabsf(v[i].y) < INFINITY && fabsf(v[i].z) < INFINITY && fabsf(v[i].w) < INFINITY);
+  for (int i = 0; i < STEPS; ++i)
+    part[i] = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
+  float mx = fold_rows<LANES>(part, lane, more), mn = mx > 0.f ? mx : INFINITY;
 #pragma unroll
-    for (int s = LANES / 2; s; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-    mx = fmaxf(mx, m);
-    if (m > 0.f) mn = fminf(mn, m);
-    float q = v[i].x * v[i].x + v[i].y * v[i].y + v[i].z * v[i].z + v[i].w * v[i].w, d = 0.f;
-    const int r = warp * ROWS + i * RPS + sub;
-    if (is_g) {
-      const float4 u = load4(obase, r);
-      d = v[i].x * u.x + v[i].y * u.y + v[i].z * u.z + v[i].w * u.w;
+  for (int i = 0; i < STEPS; ++i) part[i] = v[i].x * v[i].x + v[i].y * v[i].y + v[i].z * v[i].z + v[i].w * v[i].w;
+  float nrm = fold_rows<LANES>(part, lane, sum), dmx = 0.f;
+  bool bad = !(nrm < INFINITY);  // infinities and NaN, and values past the range anyway
+  if (is_g) {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const float4 u = load4(obase, warp * ROWS + i * RPS + sub);
+      part[i] = v[i].x * u.x + v[i].y * u.y + v[i].z * u.z + v[i].w * u.w;
     }
-#pragma unroll
-    for (int s = LANES / 2; s; s >>= 1) q += __shfl_xor_sync(0xffffffffu, q, s);
-    nrm = fmaxf(nrm, q);
-    if (is_g) {
-#pragma unroll
-      for (int s = LANES / 2; s; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
-      dmx = fmaxf(dmx, fabsf(d));
-      if (lane % LANES == 0 && r < rows) delta[(int64_t)head * a.tokens + first + r] = d;
-    }
+    const float d = fold_rows<LANES>(part, lane, sum);
+    dmx = fabsf(d);
+    bad |= !(dmx < INFINITY);
+    if (lane % (LANES / 8) == 0 && r1 < rows) delta[(int64_t)head * a.tokens + first + r1] = d;
   }
   __shared__ float red[4][WARPS];
 #pragma unroll
-  for (int s = 16; s; s >>= 1) {
+  for (int s = 16; s >= LANES / 8; s >>= 1) {
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
     mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, s));
     nrm = fmaxf(nrm, __shfl_xor_sync(0xffffffffu, nrm, s));
@@ -217,7 +233,7 @@ __global__ void __launch_bounds__(32 * split_warps<DP>(), 2048 / (64 * split_war
   // a gradient's small rows only ever add to larger sums: no limit on their range
   const bool range = mx > 0.f && (mx > 0x1p40f || mx < 0x1p-60f || (!is_g && mn < mx * 0x1p-18f));
   const bool far = !is_v && !is_g && !(nrm * a.scale <= 0x1p14f);  // so |q| |k| scale <= 2^14 of unflagged tiles
-  const bool flag = bads || range || far || !(dmx < INFINITY);
+  const bool flag = bads || range || far;
   const int e = flag ? 0 : row_exp(mx);
   const int64_t block = plane * a.tiles + t;
   if (threadIdx.x == 0) {
