@@ -13,7 +13,8 @@
 //
 // A row of up to 512 values, or 1024 in float32, belongs to one warp (8 rows a
 // CTA, no barrier); a row of up to 8192 to a CTA of 256 to 1024 threads.
-// Longer rows are walked in memory (the *_long kernels).  The backward's CTAs stay resident and walk
+// Longer rows, and in the backward doubles past 4096, are walked in memory
+// (the *_long kernels).  The backward's CTAs stay resident and walk
 // rows with a stride; each thread keeps its columns' share of dw and db in
 // registers, writes it once at its end as one row of a partial table, and a
 // second kernel adds the table's rows in their order, so the same call gives
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// ------------------------------------------------ rows over 8192 values
+// ------------------------------------------------ rows past the tiles
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
@@ -374,31 +375,33 @@ bool by_warps(int64_t rows, int64_t features) {
 }
 
 // Calls f.run<VEC, NV, TPR>() for the tile that holds a row of F values;
-// false when none does.  `wide`: doubles spread over 512 threads, which
-// leaves the backward's sums in registers ([2048, 4096]: 50 us, 62 over 256;
-// the forward has less to hold: 33 and 29).
-template <typename T, int VEC, typename F>
-bool with_tile(int64_t rows, int64_t features, bool wide, F&& f) {
+// false when none does.  SUMS: the backward, whose two rows and two sums per
+// value have to stay in registers: doubles spread over 512 threads ([2048,
+// 4096]: 50 us, 62 over 256; the forward has less to hold: 33 and 29), and more
+// than 4096 floats too ([4096, 8192]: 76 us, 102 over 1024, which spill).
+template <typename T, int VEC, bool SUMS, typename F>
+bool with_tile(int64_t rows, int64_t features, F&& f) {
   if (by_warps<T>(rows, features)) {
     if (features <= 32 * 4) f.template run<VEC, 4 / VEC, 32>();
     else if (features <= 32 * 8) f.template run<VEC, 8 / VEC, 32>();
     else if (features <= 32 * 16) f.template run<VEC, 16 / VEC, 32>();
     else if constexpr (sizeof(T) == 4) f.template run<VEC, 32 / VEC, 32>();
-  } else if (features <= 256 * 4) {
+    return true;
+  }
+  if (features <= 256 * 4) {
     f.template run<VEC, 4 / VEC, 256>();
-  } else if (sizeof(T) == 8 && wide && features <= 512 * 8) {
-    if constexpr (sizeof(T) == 8) {
-      if (features <= 512 * 4) f.template run<VEC, 4 / VEC, 512>();
-      else f.template run<VEC, 8 / VEC, 512>();
-    }
-  } else if (features <= 256 * 8) {
-    f.template run<VEC, 8 / VEC, 256>();
-  } else if (features <= 256 * 16) {
-    f.template run<VEC, 16 / VEC, 256>();
-  } else if (features <= 1024 * 8) {
-    f.template run<VEC, 8 / VEC, 1024>();
+    return true;
+  }
+  if constexpr (SUMS && sizeof(T) == 8) {
+    if (features > 512 * 8) return false;
+    if (features <= 512 * 4) f.template run<VEC, 4 / VEC, 512>();
+    else f.template run<VEC, 8 / VEC, 512>();
   } else {
-    return false;
+    if (features > 8192) return false;
+    if (features <= 256 * 8) f.template run<VEC, 8 / VEC, 256>();
+    else if (features <= 256 * 16) f.template run<VEC, 16 / VEC, 256>();
+    else if constexpr (SUMS) f.template run<VEC, 16 / VEC, 512>();
+    else f.template run<VEC, 8 / VEC, 1024>();
   }
   return true;
 }
@@ -439,7 +442,7 @@ lmpb_status forward(const void* x, const void* w, const void* b, int64_t rows, i
   constexpr int V = 16 / sizeof(T);
   Forward<T> f{(const T*)x, (const T*)w, (const T*)b, (T*)y, (T*)mean, (T*)rstd, rows, F, eps, st};
   const bool vec = F % V == 0 && aligned16(x) && aligned16(y) && aligned16(w) && aligned16(b);
-  if (!(vec ? with_tile<T, V>(rows, F, false, f) : with_tile<T, 1>(rows, F, false, f)))
+  if (!(vec ? with_tile<T, V, false>(rows, F, f) : with_tile<T, 1, false>(rows, F, f)))
     forward_long_kernel<T><<<grid_of(rows, 1, 8), kThreads, 0, st>>>(f.x, f.w, f.b, f.y, f.mean, f.rstd, rows, F,
                                                                      T(1.0 / (double)F), T(eps));
   return launch_status("layer_norm");
@@ -449,10 +452,14 @@ template <typename T>
 lmpb_status backward(const void* x, const void* w, const void* mean, const void* rstd, const void* g, int64_t rows,
                      int64_t F, void* dx, void* dw, void* db, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const bool columns = dw || db, lng = F > 8192;
+  // past the tiles ([20000, 4100] double: 0.63 ms; in a tile of 1024 threads, which spills, 1.43)
+  const bool columns = dw || db, lng = F > (sizeof(T) == 8 ? 4096 : 8192);
   const bool vec = F % V == 0 && aligned16(x) && aligned16(g) && aligned16(dx) && aligned16(w);
+  const bool warps = by_warps<T>(rows, F);
+  // as many CTAs as fit at once, two where resident() allows ([2048, 4096] double: 42 us, 47.5 with twice the CTAs)
+  const int fit = F > (warps ? 2048 / (int)sizeof(T) : sizeof(T) == 8 ? 1024 : 4096) ? 1 : 2;
   // a few rows: one CTA, whose sums over rows are the results (32 x 256: one launch instead of two)
-  const unsigned grid = !lng && rows * F <= 8192 ? 1 : grid_of(rows, by_warps<T>(rows, F) ? kThreads / 32 : 1, 2);
+  const unsigned grid = !lng && rows * F <= 8192 ? 1 : grid_of(rows, warps ? kThreads / 32 : 1, fit);
   const bool table = columns && (lng || grid > 1);
   const int64_t chunk = std::max<int64_t>(32, (rows + 63) / 64);
   const int prows = lng ? (int)((rows + chunk - 1) / chunk) : (int)grid;
@@ -462,8 +469,8 @@ lmpb_status backward(const void* x, const void* w, const void* mean, const void*
   if (!lng) {
     Backward<T> f{(const T*)x, (const T*)w, (const T*)mean, (const T*)rstd, (const T*)g,
                   (T*)dx,      part,        (T*)dw,         (T*)db,         rows, F, grid, st};
-    if (vec) with_tile<T, V>(rows, F, true, f);
-    else with_tile<T, 1>(rows, F, true, f);
+    if (vec) with_tile<T, V, true>(rows, F, f);
+    else with_tile<T, 1, true>(rows, F, f);
     s = launch_status("layer_norm_backward");
   } else {
     if (dx) {

@@ -14,7 +14,8 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 SHAPES = [(1, 1), (1, 7), (3, 64), (32, 256), (9, 100), (5, 129), (17, 513), (40, 1001), (33, 1024), (7, 1025),
-          (300, 2048), (4, 2052), (19, 4096), (3, 4099), (2, 8192), (3, 8193), (2, 20000), (1500, 32)]
+          (300, 2048), (4, 2052), (19, 4096), (3, 4099), (2, 8192), (3, 8193), (2, 20000), (1500, 32),
+          (310, 5001), (700, 1030), (330, 6144)]
 HALF = {"float32": 2.0 ** -24, "float64": 2.0 ** -53}
 C = 64
 
