@@ -12,7 +12,7 @@
 // pass costs no traffic and has no cancellation for a large mean.
 //
 // A row of up to 512 values, or 1024 in float32, belongs to one warp (8 rows a
-// CTA, no barrier); a row of up to 8192 to a CTA of 256 to 1024 threads.
+// CTA, no barrier); a row of up to 8192 to a CTA of 256 or 512 threads.
 // Longer rows, and in the backward doubles past 4096, are walked in memory
 // (the *_long kernels).  The backward's CTAs stay resident and walk
 // rows with a stride; each thread keeps its columns' share of dw and db in
@@ -376,9 +376,10 @@ bool by_warps(int64_t rows, int64_t features) {
 
 // Calls f.run<VEC, NV, TPR>() for the tile that holds a row of F values;
 // false when none does.  SUMS: the backward, whose two rows and two sums per
-// value have to stay in registers: doubles spread over 512 threads ([2048,
-// 4096]: 50 us, 62 over 256; the forward has less to hold: 33 and 29), and more
-// than 4096 floats too ([4096, 8192]: 76 us, 102 over 1024, which spill).
+// value have to stay in registers, so doubles spread over 512 threads ([2048,
+// 4096]: 50 us, 62 over 256; the forward has less to hold: 33 and 29).  More
+// than 4096 values take 512 threads too ([4096, 8192]: forward 52 us, backward
+// 76; over 1024 threads 91 and 102).
 template <typename T, int VEC, bool SUMS, typename F>
 bool with_tile(int64_t rows, int64_t features, F&& f) {
   if (by_warps<T>(rows, features)) {
@@ -400,8 +401,7 @@ bool with_tile(int64_t rows, int64_t features, F&& f) {
     if (features > 8192) return false;
     if (features <= 256 * 8) f.template run<VEC, 8 / VEC, 256>();
     else if (features <= 256 * 16) f.template run<VEC, 16 / VEC, 256>();
-    else if constexpr (SUMS) f.template run<VEC, 16 / VEC, 512>();
-    else f.template run<VEC, 8 / VEC, 1024>();
+    else f.template run<VEC, 16 / VEC, 512>();
   }
   return true;
 }
