@@ -205,3 +205,38 @@ def test_refusals(cuda):
     y = rsl.layer_norm(rsl.ones([4, 8], True))
     with pytest.raises(RuntimeError, match="shape"):
         y.backward(rsl.ones([8, 4]))
+
+
+@pytest.mark.parametrize("rows,features", [(4, 64), (700, 1030), (60, 9000)])
+def test_recorded_passes_give_the_same_bits(cuda, rows, features):
+    """Eager, recorded and replayed, on another stream too: one CTA, tiles with the fold behind them, long rows."""
+    import rushlite_b200 as rsl
+
+    rng = np.random.default_rng(rows)
+    val = {"x": (rows, features), "w": (features,), "b": (features,), "g": (rows, features)}
+    val = {n: rng.standard_normal(s).astype(np.float32) for n, s in val.items()}
+    var = {n: rsl.Variable(a, n != "g") for n, a in val.items()}
+
+    def step():
+        for n in "xwb":
+            var[n].zero_grad()
+        y = rsl.layer_norm(var["x"], var["w"], var["b"])
+        y.backward(var["g"])
+        return y
+
+    y = step()
+    want = [y.numpy()] + [var[n].grad.numpy() for n in "xwb"]
+    s = cuda.cuda.Stream()
+    try:
+        rsl.cuda.set_stream(s.cuda_stream)
+        graph = rsl.cuda.Graph()
+        with graph:
+            y = step()
+        for _ in range(3):
+            graph.replay()
+        got = [y.numpy()] + [var[n].grad.numpy() for n in "xwb"]
+    finally:
+        rsl.cuda.synchronize()
+        rsl.cuda.set_stream(0)
+    for a, b in zip(got, want):
+        assert (a == b).all()
