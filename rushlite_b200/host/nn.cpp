@@ -60,12 +60,13 @@ using tensor::TensorImpl;
 
 namespace {
 
-Tensor empty(const std::vector<size_t>& shape, DataType dt) {
+// `extra`: bytes behind the values, for what belongs to them.
+Tensor empty(const std::vector<size_t>& shape, DataType dt, size_t extra = 0) {
   auto p = std::make_shared<TensorImpl>();
   p->shape = shape;
   p->dtype = dt;
   p->device = DeviceType::CUDA;
-  p->storage = tensor::make_storage(p->nbytes(), p->device);
+  p->storage = tensor::make_storage(p->nbytes() + extra, p->device);
   return Tensor(p);
 }
 
@@ -142,7 +143,8 @@ struct LayerNormBackward : Function {
 };
 
 struct AttentionBackward : Function {
-  Tensor lse;
+  tensor::Storage buffer;  // out's, with lse behind it
+  float* lse = nullptr;
   std::shared_ptr<tensor::Sequences> seqs;
   float scale = 1.f;
   void apply(const Variable& out) override {
@@ -160,7 +162,7 @@ struct AttentionBackward : Function {
     }
     const std::vector<size_t>& s = q.shape();
     if (tensor::Graph* g = tensor::capturing_graph()) g->keep(seqs);
-    LMPB_OK_OR_THROW(lmpb_attention_backward(pq, pk, pv, (const float*)ptr(out.data()), (const float*)ptr(lse), pg,
+    LMPB_OK_OR_THROW(lmpb_attention_backward(pq, pk, pv, (const float*)ptr(out.data()), lse, pg,
                                              (float*)dq.get(), pdk, pdv, (int64_t)s[0], (int)s[1], (int)k.shape()[1],
                                              (int)s[2], scale, seqs->handle, tensor::current_stream()));
     dq.add(), dk.add(), dv.add();
@@ -224,13 +226,14 @@ Variable causal_attention(const Variable& q, const Variable& k, const Variable& 
   variable_list in{q, k, v};
   const bool rg = records(in);
   const float *pq = (const float*)ptr(q.data()), *pk = (const float*)ptr(k.data()), *pv = (const float*)ptr(v.data());
-  Tensor out = empty(s, DataType::Float32);
+  Tensor out = empty(s, DataType::Float32, s[0] * s[1] * sizeof(float));
   auto fn = std::make_shared<AttentionBackward>();
-  fn->lse = empty({s[1], s[0]}, DataType::Float32);
+  fn->buffer = out.impl()->storage;
+  fn->lse = (float*)ptr(out) + out.numel();
   fn->seqs = seqs;
   fn->scale = sc;
   if (tensor::Graph* g = tensor::capturing_graph()) g->keep(seqs);
-  LMPB_OK_OR_THROW(lmpb_attention(pq, pk, pv, (float*)ptr(out), (float*)ptr(fn->lse), (int64_t)s[0], (int)s[1], (int)t[1],
+  LMPB_OK_OR_THROW(lmpb_attention(pq, pk, pv, (float*)ptr(out), fn->lse, (int64_t)s[0], (int)s[1], (int)t[1],
                                   (int)s[2], sc, seqs->handle, tensor::current_stream()));
   return output(out, rg, fn, std::move(in));
 }
