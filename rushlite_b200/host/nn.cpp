@@ -71,7 +71,6 @@ Tensor empty(const std::vector<size_t>& shape, DataType dt, size_t extra = 0) {
 }
 
 void* ptr(const Tensor& t) { return t.impl()->data(); }
-void* row_of(const Tensor& t, size_t i) { return static_cast<char*>(ptr(t)) + i * (t.impl()->nbytes() / t.shape()[0]); }
 
 bool on_cuda(const Variable& v) { return v.data().device() == DeviceType::CUDA; }
 
@@ -125,7 +124,8 @@ Variable output(const Tensor& t, bool rg, std::shared_ptr<Function> fn, variable
 }
 
 struct LayerNormBackward : Function {
-  Tensor stats;  // [2, rows]: mean, 1 / deviation
+  tensor::Storage buffer;  // of the next two
+  void *mean = nullptr, *rstd = nullptr;
   bool has_weight = false, has_bias = false;
   void apply(const Variable& out) override {
     variable_list& in = *saved_inputs;
@@ -136,7 +136,7 @@ struct LayerNormBackward : Function {
     const void* pw = has_weight ? ptr(in[1].data()) : nullptr;
     GradOut dx(&in[0]), dw(has_weight ? &in[1] : nullptr), db(has_bias ? &in.back() : nullptr);
     const int64_t f = (int64_t)x.shape().back();
-    LMPB_OK_OR_THROW(lmpb_layer_norm_backward((int)x.type(), px, pw, ptr(stats), row_of(stats, 1), pg,
+    LMPB_OK_OR_THROW(lmpb_layer_norm_backward((int)x.type(), px, pw, mean, rstd, pg,
                                               (int64_t)x.numel() / f, f, dx.get(), dw.get(), db.get(), tensor::current_stream()));
     dx.add(), dw.add(), db.add();
   }
@@ -192,16 +192,23 @@ Variable layer_norm(const Variable& x, const Variable* weight, const Variable* b
   const void* px = ptr(x.data());
   const void* pw = weight ? ptr(weight->data()) : nullptr;
   const void* pb = bias ? ptr(bias->data()) : nullptr;
-  Tensor y = empty(s, dt);
-  const size_t rows = y.numel() / s.back();
+  size_t values = 1;
+  for (size_t n : s) values *= n;
+  const size_t rows = values / s.back(), size = dtype_size(dt), stats = rg ? 2 * rows * size : 0;
+  // The statistics go behind a small y, which then lives as long as they do, and save an allocation (1.5 of 17 us
+  // forward and backward); a large y does not have to.
+  const bool behind = values * size <= size_t(1) << 20;
+  Tensor y = empty(s, dt, behind ? stats : 0);
   auto fn = std::make_shared<LayerNormBackward>();
   if (rg) {
-    fn->stats = empty({2, rows}, dt);
+    fn->buffer = behind ? y.impl()->storage : tensor::make_storage(stats, DeviceType::CUDA);
+    fn->mean = static_cast<char*>(fn->buffer->ptr) + (behind ? values * size : 0);
+    fn->rstd = static_cast<char*>(fn->mean) + rows * size;
     fn->has_weight = weight != nullptr;
     fn->has_bias = bias != nullptr;
   }
-  LMPB_OK_OR_THROW(lmpb_layer_norm((int)dt, px, pw, pb, (int64_t)rows, (int64_t)s.back(), eps, ptr(y),
-                                   rg ? ptr(fn->stats) : nullptr, rg ? row_of(fn->stats, 1) : nullptr, tensor::current_stream()));
+  LMPB_OK_OR_THROW(lmpb_layer_norm((int)dt, px, pw, pb, (int64_t)rows, (int64_t)s.back(), eps, ptr(y), fn->mean, fn->rstd,
+                                   tensor::current_stream()));
   return output(y, rg, fn, std::move(in));
 }
 
