@@ -1,28 +1,35 @@
 // Causal attention over packed sequences on the B200 tensor cores, float32 in
 // and out: fp16 hi/lo split operands, tcgen05.mma, TMEM.
 //
-// fp32 accuracy.  A 128-row tile of q, k, v or grad is scaled by the power of
-// two that puts its largest magnitude into [2^14, 2^15) and each element x of
-// it becomes hi = fp16(x), lo = fp16(x - hi); a product of two operands is
-// the three MMAs lo.hi + hi.lo + hi.hi (lo.lo is 2^-22 of it).  hi and lo
-// together hold 22 bits of any x down to 2^-18 of the tile's maximum, and
-// 2^-40 of that maximum below.  Weights and their gradients are split the
-// same way on the fly, scaled by 2^14 (weights are at most 1) and by a bound
-// on the gradients' size.  The MMA's fp32 accumulator truncates, so nothing
-// accumulates in it for longer than one 128-row block: each block's product
-// is drained into registers, where the running sums round to nearest.
+// fp32 accuracy.  A 128-row tile of q, k or v, and each row of grad, is scaled
+// by the power of two that puts its largest magnitude into [2^14, 2^15) and
+// each element x of it becomes hi = fp16(x), lo = fp16(x - hi); a product of
+// two operands is the three MMAs lo.hi + hi.lo + hi.hi (lo.lo is 2^-22 of it).
+// hi and lo together hold 22 bits of any x down to 2^-18 of the tile's (row's)
+// maximum, and 2^-40 of that maximum below.  Weights and their gradients are
+// split the same way on the fly, under a scale for each row of the result that
+// they are summed into (see below).  The MMA's fp32 accumulator truncates, so
+// nothing accumulates in it for longer than one 128-row block: each block's
+// product is drained into registers, where the running sums round to nearest.
 //
-// Tiles whose values that cannot carry (infinities, NaN, rows over 2^18 apart,
-// magnitudes outside [2^-60, 2^40], q or k so long that a score may pass 2^14,
-// where the rounding of lse moves a weight by 2^-10) are flagged by the split; the fp32 kernels
-// of attention.cu then redo the sequences and head groups that hold one.
+// Gradients of a loss differ by many powers of two from row to row, and a
+// small row is not lost in a larger one: dq of a row depends on its own grad
+// alone, and a key may be seen by rows with a small grad only.  So grad has an
+// exponent a row; in dq it is that row's, and in dk, dv it joins the weights,
+// whose scale is then the largest of a key's row of them in the block.
+//
+// Tiles whose values that cannot carry (infinities, NaN, q, k or v with rows
+// over 2^18 apart or magnitudes below 2^-60, magnitudes over 2^40, q or k so
+// long that a score may pass 2^14, where the rounding of lse moves a weight by
+// 2^-10) are flagged by the split; the fp32 kernels of attention.cu then redo
+// the sequences and head groups that hold one.
 //
 // 1. Split pass: a CTA per tile and head plane writes the tile's hi and lo as
 //    one block in the very layout the MMAs read from shared memory (128-byte
 //    swizzled rows of 64 halves), so the kernels fetch operands with plain
 //    bulk copies, no tensor maps.  Tiles never span sequences and rows
 //    behind a sequence are 0.  For v and grad it also finds the largest row
-//    norm, for grad the row sums delta = sum(grad * out).
+//    norm, for grad the rows' exponents and the sums delta = sum(grad * out).
 // 2. forward_kernel, backward_kernel: one CTA per tile and head (dk and dv: per
 //    share of a key tile's work), one CTA per SM.  Warp 0 feeds a ring of
 //    parts (the hi or lo half of a block, 16 or 32 KB), warp 1 issues the MMAs,
@@ -77,11 +84,14 @@ __device__ __forceinline__ int first_tile(const int4& tile, int t) { return tile
 // heads, gradient heads; a plane's tile t is block plane * tiles + t.
 struct Split {
   unsigned char* blocks;
-  int* expo;             // the tile was scaled by 2^expo
-  float* norm;           // largest row norm (v, grad)
-  float* dmax;           // largest |delta| (grad)
+  int* expo;             // the tile was scaled by 2^expo (q, k, v)
+  float* norm;           // largest row norm (v; grad: of the scaled rows)
+  float* dmax;           // largest |delta| of the scaled rows (grad)
   unsigned char* flags;
+  int* row_expo;         // [heads, tokens]: grad's row was scaled by 2^row_expo; kZeroRow where it is 0
 };
+// Rows of grad below 2^-95 keep this scale and fewer bits: results are then about to underflow.
+constexpr int kMaxRowExpo = 110, kZeroRow = 127;
 
 // ------------------------------------------------------------ split pass
 
@@ -198,6 +208,16 @@ __global__ void __launch_bounds__(32 * split_warps<DP>(), 2048 / (64 * split_war
   for (int i = 0; i < STEPS; ++i)
     part[i] = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
   float mx = fold_rows<LANES>(part, lane, more), mn = mx > 0.f ? mx : INFINITY;
+  int er = 0;  // of row r1
+  if (is_g) {  // each row by its own power of two
+    er = min(row_exp(mx), kMaxRowExpo);
+    const float f = two_to(er);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const float s = __shfl_sync(0xffffffffu, f, sub * LANES + i * (LANES / 8));
+      v[i] = make_float4(v[i].x * s, v[i].y * s, v[i].z * s, v[i].w * s);
+    }
+  }
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) part[i] = v[i].x * v[i].x + v[i].y * v[i].y + v[i].z * v[i].z + v[i].w * v[i].w;
   float nrm = fold_rows<LANES>(part, lane, sum), dmx = 0.f;
@@ -211,7 +231,11 @@ __global__ void __launch_bounds__(32 * split_warps<DP>(), 2048 / (64 * split_war
     const float d = fold_rows<LANES>(part, lane, sum);
     dmx = fabsf(d);
     bad |= !(dmx < INFINITY);
-    if (lane % (LANES / 8) == 0 && r1 < rows) delta[(int64_t)head * a.tokens + first + r1] = d;
+    if (lane % (LANES / 8) == 0 && r1 < rows) {
+      const int64_t at = (int64_t)head * a.tokens + first + r1;
+      delta[at] = d * two_to(-er);
+      o.row_expo[at] = mx > 0.f ? er : kZeroRow;
+    }
   }
   __shared__ float red[4][WARPS];
 #pragma unroll
@@ -230,11 +254,10 @@ __global__ void __launch_bounds__(32 * split_warps<DP>(), 2048 / (64 * split_war
     nrm = fmaxf(nrm, red[2][w]);
     dmx = fmaxf(dmx, red[3][w]);
   }
-  // a gradient's small rows only ever add to larger sums: no limit on their range
-  const bool range = mx > 0.f && (mx > 0x1p40f || mx < 0x1p-60f || (!is_g && mn < mx * 0x1p-18f));
+  const bool range = mx > 0x1p40f || (!is_g && mx > 0.f && (mx < 0x1p-60f || mn < mx * 0x1p-18f));
   const bool far = !is_v && !is_g && !(nrm * a.scale <= 0x1p14f);  // so |q| |k| scale <= 2^14 of unflagged tiles
   const bool flag = bads || range || far;
-  const int e = flag ? 0 : row_exp(mx);
+  const int e = flag || is_g ? 0 : row_exp(mx);
   const int64_t block = plane * a.tiles + t;
   if (threadIdx.x == 0) {
     o.expo[block] = e;
@@ -539,7 +562,7 @@ constexpr int backward_ring() { return DP == 64 ? 8 : 3; }
 template <int DP>
 using ForwardLayout = Layout<DP, 1, forward_ring<DP>(), 2 * WarpsOf<DP>::kParts * 128 * 4>;
 template <int DP>
-using BackwardLayout = Layout<DP, 2, backward_ring<DP>(), 2048>;
+using BackwardLayout = Layout<DP, 2, backward_ring<DP>(), 5 * 128 * 4>;
 
 // Sets up the barriers and all of TMEM, then waits for the kernel ahead; every thread calls it.  False (for
 // all) when the shared memory does not start on a swizzle atom.
@@ -799,19 +822,24 @@ __global__ void __launch_bounds__(WarpsOf<DP>::kThreads, 1) forward_kernel(const
 
 // ------------------------------------------------------------ backward
 //
-// dS of a block is split into fp16 under a power of two chosen for the block
-// from a bound on its values: |dP_ij| <= |grad_i| |v_j| and P <= 1, so
-// |dS_ij| <= max|grad_i| max|v_j| + max|delta_i| over the block's rows.
+// Below, grad and delta are those of the scaled rows, 2^row_expo times the real
+// ones.  |dP_ij| <= |grad_i| |v_j|, so with a weight W_ij <= 1 in place of P
+// |W (dP - delta)| <= max|grad_i| max|v_j| + |delta_i|, which gives the power
+// of two under which it is split into fp16.
+//   dq: W = P, and delta is the row's own; the row's 2^-row_expo is left to the end.
+//   dk, dv: W_ij = P_ij 2^(-row_expo_i - M_j), M_j the exponent of the power of two at or
+//   above the largest P_ij 2^-row_expo_i of key j in the block.  W is dv's
+//   operand and the row of dS's; each block's product is drained times 2^M_j.
 
 struct DsScale {
   int e;        // dS enters the MMA times 2^e
-  float dp, d;  // dS 2^e = P (dp * dP' - d * delta), dP' the scaled operands' product
+  float dp, d;  // dS 2^e = W (dp * dP' - d * delta), dP' the scaled operands' product
 };
 
-__device__ __forceinline__ DsScale ds_scale(float gnorm, float vnorm, float dmax, int eg, int ev, float weight_bits) {
+__device__ __forceinline__ DsScale ds_scale(float gnorm, float vnorm, float dmax, int ev, float weight_bits) {
   DsScale s;
   s.e = min(100, row_exp(fmaf(gnorm, vnorm, dmax)));
-  s.dp = ldexpf(1.f, s.e - eg - ev - (int)weight_bits);
+  s.dp = ldexpf(1.f, s.e - ev - (int)weight_bits);
   s.d = ldexpf(1.f, s.e - (int)weight_bits);
   return s;
 }
@@ -898,9 +926,11 @@ __device__ __forceinline__ void dq_tile(const AttentionArgs& a, const Split& sp,
     const int row = tile.z * kTileRows + me.row;
     const int64_t at = (int64_t)head * a.tokens + tile.x + row;
     const float lse = row < tile.y ? a.lse[at] : INFINITY;  // rows behind the sequence: no weight
-    const float delta = row < tile.y ? a.delta[at] : 0.f;
-    const int eq = sp.expo[qblock], eg = sp.expo[gblock];
-    const float gnorm = sp.norm[gblock], dmax = sp.dmax[gblock];
+    int eg = row < tile.y ? sp.row_expo[at] : kZeroRow;
+    if (eg == kZeroRow) eg = 0;
+    const float delta = row < tile.y ? a.delta[at] * two_to(eg) : 0.f;
+    const int eq = sp.expo[qblock];
+    const float gnorm = sp.norm[gblock];
     int ek = sp.expo[kplane], ev = sp.expo[vplane];
     float vnorm = sp.norm[vplane];
     const int low = a.low_of(tile, me.row), col0 = me.part * COLS - low;
@@ -909,8 +939,8 @@ __device__ __forceinline__ void dq_tile(const AttentionArgs& a, const Split& sp,
     const auto block = [&](int j, auto diagonal) {
       constexpr bool diag = decltype(diagonal)::value;
       const float c = ldexpf(a.scale * kLog2e, -(eq + ek));
-      const DsScale ds = ds_scale(gnorm, vnorm, dmax, eg, ev, 0.f);
-      const float f = ldexpf(a.scale, -(ds.e + ek)), dd = delta * ds.d;
+      const DsScale ds = ds_scale(gnorm, vnorm, fabsf(delta), ev, 0.f);
+      const float f = ldexpf(a.scale, -(ds.e + eg + ek)), dd = delta * ds.d;
       if (j + 1 < n) ek = sp.expo[kplane + j + 1], ev = sp.expo[vplane + j + 1], vnorm = sp.norm[vplane + j + 1];
       const uint32_t s = own + (j & 1) * 128, dp = own + 256;
       warp_wait(wait, spfull, j & 1);
@@ -955,6 +985,11 @@ __device__ __forceinline__ void dq_tile(const AttentionArgs& a, const Split& sp,
   teardown(tmem);
 }
 
+// Shares of a key tile whose head has `per_head` query blocks; a.splits at most.
+__device__ __forceinline__ int shares_of(const AttentionArgs& a, int per_head) {
+  return min(a.splits, (per_head * (a.heads / a.kv_heads) + a.share - 1) / a.share);
+}
+
 // dk and dv of one key tile and key/value head, over the group's query heads
 // and their tiles from the diagonal on: one list of blocks, cut into shares of
 // about a.share blocks.  Where a tile has more than one share, their results
@@ -966,11 +1001,6 @@ __device__ __forceinline__ void dq_tile(const AttentionArgs& a, const Split& sp,
 // dv, dk: weights are computed under dP, dS under dv.
 //
 // Both running sums are held in registers, 2 x DP / 2 a thread.
-// Shares of a key tile whose head has `per_head` query blocks; a.splits at most.
-__device__ __forceinline__ int shares_of(const AttentionArgs& a, int per_head) {
-  return min(a.splits, (per_head * (a.heads / a.kv_heads) + a.share - 1) / a.share);
-}
-
 template <int DP>
 __device__ __forceinline__ void dkv_tile(const AttentionArgs& a, const Split& sp, int cta, bool vec_out) {
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -980,7 +1010,8 @@ __device__ __forceinline__ void dkv_tile(const AttentionArgs& a, const Split& sp
   constexpr int RING = backward_ring<DP>();
   const uint32_t base = smem_u32(smem), bars = base + L::kBarsAt;
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + L::kBarsAt + kBars * 8);
-  float* stat = reinterpret_cast<float*>(smem + L::kScratch);  // [2][2][128]: weight offset, -scaled delta
+  // of the block's queries [128] each: -lse, -lse - row_expo, 2^-row_expo; then of even and odd blocks: -scaled delta
+  float* const stat = reinterpret_cast<float*>(smem + L::kScratch);
   const int per_order = a.kv_heads * a.splits, order = cta / per_order, kv_head = cta % per_order / a.splits;
   const int split = cta % a.splits, group = a.heads / a.kv_heads;
   const int t = a.by_keys[order];
@@ -1066,30 +1097,69 @@ __device__ __forceinline__ void dkv_tile(const AttentionArgs& a, const Split& sp
     const int col0 = me.part * COLS - me.row;
     const unsigned span = a.high_of(tile, me.row) - me.row;
     const uint32_t own = tmem + me.lanes + me.part * COLS, oown = tmem + 256 + me.lanes + me.part * C;
-    // one value of the next block's row statistics a thread: lse (first half) or delta
+    // the next block's row statistics, a query a thread: lse (first half) or delta, and the exponent
     const int tid = threadIdx.x - 128;
     const float* source = tid < 128 ? a.lse : a.delta;
+    float next = 0.f;
+    int enext = kZeroRow;
     const auto fetch = [&](const Walk& w) {
       const int r = (tile.z + w.x) * kTileRows + (tid & 127);
-      return tid < 256 && r < tile.y ? source[(int64_t)w.head * a.tokens + tile.x + r] : tid < 128 ? INFINITY : 0.f;
+      const bool in = tid < 256 && r < tile.y;
+      const int64_t from = (int64_t)w.head * a.tokens + tile.x + r;
+      next = in ? source[from] : 0.f;
+      enext = in ? sp.row_expo[from] : kZeroRow;
     };
     Walk at = begin, ahead = begin;
-    float next = fetch(ahead);
+    fetch(ahead);
     for (int i = 0; i < n; ++i, at.next()) {
       const int64_t qb = qblock(at), gb = qb + gplanes;
-      const int eq = sp.expo[qb], eg = sp.expo[gb];
+      const int eq = sp.expo[qb];
       const float c = ldexpf(a.scale * kLog2e, -(eq + ek));
-      const DsScale ds = ds_scale(sp.norm[gb], vnorm, sp.dmax[gb], eg, ev, kWeightBits);
-      float* st = stat + (i & 1) * 256;
-      if (tid < 256) st[tid] = tid < 128 ? kWeightBits - next : -next * ds.d;
+      const DsScale ds = ds_scale(sp.norm[gb], vnorm, sp.dmax[gb], ev, kWeightBits);
+      // All warps are past the last block's weights (vfull was waited for, which
+      // their arrival at pfull precedes), so only delta has two buffers.
+      float* const st = stat + 384 + (i & 1) * 128;
+      if (tid < 128) {  // a gradient of 0, or no query: no weight
+        const bool none = enext == kZeroRow;
+        stat[tid] = none ? -INFINITY : -next;
+        stat[128 + tid] = none ? -INFINITY : -next - (float)enext;
+        stat[256 + tid] = none ? 0.f : two_to(-enext);
+      } else if (tid < 256) {
+        st[tid - 128] = enext == kZeroRow ? 0.f : -(next * two_to(enext)) * ds.d;
+      }
       compute_sync<WARPS>();
       ahead.next();
-      if (i + 1 < n) next = fetch(ahead);
+      if (i + 1 < n) fetch(ahead);
       const bool diag = at.x == 0;
-      const float4* bias = reinterpret_cast<const float4*>(st + me.part * COLS);
-      const float4* dd = reinterpret_cast<const float4*>(st + 128 + me.part * COLS);
+      const float4* bias = reinterpret_cast<const float4*>(stat + me.part * COLS);
+      const float4* dd = reinterpret_cast<const float4*>(st + me.part * COLS);
+      // the other block's delta is done with: here the parts of a row tell each other their M
+      signed char* const xch = reinterpret_cast<signed char*>(stat + 384 + (~i & 1) * 128) + 4 * me.row;
+      int top = 0;  // M of this thread's key
       warp_wait(wait, sfull, i & 1);
       const auto weights = [&](auto diagonal) {
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int k = 0; k < COLS; k += 16) {
+          uint32_t r[16];
+          tmem_ld16(own + k, r);
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            const float4 b = bias[32 + (k + j) / 4];
+            const float2 x[2] = {fma2(bits2(r[j], r[j + 1]), Two(c), Two(b.x, b.y)).get(),
+                                 fma2(bits2(r[j + 2], r[j + 3]), Two(c), Two(b.z, b.w)).get()};
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              if (!decltype(diagonal)::value || unsigned(col0 + k + j + 2 * y) < span) mx = fmaxf(mx, x[y].x);
+              if (!decltype(diagonal)::value || unsigned(col0 + k + j + 2 * y + 1) < span) mx = fmaxf(mx, x[y].y);
+            }
+          }
+        }
+        xch[me.part] = (signed char)(int)fminf(fmaxf(ceilf(mx), -112.f), 112.f);  // none, or next to nothing: -112
+        compute_sync<WARPS>();
+        top = max((int)xch[0], (int)xch[1]);
+        if (PARTS == 4) top = max(top, max((int)xch[2], (int)xch[3]));
+        const Two f(two_to((int)kWeightBits - top));
 #pragma unroll
         for (int k = 0; k < COLS; k += 16) {
           uint32_t r[16], w[16];
@@ -1098,9 +1168,9 @@ __device__ __forceinline__ void dkv_tile(const AttentionArgs& a, const Split& sp
           tmem_regs_ready(r);
 #pragma unroll
           for (int j = 0; j < 16; j += 4) {
-            const float4 b = bias[(k + j) / 4];
-            Two p[2] = {exp2_fast(fma2(bits2(r[j], r[j + 1]), Two(c), Two(b.x, b.y))),
-                        exp2_fast(fma2(bits2(r[j + 2], r[j + 3]), Two(c), Two(b.z, b.w)))};
+            const float4 b = bias[(k + j) / 4], g = bias[64 + (k + j) / 4];
+            Two p[2] = {mul2(mul2(exp2_fast(fma2(bits2(r[j], r[j + 1]), Two(c), Two(b.x, b.y))), Two(g.x, g.y)), f),
+                        mul2(mul2(exp2_fast(fma2(bits2(r[j + 2], r[j + 3]), Two(c), Two(b.z, b.w))), Two(g.z, g.w)), f)};
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               if (decltype(diagonal)::value) {
@@ -1150,9 +1220,9 @@ __device__ __forceinline__ void dkv_tile(const AttentionArgs& a, const Split& sp
       tmem_st_wait();
       warp_arrive(dsfull);
       warp_wait(wait, vfull, i & 1);
-      drain<C, false>(oown, dv, 1.f, two_to(-(int)kWeightBits - eg));
+      drain<C, false>(oown, dv, 1.f, two_to(top - (int)kWeightBits));
       warp_arrive(vempty);
-      fk = ldexpf(a.scale, -(ds.e + eq));
+      fk = ldexpf(a.scale, top - (ds.e + eq));
     }
     warp_wait(wait, kfull, (n - 1) & 1);
     drain<C, false>(oown + 128, dk, 1.f, fk);
@@ -1225,9 +1295,9 @@ lmpb_status make_split(AttentionArgs& a, bool backward, int dp, Split& s, float*
   auto up = [](size_t b) { return (b + 255) / 256 * 256; };
   const size_t planes = (size_t)(backward ? 2 : 1) * a.heads + 2 * a.kv_heads, n = planes * a.tiles;
   const size_t blocks = n * (dp == 64 ? block_bytes<64>() : block_bytes<128>());
-  const size_t dbytes = backward ? up((size_t)a.tokens * a.heads * 4) : 0;
+  const size_t dbytes = backward ? up((size_t)a.tokens * a.heads * 4) : 0;  // of delta, and of the rows' exponents
   const size_t pbytes = a.splits > 1 ? (size_t)a.splits * 2 * a.tokens * a.kv_heads * a.dim * 4 : 0;
-  LMPB_CUDA_TRY(stream_alloc(ws, blocks + 3 * up(4 * n) + up(n) + dbytes + pbytes, st));
+  LMPB_CUDA_TRY(stream_alloc(ws, blocks + 3 * up(4 * n) + up(n) + 2 * dbytes + pbytes, st));
   unsigned char* p = static_cast<unsigned char*>(*ws);
   s.blocks = p;
   s.expo = reinterpret_cast<int*>(p + blocks);
@@ -1235,7 +1305,8 @@ lmpb_status make_split(AttentionArgs& a, bool backward, int dp, Split& s, float*
   s.dmax = reinterpret_cast<float*>(p + blocks + 2 * up(4 * n));
   s.flags = p + blocks + 3 * up(4 * n);
   *delta = reinterpret_cast<float*>(s.flags + up(n));
-  if (pbytes) a.part = reinterpret_cast<float*>(s.flags + up(n) + dbytes);
+  s.row_expo = reinterpret_cast<int*>(s.flags + up(n) + dbytes);
+  if (pbytes) a.part = reinterpret_cast<float*>(s.flags + up(n) + 2 * dbytes);
   return LMPB_OK;
 }
 

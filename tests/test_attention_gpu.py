@@ -136,6 +136,160 @@ def test_forward_and_backward(cuda, case):
             assert np.linalg.norm(got[name] - ref[name][0]) <= 2.0 ** (-18 if name == "out" else -17) * norm, name
 
 
+def _rows_reference(torch, x, lengths, scale):
+    """As _reference, for gradients whose rows differ in size: what is left
+    where terms are tiny counts against the largest term of the result's own
+    row, not of its sequence or tile.
+
+    A row of grad has its own scale, its largest value g* at 2^14 or more, so
+    its parts are within 2^-39 g* (FLOOR).  Scaled rows are at most 2^15
+    sqrt(D) long and dP - delta of them at most 2^15 R with R = sqrt(D) max|v| +
+    max(|delta| / g*).  dq: a row's bound is then 2 sqrt(D) g* max|v| + |delta|,
+    and dS is within 2^-39 of it.  dk, dv: the weights of key j, P_ij over the
+    scale of row i, are scaled to have the largest between 2^13 and 2^14, so
+    with T_j = max(P_ij g*_i) a step of 2^-25 is at most
+    2^-25 2 T_j / 2^28 of a weight: 2^-37 T_j sum(|g| / g*) of dv, and with dS's
+    own step as much again times R, 2^-36 T_j R of dS.  T_j counts as 2^-98 at
+    least (the scale ends at 2^112)."""
+    x = {n: a.cuda().double() for n, a in x.items()}
+    q, k, v, g = (x[n] for n in "qkvg")
+    hq, d, hkv = q.shape[1], q.shape[2], k.shape[1]
+    zero = lambda a: [torch.zeros_like(a), torch.zeros_like(a)]  # noqa: E731
+    out = {"dq": zero(q), "dk": zero(k), "dv": zero(v)}
+    w = 2.0 ** -22
+    top = {n: float(x[n].abs().max()) for n in "qkv"}
+    vnorm = float(v.norm(dim=2).max())
+    start, parts = 0, []
+    for n in lengths:
+        rows = slice(start, start + n)
+        start += n
+        for h in range(hq if n else 0):
+            j = h * hkv // hq
+            Q, K, V, G = q[rows, h], k[rows, j], v[rows, j], g[rows, h]
+            mask = torch.ones(n, n, dtype=torch.bool, device="cuda").tril()
+            S = (scale * Q @ K.T).masked_fill(~mask, -math.inf)
+            lse = torch.logsumexp(S, 1, keepdim=True)
+            P = torch.exp(S - lse)
+            O = P @ V
+            delta = (G * O).sum(1, keepdim=True)
+            big = G.abs().amax(1, keepdim=True)
+            parts.append((rows, h, j, Q, K, V, G, mask, S, lse, P, O, delta, big))
+    ratio = max(float((p[-2].abs() / p[-1].clamp_min(1e-300)).max()) for p in parts)
+    R = math.sqrt(d) * vnorm + ratio
+    for rows, h, j, Q, K, V, G, mask, S, lse, P, O, delta, big in parts:
+        n = len(Q)
+        g1, v1, k1, q1 = (a.abs().sum(1) for a in (G, V, K, Q))
+        E = (3 + d / 2) * w * scale * (Q.abs() @ K.abs().T) + scale * FLOOR * (top["k"] * q1[:, None] + top["q"] * k1)
+        rel = 2 * E.masked_fill(~mask, 0).amax(1, keepdim=True) + w * (lse.abs() / 2 + 2)
+        sums, seen = (3 + n / 2) * w, mask.double()
+        dP = G @ V.T
+        dS = P * (dP - delta)
+        size = (G.abs() @ V.abs().T) + (G.abs() * (P @ V.abs())).sum(1, keepdim=True)
+        dSm = P * size
+        dSt = (rel + (3 + d / 2) * w + sums) * dSm + rel * dS.abs()
+        dSt = dSt + P * FLOOR * (2 * top["v"] * g1[:, None] + big * v1 + G.abs() @ V.abs().sum(0)[:, None])
+        own = FLOOR * (2 * math.sqrt(d) * big * vnorm + delta.abs()) * seen
+        T = (P * big).amax(0).clamp_min(2.0 ** -98)
+        key = 2.0 ** -36 * R * T * seen
+        unit = G.abs() / big.clamp_min(1e-300)
+        out["dq"][0][rows, h] = scale * dS @ K
+        out["dq"][1][rows, h] = scale * ((dSt + own) @ K.abs() + sums * (dSm @ K.abs()) + FLOOR * top["k"] * dSm.sum(1, keepdim=True))
+        out["dk"][0][rows, j] += scale * dS.T @ Q
+        out["dk"][1][rows, j] += scale * ((dSt + key).T @ Q.abs() + sums * (dSm.T @ Q.abs()) + FLOOR * top["q"] * dSm.sum(0)[:, None])
+        out["dv"][0][rows, j] += P.T @ G
+        out["dv"][1][rows, j] += (rel * P).T @ G.abs() + sums * (P.T @ G.abs())
+        out["dv"][1][rows, j] += 2.0 ** -37 * T[:, None] * (seen.T @ unit) + FLOOR * (P.T @ big)
+    return {n: (a.cpu().numpy(), b.cpu().numpy()) for n, (a, b) in out.items()}
+
+
+@pytest.mark.parametrize("case", [([300], 2, 1, 64, 0), ([300], 2, 2, 128, 0), ([2049], 1, 1, 64, 0),
+                                  ([1000, 64, 64, 40, 40, 7], 2, 1, 33, 0), ([40] * 6 + [600], 4, 2, 96, 3)],
+                         ids=lambda c: "%s-%d" % ("_".join(map(str, c[0][:3])), c[3]))
+@pytest.mark.parametrize("bits", [8, 14, 20, 26, 40, 80])
+@pytest.mark.parametrize("where", ["every other row", "every other sequence", "few large rows"])
+def test_rows_with_small_gradients(cuda, case, bits, where):
+    """A row whose gradient is far below its neighbours' keeps its own accuracy, alone and where sequences share a tile."""
+    if where == "every other sequence" and len(case[0]) == 1:
+        pytest.skip("one sequence")
+    lengths, hq, _, d, tail = case
+    x = _inputs(cuda, np.random.default_rng(bits + d), case)
+    t = sum(lengths)
+    if where == "every other row":
+        small = np.arange(t) % 2 == 1
+    elif where == "few large rows":
+        small = np.arange(t) % 50 != 20
+    else:
+        small = np.concatenate([np.full(n, i % 2 == 1) for i, n in enumerate(lengths)])
+    x["g"][:t][cuda.from_numpy(small)] *= 2.0 ** -bits
+    got = _gradients(cuda, x, lengths)
+    ref = _rows_reference(cuda, {n: a[:t] for n, a in x.items()}, lengths, 1 / math.sqrt(d))
+    for name in ("dq", "dk", "dv"):
+        _check(name, got[name][:t], ref[name])
+        assert not got[name][t:].any()
+    for rows in (small, ~small):  # the bar of test_forward_and_backward, for each size of its own
+        err, value = (got["dq"][:t] - ref["dq"][0])[rows], ref["dq"][0][rows]
+        assert np.linalg.norm(err) <= 2.0 ** -17 * np.linalg.norm(value)
+    if where == "every other sequence":
+        for name in ("dk", "dv"):
+            err, value = (got[name][:t] - ref[name][0])[small], ref[name][0][small]
+            assert np.linalg.norm(err) <= 2.0 ** -17 * np.linalg.norm(value), name
+
+
+def _gradients(torch, x, lengths, scale=None):
+    import rushlite_b200 as rsl
+
+    return _run(rsl, x, lengths, scale)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_sequences_of_very_different_gradients_share_a_tile(cuda, dim):
+    lengths = [31, 30, 33, 34, 200]
+    x = _inputs(cuda, np.random.default_rng(3 + dim), (lengths, 2, 1, dim, 0))
+    start = 0
+    for n, f in zip(lengths, (1.0, 1e-6, 1e-10, 1e-13, 1e-20)):
+        x["g"][start:start + n] *= f
+        start += n
+    got = _gradients(cuda, x, lengths)
+    ref = _rows_reference(cuda, x, lengths, 1 / math.sqrt(dim))
+    start = 0
+    for name in ("dq", "dk", "dv"):
+        _check(name, got[name], ref[name])
+    for n in lengths:
+        rows = slice(start, start + n)
+        start += n
+        for name in ("dq", "dk", "dv"):
+            value = ref[name][0][rows]
+            assert np.linalg.norm(got[name][rows] - value) <= 2.0 ** -17 * np.linalg.norm(value), (name, n)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("bits", [0, 20, 40])
+def test_small_gradients_with_sharp_weights(cuda, dim, bits):
+    """Scores with a deviation of 8 and more: keys that hardly a row looks at, seen by rows with large and small gradients."""
+    lengths = [500, 60, 60]
+    x = _inputs(cuda, np.random.default_rng(5 + dim), (lengths, 2, 1, dim, 0))
+    x["g"][::2] *= 2.0 ** -bits
+    got = _gradients(cuda, x, lengths, 1.0)
+    ref = _rows_reference(cuda, x, lengths, 1.0)
+    for name in ("dq", "dk", "dv"):
+        _check(name, got[name], ref[name])
+
+
+def test_rows_without_a_gradient(cuda):
+    """Rows that a loss leaves out: their dq is 0, and they change nobody's results."""
+    lengths = [200, 50, 60]
+    x = _inputs(cuda, np.random.default_rng(6), (lengths, 2, 1, 64, 0))
+    x["g"] *= 1e-12
+    out = np.arange(310) % 3 != 0
+    x["g"][cuda.from_numpy(out)] = 0
+    x["g"][250:] = 0  # a whole sequence
+    got = _gradients(cuda, x, lengths)
+    ref = _rows_reference(cuda, x, lengths, 1 / 8)
+    for name in ("dq", "dk", "dv"):
+        _check(name, got[name], ref[name])
+    assert not got["dq"][out].any() and not got["dk"][250:].any() and not got["dv"][250:].any()
+
+
 @pytest.mark.parametrize("scale", [1e-3, 0.7, 3.0])
 def test_scale(cuda, scale):
     import rushlite_b200 as rsl
