@@ -16,13 +16,16 @@
 // small row is not lost in a larger one: dq of a row depends on its own grad
 // alone, and a key may be seen by rows with a small grad only.  So grad has an
 // exponent a row; in dq it is that row's, and in dk, dv it joins the weights,
-// whose scale is then the largest of a key's row of them in the block.
+// whose scale is then the largest of a key's row of them in the block.  In the
+// forward and in dq, too, a row's weights are scaled by their largest in the
+// block: next to values far apart a small weight counts as much as a large one.
 //
 // Tiles whose values that cannot carry (infinities, NaN, q, k or v with rows
 // over 2^18 apart or magnitudes below 2^-60, magnitudes over 2^40, q or k so
 // long that a score may pass 2^14, where the rounding of lse moves a weight by
-// 2^-10) are flagged by the split; the fp32 kernels of attention.cu then redo
-// the sequences and head groups that hold one.
+// 2^-10; in the backward also outputs over 2^18 above a tile of v that their
+// rows see) are flagged by the split and the backward; the fp32 kernels of
+// attention.cu then redo the sequences and head groups that hold one.
 //
 // 1. Split pass: a CTA per tile and head plane writes the tile's hi and lo as
 //    one block in the very layout the MMAs read from shared memory (128-byte
@@ -772,8 +775,10 @@ __global__ void __launch_bounds__(WarpsOf<DP>::kThreads, 1) forward_kernel(const
       compute_sync<WARPS>();
 #pragma unroll
       for (int k = 0; k < PARTS; ++k) mx = fmaxf(mx, x[k * 128]);
-      const float mn = fmaxf(m, mx * c);  // finite: every row sees a key of every block
-      const float next = exp2_fast(m - mn), bias = kWeightBits - mn;
+      // The weights are split relative to the block's own largest (finite: every row sees a key of every block):
+      // relative to the row's, those of a block of large v but small weights would lose their bits.
+      const float mb = mx * c, mn = fmaxf(m, mb), next = exp2_fast(m - mn), up = exp2_fast(mb - mn);
+      const float bias = kWeightBits - mb;
       Two sums(0.f);
 #pragma unroll 2
       for (int k = 0; k < COLS; k += 16) {
@@ -795,11 +800,11 @@ __global__ void __launch_bounds__(WarpsOf<DP>::kThreads, 1) forward_kernel(const
       }
       tmem_st_wait();
       warp_arrive(pfull);
-      l = l * next + (sums.get().x + sums.get().y);
+      l = l * next + (sums.get().x + sums.get().y) * up;
       m = mn;
       if (j > 0) drain_block(j - 1);
       alpha = next;
-      of = f;
+      of = f * up;
     };
     for (int j = 0; j + 1 < n; ++j) block(j, std::false_type{});
     block(n - 1, std::true_type{});
@@ -826,7 +831,9 @@ __global__ void __launch_bounds__(WarpsOf<DP>::kThreads, 1) forward_kernel(const
 // ones.  |dP_ij| <= |grad_i| |v_j|, so with a weight W_ij <= 1 in place of P
 // |W (dP - delta)| <= max|grad_i| max|v_j| + |delta_i|, which gives the power
 // of two under which it is split into fp16.
-//   dq: W = P, and delta is the row's own; the row's 2^-row_expo is left to the end.
+//   dq: W_ij = P_ij 2^-M_i, M_i the exponent of the power of two at or above the largest
+//   P_ij of row i in the block, and delta is the row's own; each block's product
+//   is drained times 2^(M_i - row_expo_i).
 //   dk, dv: W_ij = P_ij 2^(-row_expo_i - M_j), M_j the exponent of the power of two at or
 //   above the largest P_ij 2^-row_expo_i of key j in the block.  W is dv's
 //   operand and the row of dS's; each block's product is drained times 2^M_j.
@@ -936,14 +943,31 @@ __device__ __forceinline__ void dq_tile(const AttentionArgs& a, const Split& sp,
     const int low = a.low_of(tile, me.row), col0 = me.part * COLS - low;
     const unsigned span = me.row - low + 1;
     const uint32_t own = tmem + me.lanes + me.part * COLS, oown = tmem + 384 + me.lanes + me.part * C;
+    float* xch = reinterpret_cast<float*>(smem + L::kScratch) + me.row;  // [PARTS][128]
     const auto block = [&](int j, auto diagonal) {
       constexpr bool diag = decltype(diagonal)::value;
       const float c = ldexpf(a.scale * kLog2e, -(eq + ek));
       const DsScale ds = ds_scale(gnorm, vnorm, fabsf(delta), ev, 0.f);
-      const float f = ldexpf(a.scale, -(ds.e + eg + ek)), dd = delta * ds.d;
+      const float dd = delta * ds.d;
+      const int expo = ds.e + eg + ek;
       if (j + 1 < n) ek = sp.expo[kplane + j + 1], ev = sp.expo[vplane + j + 1], vnorm = sp.norm[vplane + j + 1];
       const uint32_t s = own + (j & 1) * 128, dp = own + 256;
       warp_wait(wait, spfull, j & 1);
+      float mx = -INFINITY;
+#pragma unroll 1
+      for (int k = 0; k < COLS; k += 16) {
+        uint32_t r[16];
+        tmem_ld16(s + k, r);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (!diag || unsigned(col0 + k + i) < span) mx = fmaxf(mx, __uint_as_float(r[i]));
+      }
+      xch[me.part * 128] = mx;  // all warps have read the last block's: dP, which spfull tells of, is written after their dsfull
+      compute_sync<WARPS>();
+#pragma unroll
+      for (int k = 0; k < PARTS; ++k) mx = fmaxf(mx, xch[k * 128]);
+      const float top = fminf(fmaxf(ceilf(fmaf(mx, c, -lse)), -112.f), 112.f), bias = -lse - top;
+      const float f = ldexpf(a.scale, (int)top - expo);
 #pragma unroll
       for (int k = 0; k < COLS; k += 16) {
         uint32_t r[16], u[16], w[16];
@@ -954,7 +978,7 @@ __device__ __forceinline__ void dq_tile(const AttentionArgs& a, const Split& sp,
         tmem_regs_ready(u);
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          const Two p = exp2_fast(fma2(bits2(r[i], r[i + 1]), Two(c), Two(-lse)));
+          const Two p = exp2_fast(fma2(bits2(r[i], r[i + 1]), Two(c), Two(bias)));
           Two d = mul2(p, fma2(bits2(u[i], u[i + 1]), Two(ds.dp), Two(-dd)));
           if (diag) {
             float2 q = d.get();
@@ -1081,6 +1105,17 @@ __device__ __forceinline__ void dkv_tile(const AttentionArgs& a, const Split& sp
       Waiter last(33);
       commit(done);
       last(done, 0);
+    } else if (warp == 2) {
+      // dS has one bound for all queries of a block.  Where it comes from outputs, and deltas, far above
+      // these keys' v, a query with a small delta could lose its bits: a case for the fp32 kernels.
+      const float vnorm = sp.norm[vblock];
+      bool far = false;
+#pragma unroll 1
+      for (int i = threadIdx.x & 31; i < n; i += 32) {
+        const int64_t gb = (int64_t)(kv_head * group + (first + i) / per_head) * a.tiles + t + (first + i) % per_head + gplanes;
+        far |= sp.dmax[gb] > 0x1p18f * sp.norm[gb] * vnorm;
+      }
+      if (far) sp.flags[kblock] = 1;
     }
   } else {
     W::many();

@@ -275,6 +275,84 @@ def test_small_gradients_with_sharp_weights(cuda, dim, bits):
         _check(name, got[name], ref[name])
 
 
+def _tiles_reference(torch, x, scale):
+    """_rows_reference for one sequence whose 128-row tiles differ in size: what
+    is left where terms are tiny counts against the largest term of the
+    result's row in the same tile of keys (of queries, for dk and dv), 2^-39
+    of it and for powers of two between twice that."""
+    x = {n: a.cuda().double() for n, a in x.items()}
+    Q, K, V, G = (x[n][:, 0] for n in "qkvg")
+    n, d = Q.shape
+    w, sums = 2.0 ** -22, (3 + n / 2) * 2.0 ** -22
+    tiles = [slice(b, min(b + 128, n)) for b in range(0, n, 128)]
+    mask = torch.ones(n, n, dtype=torch.bool, device="cuda").tril()
+    S = (scale * Q @ K.T).masked_fill(~mask, -math.inf)
+    lse = torch.logsumexp(S, 1, keepdim=True)
+    P = torch.exp(S - lse)
+    O, dP = P @ V, G @ V.T
+    delta = (G * O).sum(1, keepdim=True)
+    dS = P * (dP - delta)
+    big = G.abs().amax(1, keepdim=True)
+    full = lambda: torch.zeros(n, n, dtype=torch.float64, device="cuda")  # noqa: E731
+    e, own, key, wrow, wcol, parts = full(), full(), full(), full(), full(), full()
+    for c in tiles:
+        kt, vt, vn = float(K[c].abs().max()), float(V[c].abs().max()), float(V[c].norm(dim=1).max())
+        top = P[:, c].amax(1, keepdim=True)
+        e[:, c] = FLOOR * kt * Q.abs().sum(1)[:, None]
+        wrow[:, c] = FLOOR * top
+        own[:, c] = 2 * FLOOR * top * (2 * math.sqrt(d) * big * vn + delta.abs())
+        parts[:, c] = FLOOR * (vt * G.abs().sum(1)[:, None] + big * V[c].abs().sum(1))
+        for r in tiles:
+            e[r, c] += FLOOR * float(Q[r].abs().max()) * K[c].abs().sum(1)
+            ratio = float((delta[r].abs() / big[r]).max())
+            T = (P[r, c] * big[r]).amax(0)
+            wcol[r, c] = 2.0 ** -37 * T
+            if ratio <= 2.0 ** 19 * math.sqrt(d) * vn:  # else the fp32 kernels' result
+                key[r, c] = 2.0 ** -36 * (math.sqrt(d) * vn + ratio) * T
+    E = (3 + d / 2) * w * scale * (Q.abs() @ K.abs().T) + scale * e
+    rel = 2 * E.masked_fill(~mask, 0).amax(1, keepdim=True) + w * (lse.abs() / 2 + 2)
+    seen = mask.double()
+    size = (G.abs() @ V.abs().T) + (G.abs() * (P @ V.abs())).sum(1, keepdim=True)
+    tv, tk, tq = (torch.cat([a[b].abs().max().expand(b.stop - b.start) for b in tiles])[:, None] for a in (V, K, Q))
+    # delta: the products, the weights' steps and v's parts of out
+    left = (G.abs() * ((wrow * seen) @ V.abs() + FLOOR * P @ tv)).sum(1, keepdim=True)
+    dSm = P * size
+    dSt = (rel + (3 + d / 2) * w + sums) * dSm + rel * dS.abs() + P * (parts + left)
+    out = {"out": (O, (rel + sums) * (P @ V.abs()) + (wrow * seen) @ V.abs() + FLOOR * (P @ tv)),
+           "dq": (scale * dS @ K, scale * ((dSt + own * seen) @ K.abs() + sums * (dSm @ K.abs()) + FLOOR * (dSm @ tk))),
+           "dk": (scale * dS.T @ Q, scale * ((dSt + key * seen).T @ Q.abs() + sums * (dSm.T @ Q.abs()) + FLOOR * (dSm.T @ tq))),
+           "dv": (P.T @ G, (rel * P).T @ G.abs() + sums * (P.T @ G.abs()) + (wcol * seen).T @ (G.abs() / big) + FLOOR * (P.T @ big))}
+    return {n: tuple(b.cpu().numpy()[:, None] for b in a) for n, a in out.items()}
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("what", ["v", "k", "vk", "q", "g"])
+@pytest.mark.parametrize("bits", [(25, 0, 0, 0), (0, 20, 0, 30), (0, 0, 30, 10), (-25, 0, -10, 0)])
+@pytest.mark.parametrize("scale", [1.0, 2.0])
+def test_tiles_of_very_different_size(cuda, dim, what, bits, scale):
+    """Tiles of 128 tokens whose values lie powers of two apart, under sharp weights: a row that hardly looks
+    at a tile of large values keeps its accuracy.  The size of k and q stands in a column where the other is 0."""
+    n = 450
+    x = _inputs(cuda, np.random.default_rng(31 + dim), ([n], 1, 1, dim, 0))
+    f = cuda.tensor([2.0 ** b for b in bits]).repeat_interleave(128)[:n, None]
+    x["k"][:, :, 0] = x["q"][:, :, 0] = 0
+    if "q" in what:
+        x["q"][:, :, 0] = f
+    if "k" in what:
+        x["k"][:, :, 0] = f
+    for name in set(what) & set("vg"):
+        x[name] *= f[:, :, None]
+    got, ref = _run_one(cuda, x, scale), _tiles_reference(cuda, x, scale)
+    for name in got:
+        _check(name, got[name], ref[name])
+
+
+def _run_one(torch, x, scale):
+    import rushlite_b200 as rsl
+
+    return _run(rsl, x, [len(x["q"])], scale)
+
+
 def test_rows_without_a_gradient(cuda):
     """Rows that a loss leaves out: their dq is 0, and they change nobody's results."""
     lengths = [200, 50, 60]
