@@ -279,10 +279,13 @@ void adamw_step(const std::vector<Variable>& params, const std::vector<Tensor>& 
       LMP_CHECK(seen.insert(x).second, "adamw_step: parameter " << i << " or its moments appear twice");
     ts.push_back(t);
   }
-  if (tensor::Graph* g = tensor::capturing_graph()) {  // the optimizer may go before its recorded step
+  if (tensor::Graph* g = tensor::capturing_graph()) {  // the optimizer and the gradients may go before the recorded step
     for (const auto* list : {&exp_avg, &exp_avg_sq})
       for (const Tensor& t : *list) g->keep(t.impl());
-    for (const Variable& p : params) g->keep(p.data().impl());
+    for (const Variable& p : params) {
+      g->keep(p.data().impl());
+      g->keep(p.grad().impl());
+    }
     g->keep(step.impl());
   }
   LMPB_OK_OR_THROW(lmpb_adamw((int)dt, ts.data(), (int)ts.size(), lr, beta1, beta2, eps, weight_decay,

@@ -15,7 +15,10 @@ class AdamW:
 
     Parameters are updated in place, so a training step with it can be
     recorded in a ``cuda.Graph``: the step count lives on the device and
-    advances with every replay (the rates are recorded as they were).  Every
+    advances with every replay (the rates are recorded as they were).  A
+    recorded step reads the gradients' memory as of its capture: record
+    ``zero_grad()`` and the backward with it, since ``zero_grad()`` outside
+    gives the parameters gradients that the recorded step does not see.  Every
     parameter must be a CUDA Variable of one dtype, float32 or float64, that
     requires a gradient; its moments have its dtype.  A parameter without
     a gradient from ``backward()`` takes a step with a gradient of 0.

@@ -136,6 +136,26 @@ def test_recorded_step_outlives_the_optimizer(cuda):
     assert all((j.numpy() == 1e9).all() for j in junk)
 
 
+@pytest.mark.parametrize("shape", [(300, 100), (5,)])
+def test_recorded_step_keeps_its_gradients(cuda, shape):
+    """A replay reads the gradients of the capture, also after zero_grad() gave the parameters others."""
+    import rushlite_b200 as rsl
+
+    rng = np.random.default_rng(8)
+    sets = [_random(rng, shape, "float32")]
+    opt, twin = _optimizer(rsl, sets, "float32"), _optimizer(rsl, sets, "float32")
+    graph = rsl.cuda.Graph()
+    with graph:
+        opt.step()
+    opt.zero_grad()
+    junk = [rsl.Variable(np.full(shape, 1e9, np.float32)) for _ in range(8)]  # over any memory given back
+    for _ in range(3):
+        graph.replay()
+        twin.step()
+    assert (opt.params[0].numpy() == twin.params[0].numpy()).all()
+    assert (opt.params[0].grad.numpy() == 0).all() and all((j.numpy() == 1e9).all() for j in junk)
+
+
 def test_special_values_stay_where_they_are(cuda):
     import rushlite_b200 as rsl
 
