@@ -78,34 +78,40 @@ bool floating(DataType d) { return d == DataType::Float32 || d == DataType::Floa
 
 // Where a kernel writes a gradient: straight into the gradient's own buffer
 // while that is the untouched zero (as gemm_accumulate does), else into a new
-// tensor that add() accumulates.
+// tensor that add() accumulates.  Without add(), as when the call fails, the
+// gradient is the zero that it was.
 class GradOut {
  public:
   explicit GradOut(Variable* v) : v_(v && v->requires_grad() ? v : nullptr) {
     if (!v_) return;
     const ImplPtr& gi = v_->grad_slot().impl();
-    direct_ = !v_->impl()->grad_shared && gi->device == DeviceType::CUDA && gi->dtype == v_->data().type() &&
-              gi->lazy && gi->lazy->kind == LazyNode::kConst && gi->lazy->p0 == 0.0;
-    if (direct_) {
+    if (!v_->impl()->grad_shared && gi->device == DeviceType::CUDA && gi->dtype == v_->data().type() &&
+        gi->lazy && gi->lazy->kind == LazyNode::kConst && gi->lazy->p0 == 0.0) {
       if (!gi->storage || gi->storage->bytes < gi->nbytes()) gi->storage = tensor::make_storage(gi->nbytes(), gi->device);
-      gi->lazy = nullptr;
+      zero_.swap(gi->lazy);  // taken: another place of the same Variable gets a tensor of its own
       t_ = Tensor(gi);
     } else {
       t_ = empty(v_->data().shape(), v_->data().type());
     }
+  }
+  GradOut(const GradOut&) = delete;
+  GradOut& operator=(const GradOut&) = delete;
+  ~GradOut() {
+    if (zero_) t_.impl()->lazy = zero_;
   }
   bool wanted() const { return v_ != nullptr; }
   void* get() const { return v_ ? ptr(t_) : nullptr; }
   // After the kernel that writes get() is queued.
   void add() {
     if (!v_) return;
-    if (!direct_) v_->incr_grad(t_);
-    else if (v_->impl()->grad_hook) v_->impl()->grad_hook();
+    if (!zero_) return v_->incr_grad(t_);
+    zero_ = nullptr;
+    if (v_->impl()->grad_hook) v_->impl()->grad_hook();
   }
 
  private:
   Variable* v_;
-  bool direct_ = false;
+  std::shared_ptr<LazyNode> zero_;  // what the gradient was, while its buffer is being written
   Tensor t_;
 };
 

@@ -197,3 +197,83 @@ def test_backward_from_a_given_gradient(cuda):
     assert (leaf.grad.numpy() == g + 2).all() and (seed.numpy() == g).all()
     with pytest.raises(RuntimeError, match="dtype"):
         leaf.backward(rsl.Variable(g, dtype=rsl.dtype.float64))
+
+
+_FAILING = r"""
+#include <dlfcn.h>
+#include <stdlib.h>
+#include "lmpb.h"
+static int calls;
+static void* real(const char* name) { return dlsym(dlopen(getenv("REAL_LMPB"), RTLD_NOW | RTLD_NOLOAD), name); }
+lmpb_status lmpb_attention_backward(const float* q, const float* k, const float* v, const float* out, const float* lse,
+                                    const float* grad, float* dq, float* dk, float* dv, int64_t tokens, int heads,
+                                    int kv_heads, int head_dim, float scale, lmpb_sequences s, void* stream) {
+  if (calls++ % 2 == 0) return LMPB_ERR_CUDA;
+  lmpb_status (*f)() = (lmpb_status (*)())real("lmpb_attention_backward");
+  return ((lmpb_status (*)(const float*, const float*, const float*, const float*, const float*, const float*, float*, float*,
+                           float*, int64_t, int, int, int, float, lmpb_sequences, void*))f)(
+      q, k, v, out, lse, grad, dq, dk, dv, tokens, heads, kv_heads, head_dim, scale, s, stream);
+}
+lmpb_status lmpb_layer_norm_backward(int dtype, const void* x, const void* w, const void* mean, const void* rstd,
+                                     const void* grad, int64_t rows, int64_t features, void* dx, void* dw, void* db,
+                                     void* stream) {
+  if (calls++ % 2 == 0) return LMPB_ERR_CUDA;
+  lmpb_status (*f)() = (lmpb_status (*)())real("lmpb_layer_norm_backward");
+  return ((lmpb_status (*)(int, const void*, const void*, const void*, const void*, const void*, int64_t, int64_t, void*,
+                           void*, void*, void*))f)(dtype, x, w, mean, rstd, grad, rows, features, dx, dw, db, stream);
+}
+"""
+
+_AFTER_FAILURE = r"""
+import numpy as np
+import rushlite_b200 as rsl
+
+def run(fail):
+    rng = np.random.default_rng(0)
+    q, k, v, g = (rsl.Variable(rng.standard_normal((50, 2, 8)).astype(np.float32), i < 3) for i in range(4))
+    x = rsl.Variable(rng.standard_normal((9, 40)).astype(np.float32), True)
+    w = rsl.Variable(rng.standard_normal(40).astype(np.float32), True)
+    b, gy = rsl.zeros([40], True), rsl.Variable(rng.standard_normal((9, 40)).astype(np.float32))
+    junk = [rsl.Variable(np.full((50, 2, 8), 1e9, np.float32)) for _ in range(8)]  # what fresh memory may hold
+    del junk
+    for make, seed in ((lambda: rsl.causal_attention(q, q, v, rsl.Sequences([50])), g),
+                       (lambda: rsl.causal_attention(q, k, v, rsl.Sequences([50])), g), (lambda: rsl.layer_norm(x, w, b), gy)):
+        for attempt in range(2):
+            try:
+                make().backward(seed)
+                assert attempt or not fail, "the call was to fail"
+                if not fail:
+                    break
+            except RuntimeError:
+                assert fail and attempt == 0
+    return [a.grad.numpy() for a in (q, k, v, x, w, b)]
+
+import os, sys
+np.save(sys.argv[2], np.concatenate([a.ravel() for a in run(sys.argv[1] == "fail")]))
+"""
+
+
+def test_gradients_after_a_failed_backward(cuda, tmp_path):
+    """A backward call that fails (a fake of the C entries returns an error
+    every other time) leaves the gradients as they were: tried again, it gives
+    what it gives without a failure."""
+    import os
+    import subprocess
+    import sys
+
+    from rushlite_b200 import capi
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    (tmp_path / "fake.c").write_text(_FAILING)
+    subprocess.run(["gcc", "-shared", "-fPIC", "-I", os.path.join(root, "include"), "-o", str(tmp_path / "fake.so"),
+                    str(tmp_path / "fake.c"), "-ldl"], check=True)
+    env = {**os.environ, "REAL_LMPB": os.path.abspath(capi.LIB_PATH), "PYTHONPATH": root}
+    got = {}
+    for what in ("pass", "fail"):
+        if what == "fail":
+            env["LD_PRELOAD"] = str(tmp_path / "fake.so")
+        r = subprocess.run([sys.executable, "-c", _AFTER_FAILURE, what, str(tmp_path / what)], env=env, cwd=root,
+                           capture_output=True, text=True, timeout=300)
+        assert r.returncode == 0, r.stderr[-2000:]
+        got[what] = np.load(str(tmp_path / what) + ".npy")
+    assert np.isfinite(got["pass"]).all() and (got["pass"] == got["fail"]).all()
