@@ -8,6 +8,12 @@ class LayerNorm(Module):
 
     def __init__(self, features: int, eps: float = 1e-5, bias: bool = True, device=None, dtype=None) -> None:
         super().__init__()
+        if features < 1:
+            raise ValueError("features must be at least 1")
+        if not 0 <= eps < float("inf"):
+            raise ValueError("eps must be finite and not negative")
+        if dtype is not None and dtype not in (_C.dtype.float32, _C.dtype.float64):
+            raise ValueError("LayerNorm computes in float32 or float64 only")
         kw = {}
         if device is not None:
             kw["device"] = device

@@ -75,3 +75,27 @@ def test_layers_check_their_arguments():
     for args in ((10, 3), (12, 0), (12, 4, 3), (12, 4, 0)):
         with pytest.raises(ValueError):
             layers.CausalSelfAttention(*args)
+
+
+def test_layers_refuse_what_they_cannot_compute():
+    import rushlite_b200 as rsl
+    from rushlite_b200.nets import layers
+
+    cpu = rsl.device.cpu  # construction alone needs no GPU
+    for kw in (dict(dtype=rsl.dtype.float64), dict(dtype=rsl.dtype.int32)):
+        with pytest.raises(ValueError, match="float32"):
+            layers.CausalSelfAttention(64, 4, device=cpu, **kw)
+    with pytest.raises(ValueError, match="multiple"):
+        layers.CausalSelfAttention(0, 4, device=cpu)
+    for args in ((1024, 4), (129, 1), (516, 4, 2)):
+        with pytest.raises(ValueError, match="128"):
+            layers.CausalSelfAttention(*args, device=cpu)
+    for args in ((512, 4), (128, 1), (64, 4, 2)):
+        for dtype in (None, rsl.dtype.float32):
+            layers.CausalSelfAttention(*args, device=cpu, dtype=dtype)
+    for kw in (dict(features=0), dict(features=8, eps=-1e-5), dict(features=8, eps=math.nan), dict(features=8, eps=math.inf),
+               dict(features=8, dtype=rsl.dtype.int64)):
+        with pytest.raises(ValueError):
+            layers.LayerNorm(**kw, device=cpu)
+    for dtype in (None, rsl.dtype.float32, rsl.dtype.float64):
+        layers.LayerNorm(8, 0.0, device=cpu, dtype=dtype)
