@@ -136,6 +136,12 @@ def test_forward_and_backward(cuda, case):
             assert np.linalg.norm(got[name] - ref[name][0]) <= 2.0 ** (-18 if name == "out" else -17) * norm, name
 
 
+def _results(x, lengths, scale=None):
+    import rushlite_b200 as rsl
+
+    return _run(rsl, x, lengths, scale)
+
+
 def _rows_reference(torch, x, lengths, scale):
     """As _reference, for gradients whose rows differ in size: what is left
     where terms are tiny counts against the largest term of the result's own
@@ -202,15 +208,17 @@ def _rows_reference(torch, x, lengths, scale):
     return {n: (a.cpu().numpy(), b.cpu().numpy()) for n, (a, b) in out.items()}
 
 
-@pytest.mark.parametrize("case", [([300], 2, 1, 64, 0), ([300], 2, 2, 128, 0), ([2049], 1, 1, 64, 0),
-                                  ([1000, 64, 64, 40, 40, 7], 2, 1, 33, 0), ([40] * 6 + [600], 4, 2, 96, 3)],
-                         ids=lambda c: "%s-%d" % ("_".join(map(str, c[0][:3])), c[3]))
+SMALL_ROWS = [(case, where) for case in (([300], 2, 1, 64, 0), ([300], 2, 2, 128, 0), ([2049], 1, 1, 64, 0),
+                                         ([1000, 64, 64, 40, 40, 7], 2, 1, 33, 0), ([40] * 6 + [600], 4, 2, 96, 3))
+              for where in ("every other row", "few large rows", "every other sequence")
+              if where != "every other sequence" or len(case[0]) > 1]
+
+
+@pytest.mark.parametrize("case,where", SMALL_ROWS, ids=lambda a: a if isinstance(a, str) else
+                         "%s-%d" % ("_".join(map(str, a[0][:3])), a[3]))
 @pytest.mark.parametrize("bits", [8, 14, 20, 26, 40, 80])
-@pytest.mark.parametrize("where", ["every other row", "every other sequence", "few large rows"])
-def test_rows_with_small_gradients(cuda, case, bits, where):
+def test_rows_with_small_gradients(cuda, case, where, bits):
     """A row whose gradient is far below its neighbours' keeps its own accuracy, alone and where sequences share a tile."""
-    if where == "every other sequence" and len(case[0]) == 1:
-        pytest.skip("one sequence")
     lengths, hq, _, d, tail = case
     x = _inputs(cuda, np.random.default_rng(bits + d), case)
     t = sum(lengths)
@@ -221,7 +229,7 @@ def test_rows_with_small_gradients(cuda, case, bits, where):
     else:
         small = np.concatenate([np.full(n, i % 2 == 1) for i, n in enumerate(lengths)])
     x["g"][:t][cuda.from_numpy(small)] *= 2.0 ** -bits
-    got = _gradients(cuda, x, lengths)
+    got = _results(x, lengths)
     ref = _rows_reference(cuda, {n: a[:t] for n, a in x.items()}, lengths, 1 / math.sqrt(d))
     for name in ("dq", "dk", "dv"):
         _check(name, got[name][:t], ref[name])
@@ -235,12 +243,6 @@ def test_rows_with_small_gradients(cuda, case, bits, where):
             assert np.linalg.norm(err) <= 2.0 ** -17 * np.linalg.norm(value), name
 
 
-def _gradients(torch, x, lengths, scale=None):
-    import rushlite_b200 as rsl
-
-    return _run(rsl, x, lengths, scale)
-
-
 @pytest.mark.parametrize("dim", [64, 128])
 def test_sequences_of_very_different_gradients_share_a_tile(cuda, dim):
     lengths = [31, 30, 33, 34, 200]
@@ -249,7 +251,7 @@ def test_sequences_of_very_different_gradients_share_a_tile(cuda, dim):
     for n, f in zip(lengths, (1.0, 1e-6, 1e-10, 1e-13, 1e-20)):
         x["g"][start:start + n] *= f
         start += n
-    got = _gradients(cuda, x, lengths)
+    got = _results(x, lengths)
     ref = _rows_reference(cuda, x, lengths, 1 / math.sqrt(dim))
     start = 0
     for name in ("dq", "dk", "dv"):
@@ -269,7 +271,7 @@ def test_small_gradients_with_sharp_weights(cuda, dim, bits):
     lengths = [500, 60, 60]
     x = _inputs(cuda, np.random.default_rng(5 + dim), (lengths, 2, 1, dim, 0))
     x["g"][::2] *= 2.0 ** -bits
-    got = _gradients(cuda, x, lengths, 1.0)
+    got = _results(x, lengths, 1.0)
     ref = _rows_reference(cuda, x, lengths, 1.0)
     for name in ("dq", "dk", "dv"):
         _check(name, got[name], ref[name])
@@ -342,15 +344,9 @@ def test_tiles_of_very_different_size(cuda, dim, what, bits, scale):
         x["k"][:, :, 0] = f
     for name in set(what) & set("vg"):
         x[name] *= f[:, :, None]
-    got, ref = _run_one(cuda, x, scale), _tiles_reference(cuda, x, scale)
+    got, ref = _results(x, [n], scale), _tiles_reference(cuda, x, scale)
     for name in got:
         _check(name, got[name], ref[name])
-
-
-def _run_one(torch, x, scale):
-    import rushlite_b200 as rsl
-
-    return _run(rsl, x, [len(x["q"])], scale)
 
 
 def test_rows_without_a_gradient(cuda):
@@ -361,7 +357,7 @@ def test_rows_without_a_gradient(cuda):
     out = np.arange(310) % 3 != 0
     x["g"][cuda.from_numpy(out)] = 0
     x["g"][250:] = 0  # a whole sequence
-    got = _gradients(cuda, x, lengths)
+    got = _results(x, lengths)
     ref = _rows_reference(cuda, x, lengths, 1 / 8)
     for name in ("dq", "dk", "dv"):
         _check(name, got[name], ref[name])
@@ -724,6 +720,34 @@ def test_unaligned_buffers_through_the_c_entry(cuda):
     for n, b in outs.items():
         _check(n, b[1:-1].cpu().numpy().reshape(ref[n][0].shape), ref[n])
         assert b[0] == 7 and b[-1] == 7, n
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(16400, 16400), (32768, 16384)])
+def test_more_heads_than_the_tensor_core_kernels_take(cuda, heads, kv_heads):
+    """The plain fp32 kernels on their own; some groups of heads against the formula."""
+    lengths, dim, group = [41, 1, 0, 70], 3, heads // kv_heads
+    x = _inputs(cuda, np.random.default_rng(33), (lengths, heads, kv_heads, dim, 2))
+    got = _results(x, lengths)
+    for j in (0, 1, 8191, kv_heads - 1):
+        h = slice(j * group, (j + 1) * group)
+        part = {"q": x["q"][:, h], "k": x["k"][:, j:j + 1], "v": x["v"][:, j:j + 1], "g": x["g"][:, h]}
+        ref = _reference(cuda, part, lengths)
+        for name in got:
+            _check(name, got[name][:, h if name in ("out", "dq") else slice(j, j + 1)], ref[name])
+
+
+def test_plain_fp32_kernels_on_every_case(cuda):
+    """The cases above, in a process that takes the plain fp32 kernels for all of them."""
+    import os
+    import subprocess
+    import sys
+
+    names = ("test_forward_and_backward or test_scale or test_rows_with_small_gradients or test_scores_far_apart "
+             "or test_repeats_to_the_bit or test_tiles_of_very_different_size or does_not_see")
+    r = subprocess.run([sys.executable, "-m", "pytest", "-m", "gpu", "-x", "-q", "-p", "no:cacheprovider", "-k", names,
+                        os.path.abspath(__file__)], env={**os.environ, "LMPB_ATTENTION": "simt"}, capture_output=True,
+                       text=True, timeout=600)
+    assert r.returncode == 0 and " passed" in r.stdout, r.stdout[-3000:]
 
 
 def test_refusals(cuda):
