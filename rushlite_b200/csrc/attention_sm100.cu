@@ -1024,7 +1024,7 @@ __device__ __forceinline__ int shares_of(const AttentionArgs& a, int per_head) {
 // [256, 256 + DP) and [384, 384 + DP).  The MMAs of a block run scores, dP,
 // dv, dk: weights are computed under dP, dS under dv.
 //
-// Both running sums are held in registers, 2 x DP / 2 a thread.
+// Both running sums are held in registers, 2 x DP / PARTS a thread.
 template <int DP>
 __device__ __forceinline__ void dkv_tile(const AttentionArgs& a, const Split& sp, int cta, bool vec_out) {
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -1107,8 +1107,17 @@ __device__ __forceinline__ void dkv_tile(const AttentionArgs& a, const Split& sp
       last(done, 0);
     } else if (warp == 2) {
       // dS has one bound for all queries of a block.  Where it comes from outputs, and deltas, far above
-      // these keys' v, a query with a small delta could lose its bits: a case for the fp32 kernels.
-      const float vnorm = sp.norm[vblock];
+      // these keys' v (all 0: the sequence's least), a query with a small delta could lose its bits: a
+      // case for the fp32 kernels.
+      float vnorm = sp.norm[vblock];
+      if (!(vnorm > 0.f)) {
+        vnorm = INFINITY;
+#pragma unroll 1
+        for (int k = (tile.y + kTileRows - 1) / kTileRows; k-- > 0;) {
+          const float x = sp.norm[vblock - t + first_tile(tile, t) + k];
+          if (x > 0.f) vnorm = fminf(vnorm, x);
+        }
+      }
       bool far = false;
 #pragma unroll 1
       for (int i = threadIdx.x & 31; i < n; i += 32) {

@@ -297,6 +297,7 @@ def _tiles_reference(torch, x, scale):
     big = G.abs().amax(1, keepdim=True)
     full = lambda: torch.zeros(n, n, dtype=torch.float64, device="cuda")  # noqa: E731
     e, own, key, wrow, wcol, parts = full(), full(), full(), full(), full(), full()
+    least = min(float(V[c].norm(dim=1).max()) or math.inf for c in tiles)
     for c in tiles:
         kt, vt, vn = float(K[c].abs().max()), float(V[c].abs().max()), float(V[c].norm(dim=1).max())
         top = P[:, c].amax(1, keepdim=True)
@@ -309,7 +310,7 @@ def _tiles_reference(torch, x, scale):
             ratio = float((delta[r].abs() / big[r]).max())
             T = (P[r, c] * big[r]).amax(0)
             wcol[r, c] = 2.0 ** -37 * T
-            if ratio <= 2.0 ** 19 * math.sqrt(d) * vn:  # else the fp32 kernels' result
+            if ratio <= 2.0 ** 19 * math.sqrt(d) * (vn or least):  # else the fp32 kernels' result
                 key[r, c] = 2.0 ** -36 * (math.sqrt(d) * vn + ratio) * T
     E = (3 + d / 2) * w * scale * (Q.abs() @ K.abs().T) + scale * e
     rel = 2 * E.masked_fill(~mask, 0).amax(1, keepdim=True) + w * (lse.abs() / 2 + 2)
@@ -345,6 +346,18 @@ def test_tiles_of_very_different_size(cuda, dim, what, bits, scale):
     for name in set(what) & set("vg"):
         x[name] *= f[:, :, None]
     got, ref = _results(x, [n], scale), _tiles_reference(cuda, x, scale)
+    for name in got:
+        _check(name, got[name], ref[name])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("sizes", [(1.0, 0.0, 1.0, 1.0), (0.0, 1.0, 0.0, 2.0 ** -25), (2.0 ** 22, 0.0, 1.0, 1.0)])
+def test_tiles_without_values(cuda, dim, sizes):
+    """Tiles of 128 tokens whose v is 0, as a program that masks keys may leave them."""
+    n = 500
+    x = _inputs(cuda, np.random.default_rng(35 + dim), ([n], 1, 1, dim, 0))
+    x["v"] *= cuda.tensor(sizes).repeat_interleave(128)[:n, None, None]
+    got, ref = _results(x, [n], 1.0), _tiles_reference(cuda, x, 1.0)
     for name in got:
         _check(name, got[name], ref[name])
 
