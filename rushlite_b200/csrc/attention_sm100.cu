@@ -21,7 +21,7 @@
 // block: next to values far apart a small weight counts as much as a large one.
 //
 // Tiles whose values that cannot carry (infinities, NaN, q, k or v with rows
-// over 2^18 apart or magnitudes below 2^-60, magnitudes over 2^40, q or k so
+// over 2^18 apart or magnitudes below 2^-60, grad below 2^-110, magnitudes over 2^40, q or k so
 // long that a score may pass 2^14, where the rounding of lse moves a weight by
 // 2^-10; in the backward also outputs over 2^18 above a tile of v that their
 // rows see) are flagged by the split and the backward; the fp32 kernels of
@@ -93,8 +93,7 @@ struct Split {
   unsigned char* flags;
   int* row_expo;         // [heads, tokens]: grad's row was scaled by 2^row_expo; kZeroRow where it is 0
 };
-// Rows of grad below 2^-95 keep this scale and fewer bits: results are then about to underflow.
-constexpr int kMaxRowExpo = 110, kZeroRow = 127;
+constexpr int kMaxRowExpo = 110, kZeroRow = 127;  // rows of grad below 2^-110, which this would not carry, are flagged
 
 // ------------------------------------------------------------ split pass
 
@@ -257,7 +256,7 @@ __global__ void __launch_bounds__(32 * split_warps<DP>(), 2048 / (64 * split_war
     nrm = fmaxf(nrm, red[2][w]);
     dmx = fmaxf(dmx, red[3][w]);
   }
-  const bool range = mx > 0x1p40f || (!is_g && mx > 0.f && (mx < 0x1p-60f || mn < mx * 0x1p-18f));
+  const bool range = mx > 0x1p40f || (is_g ? mn < 0x1p-110f : mx > 0.f && (mx < 0x1p-60f || mn < mx * 0x1p-18f));
   const bool far = !is_v && !is_g && !(nrm * a.scale <= 0x1p14f);  // so |q| |k| scale <= 2^14 of unflagged tiles
   const bool flag = bads || range || far;
   const int e = flag || is_g ? 0 : row_exp(mx);

@@ -362,6 +362,18 @@ def test_tiles_without_values(cuda, dim, sizes):
         _check(name, got[name], ref[name])
 
 
+@pytest.mark.parametrize("size", [1e-30, 1e-33, 1e-35, 1e-37])
+def test_gradients_next_to_underflow(cuda, size):
+    """The bar of test_forward_and_backward where the results' own steps, 2^-149, still pass it."""
+    lengths = [40, 40, 40]
+    x = _inputs(cuda, np.random.default_rng(36), (lengths, 2, 1, 64, 0))
+    x["g"] *= size
+    got, ref = _results(x, lengths), _reference(cuda, x, lengths)
+    for name in ("dq", "dk", "dv"):
+        want = ref[name][0]
+        assert np.linalg.norm((got[name] - want) / size) <= 2.0 ** -17 * np.linalg.norm(want / size), name
+
+
 def test_rows_without_a_gradient(cuda):
     """Rows that a loss leaves out: their dq is 0, and they change nobody's results."""
     lengths = [200, 50, 60]
