@@ -12,6 +12,13 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA GPU (B200, sm_100a)")
 
 
+def pytest_collection_modifyitems(items):
+    """The tests of the reference's own front-end, whose build needs its source
+    tree, come last: where that is missing, a run that stops at the first
+    failure has been through everything else."""
+    items.sort(key=lambda item: item.path.name == "test_lamp3_front_gpu.py")
+
+
 @pytest.fixture(scope="session")
 def cuda():
     """torch with a CUDA device; GPU tests fail loudly if the kernels are missing."""
