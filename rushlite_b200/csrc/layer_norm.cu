@@ -458,8 +458,10 @@ lmpb_status backward(const void* x, const void* w, const void* mean, const void*
   const bool warps = by_warps<T>(rows, F);
   // as many CTAs as fit at once, two where resident() allows ([2048, 4096] double: 42 us, 47.5 with twice the CTAs)
   const int fit = F > (warps ? 2048 / (int)sizeof(T) : sizeof(T) == 8 ? 1024 : 4096) ? 1 : 2;
-  // a few rows: one CTA, whose sums over rows are the results (32 x 256: one launch instead of two)
-  const unsigned grid = !lng && rows * F <= 8192 ? 1 : grid_of(rows, warps ? kThreads / 32 : 1, fit);
+  // a few rows, 8 an owner (warp or CTA): one CTA, whose sums over rows are the results, and one launch instead of
+  // two (us: [32, 256] 6.0 and 6.8, [64, 64] 6.1 and 7.0; more rows wait on one another: [128, 64] 8.3 and 6.9,
+  // [512, 16] 23 and 6.9, [8192, 1] 354 and 10.3)
+  const unsigned grid = !lng && rows * F <= 8192 && rows <= (warps ? 64 : 8) ? 1 : grid_of(rows, warps ? kThreads / 32 : 1, fit);
   const bool table = columns && (lng || grid > 1);
   const int64_t chunk = std::max<int64_t>(32, (rows + 63) / 64);
   const int prows = lng ? (int)((rows + chunk - 1) / chunk) : (int)grid;

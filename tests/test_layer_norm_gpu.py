@@ -74,6 +74,13 @@ def test_forward_and_backward(cuda, rows, features, dtype):
             _check("db", vb.grad.numpy(), ref["db"], HALF[dtype])
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("rows,features", [(64, 64), (65, 64), (512, 16), (8192, 1), (1000, 8), (8, 1024), (9, 900)])
+def test_few_and_many_narrow_rows(cuda, rows, features, dtype):
+    """Both sides of where one CTA takes all rows."""
+    test_forward_and_backward(cuda, rows, features, dtype)
+
+
 def test_dimensions_before_the_last_are_rows(cuda):
     import rushlite_b200 as rsl
 
