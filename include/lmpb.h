@@ -335,10 +335,11 @@ lmpb_status lmpb_sequences_release(lmpb_sequences handle);
  * lse is what the backward wants back.  Tokens behind the last sequence get 0
  * (their lse is not written) and are not read.  head_dim <= 128, heads a
  * multiple of kv_heads, 0 < scale <= 2^64.  Products are fp32-accurate on the
- * tensor cores; sequences and head groups whose values these cannot carry
+ * tensor cores (operands of 22 bits, each row of a result against what is
+ * added into it); sequences and head groups whose values these cannot carry
  * (infinities, NaN, scores past 2^14, rows of q, k or v over 2^18 apart within 128 tokens;
  * in the backward also outputs over 2^18 above the v of 128 tokens that they come from)
- * are computed in plain fp32, several times slower.  A value that a row does
+ * are computed in plain fp32, 15 to 30 times slower.  A value that a row does
  * not see never reaches it, whatever it is. */
 lmpb_status lmpb_attention(const float* q, const float* k, const float* v, float* out, float* lse, int64_t tokens,
                            int heads, int kv_heads, int head_dim, float scale, lmpb_sequences sequences,

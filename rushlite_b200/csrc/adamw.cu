@@ -8,7 +8,7 @@
 // Bound: HBM.  Every value is read once (p, g, m, v) and written once (p, m,
 // v): 28 bytes in float32.  All tensors of a step go through one launch: the
 // table of their addresses travels in the kernel's parameters, so a captured
-// graph holds it by value, and a CTA finds its chunk of 4096 values by a
+// graph holds it by value, and a CTA finds its chunk of 16 KB of values by a
 // binary search in the table's running chunk count.
 //
 // The step count lives on the device, so that a recorded step counts its own

@@ -18,7 +18,8 @@
 // grids hold.  Masked positions never enter a sum, so a NaN or infinity in a
 // row that a query does not see does not reach it.  Bound: FFMA and the
 // shared-memory loads that feed it, [16384] x 8 heads (2) of 128: forward
-// 16 ms, backward 65, against 1.15 and 4.7 on the tensor cores.
+// 16 ms, backward 65, against 1.15 and 4.8 on the tensor cores; 36 and 81 for
+// flagged sequences, as that launch is one CTA an SM.
 #include <cuda_runtime.h>
 
 #include <algorithm>

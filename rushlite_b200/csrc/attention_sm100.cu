@@ -146,7 +146,7 @@ __device__ __forceinline__ float two_to(int e) { return __int_as_float((e + 127)
 // one of two rows (DP = 64).  Bound by HBM and, one tile a CTA, by latency:
 // 32 warps an SM are needed ([1500, 31, 700, 1, 1865] x 24 planes of 128: 27
 // us with 16 rows a warp, 25 with 8; 40 planes of the backward: 64 and 50;
-// with fold_rows in place of a tree for each row then 21 and 45).
+// with fold_rows in place of a tree for each row then 22 and 46).
 template <int DP>
 constexpr int split_warps() { return DP / 8; }
 
@@ -542,8 +542,9 @@ struct Warps {
 using Warps8 = Warps<8, 168, 88, 208>;
 using Warps16 = Warps<16, 96, 64, 104>;
 // With DP = 64, where the weights' arithmetic weighs as much as the MMAs, 16
-// warps ([8192] x 16 heads: forward 0.390 ms, backward 1.55; 8 warps 0.44 and
-// 1.63; a forward of two pipelines of 8 that take the key blocks in turn 0.42).
+// warps (backward of [8192] x 16 heads (4) 1.65 ms, of [1024] x 4 x 8 heads (2) 89 us, with 8
+// warps 1.68 and 97; forward 0.392 ms and 33.0 us, with 8 warps 0.382 and 31.1;
+// a forward of two pipelines of 8 that take the key blocks in turn 0.42).
 // With DP = 128, where the MMAs outweigh it, 8 warps of twice the registers.
 template <int DP>
 using WarpsOf = std::conditional_t<DP == 64, Warps16, Warps8>;
@@ -1398,13 +1399,12 @@ bool attention_fits_sm100(const AttentionArgs& a) {
 // after the others (one key/value head, or a long sequence): five quarters of
 // what an SM gets on average, as dq's CTAs fill what is left, and 2 blocks
 // for what starting a CTA and joining the shares cost.  Backward, us:
-//                                             2 + 1.25   2 + 1   3 + 1.25   at least 8, 1.5
-//   [300] x 4 heads (1) of 64                    28        28       31          50
-//   [2500] x 4 (1) of 64                         75        82       74          87
-//   [1024] x 4, 8 (2) of 64                      86        91       89          92
-//   [600, 300, 900] x 12 (1) of 128             102       102      103         130
-//   [1500, 31, 700, 1, 1865] x 16 (4) of 128    310       319      309         319
-// (the last column with a slower join than now)
+//                                             2 + 1.25   2 + 1   3 + 1.25
+//   [300] x 4 heads (1) of 64                    28        28       32
+//   [2500] x 4 (1) of 64                         78        84       77
+//   [1024] x 4, 8 (2) of 64                      89        94       93
+//   [600, 300, 900] x 12 (1) of 128             102       102      104
+//   [1500, 31, 700, 1, 1865] x 16 (4) of 128    320       328      318
 void cut_dkv(AttentionArgs& a) {
   const int64_t group = a.heads / a.kv_heads, most = a.longest_tiles * group;
   const double average = (double)a.pair_tiles * a.heads / sm_count();

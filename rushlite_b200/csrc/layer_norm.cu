@@ -45,7 +45,7 @@ __device__ __forceinline__ T warp_sum(T v) {
 }
 
 // Sum over the TPR threads of a row, returned to all of them.  For a whole
-// CTA, `red` is two alternating buffers of 8 partials per value (`phase`
+// CTA, `red` is two alternating buffers of a partial a warp per value (`phase`
 // flips), so one barrier per call is enough: a thread can only reach the
 // buffer again two barriers later.
 template <typename T, int TPR, int N>
@@ -257,7 +257,8 @@ __global__ void __launch_bounds__(block_of(TPR), resident<T, NV * VEC, TPR>())
 
 // out[c] = sum over the table's rows of column c: 32 columns a CTA, 32 row
 // lanes folded in order (8 lanes of four times the rows waited 13 us for
-// [296, 2 x 4096], these 6.5).  It starts under the last rows' CTAs: 2.5 us less.  Columns [0, F) go to dw, [F, 2F) to db.
+// [296, 2 x 4096], these 6.5).  It is launched while the rows' CTAs run and starts as the last one ends: 2.5 us less.
+// Columns [0, F) go to dw, [F, 2F) to db.
 template <typename T>
 __global__ void __launch_bounds__(1024)
     fold_kernel(const T* part, int rows, int F, T* dw, T* db) {
