@@ -338,7 +338,8 @@ lmpb_status lmpb_sequences_release(lmpb_sequences handle);
  * tensor cores (operands of 22 bits, each row of a result against what is
  * added into it); sequences and head groups whose values these cannot carry
  * (infinities, NaN, scores past 2^14, rows of q, k or v over 2^18 apart within 128 tokens;
- * in the backward also outputs over 2^18 above the v of 128 tokens that they come from)
+ * in the backward also rows of v, or outputs above them, and rows of q or k that are
+ * together over 2^18 apart)
  * are computed in plain fp32, 15 to 30 times slower.  A value that a row does
  * not see never reaches it, whatever it is. */
 lmpb_status lmpb_attention(const float* q, const float* k, const float* v, float* out, float* lse, int64_t tokens,

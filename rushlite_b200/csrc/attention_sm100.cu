@@ -23,9 +23,10 @@
 // Tiles whose values that cannot carry (infinities, NaN, q, k or v with rows
 // over 2^18 apart or magnitudes below 2^-60, grad below 2^-110, magnitudes over 2^40, q or k so
 // long that a score may pass 2^14, where the rounding of lse moves a weight by
-// 2^-10; in the backward also outputs over 2^18 above a tile of v that their
-// rows see) are flagged by the split and the backward; the fp32 kernels of
-// attention.cu then redo the sequences and head groups that hold one.
+// 2^-10; in the backward also rows of v, or outputs above them, and rows of q
+// or k that are together over 2^18 apart) are flagged by the split and the
+// backward; the fp32 kernels of attention.cu then redo the sequences and head
+// groups that hold one.
 //
 // 1. Split pass: a CTA per tile and head plane writes the tile's hi and lo as
 //    one block in the very layout the MMAs read from shared memory (128-byte
@@ -90,9 +91,14 @@ struct Split {
   int* expo;             // the tile was scaled by 2^expo (q, k, v)
   float* norm;           // largest row norm (v; grad: of the scaled rows)
   float* dmax;           // largest |delta| of the scaled rows (grad)
+  int* span;             // the tile's rows lie within 2^span (q, k, v)
   unsigned char* flags;
   int* row_expo;         // [heads, tokens]: grad's row was scaled by 2^row_expo; kZeroRow where it is 0
 };
+// By how many powers of two, together, two operands of a product may exceed
+// what the row of a result takes most of its sum from: the halves' step,
+// 2^-39 of the largest, is then 2^-21 of that.
+constexpr int kMaxSpan = 18;
 constexpr int kMaxRowExpo = 110, kZeroRow = 127;  // rows of grad below 2^-110, which this would not carry, are flagged
 
 // ------------------------------------------------------------ split pass
@@ -263,6 +269,7 @@ __global__ void __launch_bounds__(32 * split_warps<DP>(), 2048 / (64 * split_war
   const int64_t block = plane * a.tiles + t;
   if (threadIdx.x == 0) {
     o.expo[block] = e;
+    o.span[block] = mx > 0.f ? row_exp(mn) - row_exp(mx) : 0;
     o.flags[block] = flag;
     if (is_v || is_g) {
       o.norm[block] = sqrtf(nrm) * 1.0001f;  // rounded sums: never below the norm
@@ -921,6 +928,11 @@ __device__ __forceinline__ void dq_tile(const AttentionArgs& a, const Split& sp,
     Waiter last(33);
     commit(done);
     last(done, 0);
+    } else if (warp == 2) {  // dS follows the size of v and is multiplied by k: both far apart are a case for the fp32 kernels
+      bool far = false;
+#pragma unroll 1
+      for (int j = threadIdx.x & 31; j < n; j += 32) far |= sp.span[kplane + j] + sp.span[vplane + j] > kMaxSpan;
+      if (far) sp.flags[qblock] = 1;
     }
   } else {
     W::many();
@@ -1106,9 +1118,10 @@ __device__ __forceinline__ void dkv_tile(const AttentionArgs& a, const Split& sp
       commit(done);
       last(done, 0);
     } else if (warp == 2) {
-      // dS has one bound for all queries of a block.  Where it comes from outputs, and deltas, far above
-      // these keys' v (all 0: the sequence's least), a query with a small delta could lose its bits: a
-      // case for the fp32 kernels.
+      // dS has one bound for all queries of a block, and is multiplied by q.  Where the bound comes from
+      // larger rows of v, or from outputs, and deltas, far above these keys' v (all 0: the sequence's
+      // least), and q lies apart too, a query with a small q and dS could lose its bits: a case for the
+      // fp32 kernels.
       float vnorm = sp.norm[vblock];
       if (!(vnorm > 0.f)) {
         vnorm = INFINITY;
@@ -1121,8 +1134,9 @@ __device__ __forceinline__ void dkv_tile(const AttentionArgs& a, const Split& sp
       bool far = false;
 #pragma unroll 1
       for (int i = threadIdx.x & 31; i < n; i += 32) {
-        const int64_t gb = (int64_t)(kv_head * group + (first + i) / per_head) * a.tiles + t + (first + i) % per_head + gplanes;
-        far |= sp.dmax[gb] > 0x1p18f * sp.norm[gb] * vnorm;
+        const int64_t qb = (int64_t)(kv_head * group + (first + i) / per_head) * a.tiles + t + (first + i) % per_head, gb = qb + gplanes;
+        const float gv = sp.norm[gb] * vnorm;
+        far |= sp.dmax[gb] + gv > two_to(kMaxSpan - sp.span[qb] - sp.span[vblock]) * gv;
       }
       if (far) sp.flags[kblock] = 1;
     }
@@ -1341,13 +1355,14 @@ lmpb_status make_split(AttentionArgs& a, bool backward, int dp, Split& s, float*
   const size_t blocks = n * (dp == 64 ? block_bytes<64>() : block_bytes<128>());
   const size_t dbytes = backward ? up((size_t)a.tokens * a.heads * 4) : 0;  // of delta, and of the rows' exponents
   const size_t pbytes = a.splits > 1 ? (size_t)a.splits * 2 * a.tokens * a.kv_heads * a.dim * 4 : 0;
-  LMPB_CUDA_TRY(stream_alloc(ws, blocks + 3 * up(4 * n) + up(n) + 2 * dbytes + pbytes, st));
+  LMPB_CUDA_TRY(stream_alloc(ws, blocks + 4 * up(4 * n) + up(n) + 2 * dbytes + pbytes, st));
   unsigned char* p = static_cast<unsigned char*>(*ws);
   s.blocks = p;
   s.expo = reinterpret_cast<int*>(p + blocks);
   s.norm = reinterpret_cast<float*>(p + blocks + up(4 * n));
   s.dmax = reinterpret_cast<float*>(p + blocks + 2 * up(4 * n));
-  s.flags = p + blocks + 3 * up(4 * n);
+  s.span = reinterpret_cast<int*>(p + blocks + 3 * up(4 * n));
+  s.flags = p + blocks + 4 * up(4 * n);
   *delta = reinterpret_cast<float*>(s.flags + up(n));
   s.row_expo = reinterpret_cast<int*>(s.flags + up(n) + dbytes);
   if (pbytes) a.part = reinterpret_cast<float*>(s.flags + up(n) + 2 * dbytes);

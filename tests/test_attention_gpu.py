@@ -362,6 +362,38 @@ def test_tiles_without_values(cuda, dim, sizes):
         _check(name, got[name], ref[name])
 
 
+@pytest.mark.parametrize("dim", [33, 64, 128])
+@pytest.mark.parametrize("bits", [dict(v=16, k=10), dict(v=14, k=14), dict(v=16, q=10), dict(v=12, q=16), dict(v=15, q=10, k=10)],
+                         ids=lambda b: "-".join(n + str(a) for n, a in b.items()))
+def test_two_operands_with_rows_far_apart(cuda, dim, bits):
+    """A gradient's weight follows the size of v and is multiplied by q or k.  Where rows of both differ, terms of
+    small rows stand next to large ones of little weight.  Each row against the magnitudes of its terms: the roundings
+    of scores (up to 60 here, 2^-24 of them twice) move weights by 2^-17 at most, and sums average out: 2^-16."""
+    lengths = [5, 20, 50, 33, 20, 12, 48, 47, 70, 9, 60, 60, 41, 80, 128, 200, 300] * 4
+    t = sum(lengths)
+    x = _inputs(cuda, np.random.default_rng(37 + dim), (lengths, 2, 1, dim, 0))
+    for name, b in bits.items():
+        x[name] *= 2.0 ** -(b * (cuda.arange(t) % 2).float())[:, None, None]
+    scale = float(np.float32(10 / math.sqrt(dim)))
+    got = _results(x, lengths, scale)
+    ref = _reference(cuda, x, lengths, scale)
+    x = {n: a.cuda().double() for n, a in x.items()}
+    size = {"dq": cuda.zeros_like(x["q"]), "dk": cuda.zeros_like(x["k"])}
+    start = 0
+    for n in lengths:
+        r = slice(start, start + n)
+        start += n
+        for h in range(2):
+            Q, K, V, G = x["q"][r, h], x["k"][r, 0], x["v"][r, 0], x["g"][r, h]
+            P = (scale * Q @ K.T).masked_fill(~cuda.ones(n, n, dtype=cuda.bool, device="cuda").tril(), -math.inf).softmax(1)
+            A = scale * P * (G.abs() @ V.abs().T + (G.abs() * (P @ V.abs())).sum(1, keepdim=True))
+            size["dq"][r, h] = A @ K.abs()
+            size["dk"][r, 0] += A.T @ Q.abs()
+    for name in size:
+        off = np.linalg.norm(got[name] - ref[name][0], axis=-1) / size[name].norm(dim=-1).cpu().numpy()
+        assert off.max() <= 2.0 ** -16, (name, off.argmax(), math.log2(off.max()))
+
+
 @pytest.mark.parametrize("size", [1e-30, 1e-33, 1e-35, 1e-37])
 def test_gradients_next_to_underflow(cuda, size):
     """The bar of test_forward_and_backward where the results' own steps, 2^-149, still pass it."""
