@@ -337,11 +337,12 @@ lmpb_status lmpb_sequences_release(lmpb_sequences handle);
  * multiple of kv_heads, 0 < scale <= 2^64.  Products are fp32-accurate on the
  * tensor cores (operands of 22 bits, each row of a result against what is
  * added into it); sequences and head groups whose values these cannot carry
- * (infinities, NaN, scores past 2^14, rows of q, k or v over 2^18 apart within 128 tokens;
- * in the backward also rows of v, or outputs above them, and rows of q or k that are
- * together over 2^18 apart)
- * are computed in plain fp32, 15 to 30 times slower.  A value that a row does
- * not see never reaches it, whatever it is. */
+ * (infinities, NaN, values over 2^40, scores past 2^14; within 128 tokens rows
+ * of q, k or v over 2^18 apart, or none over 2^-60; in the backward also rows
+ * of v, or outputs above them, and rows of q or k that are together over 2^18
+ * apart, and gradient rows under 2^-110) are computed in plain fp32, 15 to 30
+ * times slower.  A value that a row does not see never reaches it, whatever it
+ * is. */
 lmpb_status lmpb_attention(const float* q, const float* k, const float* v, float* out, float* lse, int64_t tokens,
                            int heads, int kv_heads, int head_dim, float scale, lmpb_sequences sequences,
                            void* stream);
